@@ -20,6 +20,7 @@ DEFAULT_LIB = os.path.join(_PKG, "libhyacin.so")
 # hyacinPrecision_t
 F64, F64_COMPLEX, F32, F32_COMPLEX, F16, F16_COMPLEX, DD, DD_COMPLEX, TF, TF_COMPLEX, QF, QF_COMPLEX = range(12)
 ELEM_BYTES = [8, 16, 4, 8, 2, 4, 16, 32, 12, 24, 16, 32]
+BF16 = 32            # HYACIN_B200_BF16: taken by the 4-bit weight and distillation entry points only
 
 PUBLIC_SYMBOLS = [
     "hyacinCreate", "hyacinDestroy", "hyacinInterpolateFit", "hyacinTsvdFit", "hyacinTsvdFitSegmentN",
@@ -32,7 +33,7 @@ B200_SYMBOLS = [
     "hyacinB200GramResidues", "hyacinB200Reconstruct", "hyacinB200LaunchCount", "hyacinB200ProfileEnable",
     "hyacinB200ProfileRead", "hyacinB200SlicePlan", "hyacinB200HerkBatchStatic", "hyacinB200QuantizeLimbs", "hyacinB200GramLimbs",
     "hyacinB200DequantizeViaSlices", "hyacinB200ProfileReadTail", "hyacinB200PivotedCholesky", "hyacinB200SelfTestWait", "hyacinB200VectorRange",
-    "hyacinB200GramItem",
+    "hyacinB200GramItem", "hyacinB200QuantizeW4", "hyacinB200ProductW4", "hyacinB200DistillLoss", "hyacinB200DistillGrad",
 ]
 
 
@@ -94,6 +95,10 @@ def load(path: str | None = None) -> ctypes.CDLL:
         "hyacinB200SelfTestWait": (i32, [H, c_uint32, c_uint32]),
         "hyacinB200PivotedCholesky": (i32, [H, f64, i32, i32, i32, vp, i32, vp, vp, i32]),
         "hyacinB200GramItem": (i32, [i32, i32, i32, i32, i32, i32, i32, POINTER(i32), POINTER(i32), POINTER(i32), POINTER(i32)]),
+        "hyacinB200QuantizeW4": (i32, [H, i32, i32, i32, vp, i32, i32, i32, vp, i64, vp, vp, i32, vp, i32]),
+        "hyacinB200ProductW4": (i32, [H, c_char, i32, i32, i32, i32, vp, i64, i32, vp, vp, i32, vp, i32, i32, vp, i32, vp, i32, vp, i32]),
+        "hyacinB200DistillLoss": (i32, [H, i32, i32, i32, vp, i32, i32, vp, vp, i32, f64, vp, vp, vp, vp, vp, i32]),
+        "hyacinB200DistillGrad": (i32, [H, i32, i32, i32, vp, i32, i32, vp, vp, i32, f64, vp, vp, vp, vp, i32]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name, None)
@@ -274,3 +279,24 @@ class Hyacin:
 
     def reconstruct(self, n, moduli, residues, beta, order_c, C):
         self.lib.hyacinB200Reconstruct(byref(self.h), n, moduli, _dp(residues), beta, order_c, _dp(C))
+
+    # ---- compressed weight matrices (hyacin_b200.h) ----------------------------------------------------
+    def quantize_w4(self, wtype, m, n, W, ldw, seg_m, stype, codes, ldq, scales, zeros, lds, R=None, ldr=0) -> int:
+        """4-bit codes, scales and optional zero points of W, and optionally the residual a low-rank fit takes; 0 on success."""
+        return int(self.lib.hyacinB200QuantizeW4(byref(self.h), wtype, m, n, _dp(W), ldw, seg_m, stype, _dp(codes), ldq, _dp(scales),
+                                                 _dp(zeros), lds, _dp(R), ldr))
+
+    def product_w4(self, op, m, n, t, xtype, codes, ldq, seg_m, scales, zeros, lds, X, ldx, rank, U, ldu, V, ldv, Y, ldy) -> int:
+        """op 'T': Y = Wq^T X + V (U^T X); op 'N': Y = Wq X + U (V^T X); 0 on success."""
+        return int(self.lib.hyacinB200ProductW4(byref(self.h), op.encode(), m, n, t, xtype, _dp(codes), ldq, seg_m, _dp(scales), _dp(zeros),
+                                                lds, _dp(X), ldx, rank, _dp(U), ldu, _dp(V), ldv, _dp(Y), ldy))
+
+    def distill_loss(self, ztype, n, t, Z, ldz, k, ids, teacher, ldk, tau, teacher_lse, weight, loss, stats, dZ, lddz) -> int:
+        """Weighted KL per token against the teacher's top logits, optionally with its gradient; 0 on success."""
+        return int(self.lib.hyacinB200DistillLoss(byref(self.h), ztype, n, t, _dp(Z), ldz, k, _dp(ids), _dp(teacher), ldk, tau,
+                                                  _dp(teacher_lse), _dp(weight), _dp(loss), _dp(stats), _dp(dZ), lddz))
+
+    def distill_grad(self, ztype, n, t, Z, ldz, k, ids, teacher, ldk, tau, teacher_lse, weight, stats, dZ, lddz) -> int:
+        """The gradient of distill_loss from its saved statistics; 0 on success."""
+        return int(self.lib.hyacinB200DistillGrad(byref(self.h), ztype, n, t, _dp(Z), ldz, k, _dp(ids), _dp(teacher), ldk, tau,
+                                                  _dp(teacher_lse), _dp(weight), _dp(stats), _dp(dZ), lddz))

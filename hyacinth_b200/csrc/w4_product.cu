@@ -1,0 +1,132 @@
+// Products of a few vectors with a 4-bit weight matrix, Y = Wq^T X + V (U^T X) and Y = Wq X + U (V^T X), with
+// Wq(r, j) = s(j, r / segM) (q(r, j) - zero(j, r / segM)).
+#include "w4.cuh"
+
+namespace hyb {
+namespace {
+
+struct ProductArgs {
+  const uint8_t* codes; int64_t ldq; int m, n, t, seg;
+  const void* scales; const uint8_t* zeros; int64_t lds;
+  const void* x; int64_t ldx;
+  int rank; const void* second; int64_t ld2; const float* mid;      // correction: second (out x rank) times mid (rank x t)
+  void* y; int64_t ldy;
+};
+
+// y += sum_k second(row, k) mid(k, token)
+template <class T> __device__ __forceinline__ float add_correction(const ProductArgs& a, float y, int row, int token) {
+  const T* f = static_cast<const T*>(a.second) + row;
+  const float* m = a.mid + int64_t(token) * a.rank;
+  for (int k = 0; k < a.rank; ++k) y += to_f32(f[k * a.ld2]) * m[k];
+  return y;
+}
+
+// mid(k, token) = sum_r first(r, k) x(r, token): one warp per entry.
+template <class T> __global__ void __launch_bounds__(256) correction_mid_kernel(const T* first, int64_t ld1, int rows, int rank, const T* x, int64_t ldx, int t, float* mid) {
+  const int64_t task = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  if (task >= int64_t(rank) * t) return;
+  const int lane = threadIdx.x & 31, k = int(task % rank), token = int(task / rank);
+  float s = 0.f;
+  for (int r = lane; r < rows; r += 32) s += to_f32(first[k * ld1 + r]) * to_f32(x[token * ldx + r]);
+  for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(~0u, s, d);
+  if (lane == 0) mid[task] = s;
+}
+
+constexpr int kPlainTokens = 4;
+
+// op 'T', plain: one warp per column, the lanes share its words.
+template <class T> __global__ void __launch_bounds__(256) product_t_plain_kernel(ProductArgs a) {
+  const int lane = threadIdx.x & 31, col = blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (col >= a.n) return;
+  const T* x = static_cast<const T*>(a.x);
+  const T* scales = static_cast<const T*>(a.scales) + col * a.lds;
+  const int words = (a.m + kW4Block - 1) / kW4Block * 16;
+  for (int64_t t0 = int64_t(blockIdx.y) * kPlainTokens; t0 < a.t; t0 += int64_t(gridDim.y) * kPlainTokens) {
+    float acc[kPlainTokens] = {};
+    for (int w = lane; w < words; w += 32) {
+      const int row = w / 16 * kW4Block + w4_word_row(w & 15);
+      if (row >= a.m) continue;
+      const uint32_t word = *reinterpret_cast<const uint32_t*>(a.codes + col * a.ldq + int64_t(w) * 4);
+      const int seg = row / a.seg;
+      const float s = to_f32(scales[seg]); const int zero = a.zeros ? a.zeros[col * a.lds + seg] : 8;
+      for (int e = 0; e < 8 && row + e < a.m; ++e) {
+        const float v = s * float(int((word >> (4 * w4_row_nibble(e))) & 15u) - zero);
+        for (int t = 0; t < kPlainTokens; ++t) if (t0 + t < a.t) acc[t] += v * to_f32(x[(t0 + t) * a.ldx + row + e]);
+      }
+    }
+    for (int t = 0; t < kPlainTokens; ++t) {
+      for (int d = 16; d; d >>= 1) acc[t] += __shfl_xor_sync(~0u, acc[t], d);
+      if (lane == 0 && t0 + t < a.t) static_cast<T*>(a.y)[(t0 + t) * a.ldy + col] = from_f32<T>(add_correction<T>(a, acc[t], col, int(t0 + t)));
+    }
+  }
+}
+
+// op 'N', plain: one thread per row of a block of 128, running over the columns.
+template <class T> __global__ void __launch_bounds__(kW4Block) product_n_plain_kernel(ProductArgs a) {
+  const int row = blockIdx.x * kW4Block + threadIdx.x;
+  if (row >= a.m) return;
+  const int in = threadIdx.x, word = 4 * ((in & 31) >> 3) + (in >> 5), shift = 4 * w4_row_nibble(in & 7), seg = row / a.seg;
+  const uint8_t* codes = a.codes + int64_t(blockIdx.x) * 64 + word * 4;
+  const T* x = static_cast<const T*>(a.x);
+  const T* scales = static_cast<const T*>(a.scales) + seg;
+  for (int64_t t0 = int64_t(blockIdx.y) * kPlainTokens; t0 < a.t; t0 += int64_t(gridDim.y) * kPlainTokens) {
+    float acc[kPlainTokens] = {};
+    for (int j = 0; j < a.n; ++j) {
+      const uint32_t q = (*reinterpret_cast<const uint32_t*>(codes + j * a.ldq) >> shift) & 15u;
+      const float v = to_f32(scales[j * a.lds]) * float(int(q) - (a.zeros ? int(a.zeros[j * a.lds + seg]) : 8));
+      for (int t = 0; t < kPlainTokens; ++t) if (t0 + t < a.t) acc[t] += v * to_f32(x[(t0 + t) * a.ldx + j]);
+    }
+    for (int t = 0; t < kPlainTokens; ++t)
+      if (t0 + t < a.t) static_cast<T*>(a.y)[(t0 + t) * a.ldy + row] = from_f32<T>(add_correction<T>(a, acc[t], row, int(t0 + t)));
+  }
+}
+
+}  // namespace
+}  // namespace hyb
+
+extern "C" int32_t hyacinB200ProductW4(const hyacinHandle_t* handle, char opW, int32_t M, int32_t N, int32_t T, hyacinPrecision_t Xtype,
+                                       const uint8_t* codes, int64_t ldq, int32_t segM, const void* scales, const uint8_t* zeros,
+                                       int32_t lds, const void* X, int32_t ldx, int32_t rank, const void* U, int32_t ldu, const void* V,
+                                       int32_t ldv, void* Y, int32_t ldy) {
+  using namespace hyb;
+  const char* fn = "hyacinB200ProductW4";
+  if (!handle) return w4_refuse(fn, "no handle");
+  const bool trans = opW == 'T' || opW == 't';
+  if (!trans && opW != 'N' && opW != 'n') return w4_refuse(fn, "opW must be 'T' or 'N'");
+  if (!is_w4_type(Xtype)) return w4_refuse(fn, "type not supported");
+  if (M < 0 || N < 0 || T < 0 || rank < 0 || segM <= 0 || segM % 32) return w4_refuse(fn, "sizes: M, N, T, rank >= 0 and segM a positive multiple of 32");
+  const int in = trans ? M : N, out = trans ? N : M;
+  if (T == 0 || out == 0) return 0;
+  if (!Y || ldy < out) return w4_refuse(fn, "Y: null or leading dimension too small");
+  if (in > 0) {
+    if (!X || ldx < in) return w4_refuse(fn, "X: null or leading dimension too small");
+    if (!codes || !scales) return w4_refuse(fn, "null pointer");
+    if (lds < (int64_t(M) + segM - 1) / segM) return w4_refuse(fn, "lds too small");
+    if (ldq % 16 || ldq < (int64_t(M) + 127) / 128 * 64 || reinterpret_cast<uintptr_t>(codes) % 16) return w4_refuse(fn, "codes: 16-byte aligned, ldq a multiple of 16 and at least 64 ceil(M / 128)");
+    if (rank > 0 && (!U || !V || ldu < M || ldv < N)) return w4_refuse(fn, "U, V: null or leading dimension too small");
+  }
+  if (!w4_device_ok(handle)) return w4_refuse(fn, "the handle belongs to another device than the current one");
+  cudaStream_t stream = handle->cudaStream;
+  ProductArgs a{codes, ldq, M, N, T, segM, scales, zeros, lds, X, ldx, in > 0 ? rank : 0, trans ? V : U, trans ? ldv : ldu, nullptr, Y, ldy};
+  timer_mark(handle, Segment::Replicated);
+  float* mid = nullptr;
+  int32_t rc = 0;
+  with_w4_type(Xtype, [&](auto tag) {
+    using E = decltype(tag);
+    if (a.rank) {
+      const int64_t entries = int64_t(a.rank) * T;
+      const cudaError_t e = cudaMallocFromPoolAsync(reinterpret_cast<void**>(&mid), entries * sizeof(float), handle->mempool, stream);
+      if (e != cudaSuccess) { report_cuda_error(e, "cudaMallocFromPoolAsync", __FILE__, __LINE__); rc = -3; return; }
+      a.mid = mid;
+      count_launch();
+      correction_mid_kernel<E><<<unsigned((entries + 7) / 8), 256, 0, stream>>>(static_cast<const E*>(trans ? U : V), trans ? ldu : ldv, in, a.rank, static_cast<const E*>(X), ldx, T, mid);
+    }
+    const unsigned ty = unsigned(min((T + kPlainTokens - 1) / kPlainTokens, 65535));
+    count_launch();
+    if (trans) product_t_plain_kernel<E><<<dim3((N + 7) / 8, ty), 256, 0, stream>>>(a);
+    else product_n_plain_kernel<E><<<dim3((M + kW4Block - 1) / kW4Block, ty), kW4Block, 0, stream>>>(a);
+    rc = w4_launched(fn);
+  });
+  if (mid) HYB_CUDA(cudaFreeAsync(mid, stream));
+  return rc;
+}

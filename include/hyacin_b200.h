@@ -141,6 +141,65 @@ void hyacinB200ProfileReadTail(double* choleskyMs, int32_t* choleskyLaunches, do
 int32_t hyacinB200PivotedCholesky(const hyacinHandle_t* handle, double eps, int32_t N, int32_t K, hyacinPrecision_t Gtype,
                                   const void* G, int32_t ldg, int32_t* jpiv, void* R, int32_t ldr);
 
+/* ---- compressed weight matrices: 4-bit form, products, distillation -----------------------------------------
+ * A weight matrix W (M x N, column-major: column j holds the M weights of output j) is kept as 4-bit codes with one
+ * scale per (column, segment of segM rows) -- the table of hyacinXquantizeScaleBatch with short segments -- plus, where
+ * wanted, the truncated SVD of what that loses: W = Wq + U V^T, V from hyacinTsvdFit on the residual R = W - Wq, U = R V.
+ * The products below apply Wq + U V^T or its transpose to a few vectors, the distillation loss measures (and
+ * differentiates) what the compressed model's logits lose against the original's.  None of these has a counterpart in
+ * the reference.
+ *
+ * Storage.  Wq(r, j) = scales[j * lds + r / segM] * (q(r, j) - zero), zero = zeros[j * lds + r / segM] (0 .. 15), or 8 when
+ * zeros is NULL.  Codes: column j starts at codes + j * ldq (bytes, a multiple of 16 and at least 64 * ceil(M / 128); codes
+ * 16-byte aligned) and holds blocks of 128 rows as sixteen little-endian 32-bit words; row 32 i + 8 c + 2 p + h of a
+ * block (i, c, p < 4, h < 2) is the nibble p + 4 h of word 4 c + i.  Nibbles of rows >= M are written as 0 and ignored.
+ * Types: HYACIN_F32, HYACIN_F16 and HYACIN_B200_BF16 (no other entry point takes the latter).
+ * segM: a multiple of 32.  lds >= ceil(M / segM).
+ *
+ * All calls are asynchronous on handle->cudaStream, may be captured into a CUDA graph, and return 0, -1 for arguments
+ * they do not take (message on stderr, nothing launched), or -3 when CUDA refused a launch or an allocation.  The handle
+ * has to belong to the current device.  Scratch comes from handle->mempool in stream order.  Outputs do not overlap inputs
+ * unless stated.  Results do not depend on timing: there are no atomic sums. */
+#define HYACIN_B200_BF16 ((hyacinPrecision_t)32)
+
+/* 4-bit form of W (type Wtype, leading dimension ldw).  scales has type Stype.  zeros == NULL: symmetric,
+ * s = Stype(max|w| / 7), q = clamp(rint(w / s), -7, 7) + 8.  Otherwise lo = min(0, min w), hi = max(0, max w),
+ * s = Stype((hi - lo) / 15), zero = clamp(rint(-lo / s), 0, 15), q = clamp(rint(w / s) + zero, 0, 15).  Quotients are rounded as if
+ * exact, ties to even.  A scale of zero gives q = zero (8, or 0).  A segment that holds a NaN or an infinity gets a NaN scale and
+ * q = zero.  R (float, ldr >= M) receives W - Wq when it is not NULL. */
+int32_t hyacinB200QuantizeW4(const hyacinHandle_t* handle, hyacinPrecision_t Wtype, int32_t M, int32_t N, const void* W, int32_t ldw,
+                             int32_t segM, hyacinPrecision_t Stype, uint8_t* codes, int64_t ldq, void* scales, uint8_t* zeros,
+                             int32_t lds, float* R, int32_t ldr);
+
+/* opW 'T': Y (N x T) = Wq^T X + V (U^T X), X (M x T).   opW 'N': Y (M x T) = Wq X + U (V^T X), X (N x T), the gradient of
+ * the former to its input.  U is M x rank, V is N x rank; rank 0 leaves the correction out.  scales, X, Y, U and V have type
+ * Xtype.  Any T >= 0; made for few vectors.  Sums are held in 32 bits and Y is rounded once.  The 16-bit types round the
+ * scaled weights to 16 bits before the product for opW 'N' and for T > 16. */
+int32_t hyacinB200ProductW4(const hyacinHandle_t* handle, char opW, int32_t M, int32_t N, int32_t T, hyacinPrecision_t Xtype,
+                            const uint8_t* codes, int64_t ldq, int32_t segM, const void* scales, const uint8_t* zeros, int32_t lds,
+                            const void* X, int32_t ldx, int32_t rank, const void* U, int32_t ldu, const void* V, int32_t ldv,
+                            void* Y, int32_t ldy);
+
+/* Distillation from a teacher's top logits.  Column t of Z (N x T, type Ztype) holds the logits of token t over N classes;
+ * ids (K x T) and teacher (K x T, float), both with leading dimension ldk, the teacher's K largest logits and their
+ * classes.  Entries whose id lies outside [0, N) are skipped (pad with -1); a class listed twice counts with both its
+ * probabilities.  With u = z / tau, q = softmax(u) and p = softmax(teacher / tau) over the listed entries,
+ *     KL_t = sum_i p_i (log p_i - log q_i).
+ * teacherLse != NULL (T floats: log-sum-exp of ALL the teacher's logits over tau) makes p the teacher's true probabilities and
+ * everything that is not listed one more outcome: KL_t += p_r log(p_r / q_r), p_r = max(0, 1 - sum p_i), q_r = sum of q outside.
+ * loss[t] = weight[t] * KL_t and dZ (N x T, type Ztype, leading dimension lddz; may be Z itself with lddz == ldz) =
+ * weight[t] * dKL_t / dz; weight == NULL means 1; a token with weight 0 is not read and gets loss 0 and a zero gradient.
+ * loss, dZ and stats may each be NULL; stats (2 floats per token) is what hyacinB200DistillGrad needs to give the same
+ * gradient later, with the weights known by then (NaN for a token that had weight 0).  1e-30 <= tau <= 1e30, 0 <= K <= 1024,
+ * 1 <= N <= 2^20.  A student probability of zero under a
+ * positive teacher probability gives an infinite loss and a finite gradient. */
+int32_t hyacinB200DistillLoss(const hyacinHandle_t* handle, hyacinPrecision_t Ztype, int32_t N, int32_t T, const void* Z, int32_t ldz,
+                              int32_t K, const int32_t* ids, const float* teacher, int32_t ldk, double tau, const float* teacherLse,
+                              const float* weight, float* loss, float* stats, void* dZ, int32_t lddz);
+int32_t hyacinB200DistillGrad(const hyacinHandle_t* handle, hyacinPrecision_t Ztype, int32_t N, int32_t T, const void* Z, int32_t ldz,
+                              int32_t K, const int32_t* ids, const float* teacher, int32_t ldk, double tau, const float* teacherLse,
+                              const float* weight, const float* stats, void* dZ, int32_t lddz);
+
 #ifdef __cplusplus
 }
 #endif
