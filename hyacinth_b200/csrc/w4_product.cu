@@ -1,20 +1,14 @@
 // Products of a few vectors with a 4-bit weight matrix, Y = Wq^T X + V (U^T X) and Y = Wq X + U (V^T X), with
 // Wq(r, j) = s(j, r / segM) (q(r, j) - zero(j, r / segM)).
-#include "w4.cuh"
+#include "w4_product.h"
 
 namespace hyb {
 namespace {
 
-struct ProductArgs {
-  const uint8_t* codes; int64_t ldq; int m, n, t, seg;
-  const void* scales; const uint8_t* zeros; int64_t lds;
-  const void* x; int64_t ldx;
-  int rank; const void* second; int64_t ld2; const float* mid;      // correction: second (out x rank) times mid (rank x t)
-  void* y; int64_t ldy;
-};
+struct PlainArgs : ProductArgs { const float* mid = nullptr; };
 
 // y += sum_k second(row, k) mid(k, token)
-template <class T> __device__ __forceinline__ float add_correction(const ProductArgs& a, float y, int row, int token) {
+template <class T> __device__ __forceinline__ float add_correction(const PlainArgs& a, float y, int row, int token) {
   const T* f = static_cast<const T*>(a.second) + row;
   const float* m = a.mid + int64_t(token) * a.rank;
   for (int k = 0; k < a.rank; ++k) y += to_f32(f[k * a.ld2]) * m[k];
@@ -35,7 +29,7 @@ template <class T> __global__ void __launch_bounds__(256) correction_mid_kernel(
 constexpr int kPlainTokens = 4;
 
 // op 'T', plain: one warp per column, the lanes share its words.
-template <class T> __global__ void __launch_bounds__(256) product_t_plain_kernel(ProductArgs a) {
+template <class T> __global__ void __launch_bounds__(256) product_t_plain_kernel(PlainArgs a) {
   const int lane = threadIdx.x & 31, col = blockIdx.x * 8 + (threadIdx.x >> 5);
   if (col >= a.n) return;
   const T* x = static_cast<const T*>(a.x);
@@ -62,7 +56,7 @@ template <class T> __global__ void __launch_bounds__(256) product_t_plain_kernel
 }
 
 // op 'N', plain: one thread per row of a block of 128, running over the columns.
-template <class T> __global__ void __launch_bounds__(kW4Block) product_n_plain_kernel(ProductArgs a) {
+template <class T> __global__ void __launch_bounds__(kW4Block) product_n_plain_kernel(PlainArgs a) {
   const int row = blockIdx.x * kW4Block + threadIdx.x;
   if (row >= a.m) return;
   const int in = threadIdx.x, word = 4 * ((in & 31) >> 3) + (in >> 5), shift = 4 * w4_row_nibble(in & 7), seg = row / a.seg;
@@ -107,8 +101,11 @@ extern "C" int32_t hyacinB200ProductW4(const hyacinHandle_t* handle, char opW, i
   }
   if (!w4_device_ok(handle)) return w4_refuse(fn, "the handle belongs to another device than the current one");
   cudaStream_t stream = handle->cudaStream;
-  ProductArgs a{codes, ldq, M, N, T, segM, scales, zeros, lds, X, ldx, in > 0 ? rank : 0, trans ? V : U, trans ? ldv : ldu, nullptr, Y, ldy};
+  PlainArgs a;
+  static_cast<ProductArgs&>(a) = ProductArgs{codes, ldq, M, N, T, segM, scales, zeros, lds, X, ldx, in > 0 ? rank : 0,
+                                             trans ? U : V, trans ? ldu : ldv, trans ? V : U, trans ? ldv : ldu, Y, ldy};
   timer_mark(handle, Segment::Replicated);
+  if (in > 0 && Xtype != HYACIN_F32 && (!trans || T > 16)) return launch_product_umma(handle, fn, trans, Xtype, a);
   float* mid = nullptr;
   int32_t rc = 0;
   with_w4_type(Xtype, [&](auto tag) {
@@ -119,7 +116,7 @@ extern "C" int32_t hyacinB200ProductW4(const hyacinHandle_t* handle, char opW, i
       if (e != cudaSuccess) { report_cuda_error(e, "cudaMallocFromPoolAsync", __FILE__, __LINE__); rc = -3; return; }
       a.mid = mid;
       count_launch();
-      correction_mid_kernel<E><<<unsigned((entries + 7) / 8), 256, 0, stream>>>(static_cast<const E*>(trans ? U : V), trans ? ldu : ldv, in, a.rank, static_cast<const E*>(X), ldx, T, mid);
+      correction_mid_kernel<E><<<unsigned((entries + 7) / 8), 256, 0, stream>>>(static_cast<const E*>(a.first), a.ld1, in, a.rank, static_cast<const E*>(X), ldx, T, mid);
     }
     const unsigned ty = unsigned(min((T + kPlainTokens - 1) / kPlainTokens, 65535));
     count_launch();

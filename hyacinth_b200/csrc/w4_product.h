@@ -1,0 +1,19 @@
+// Interfaces between the kernels of hyacinB200ProductW4 (host side).
+#pragma once
+#include "w4.cuh"
+
+namespace hyb {
+
+struct ProductArgs {
+  const uint8_t* codes; int64_t ldq; int m, n, t, seg;
+  const void* scales; const uint8_t* zeros; int64_t lds;
+  const void* x; int64_t ldx;
+  // correction: second (outputs x rank) times mid = first^T x (rank x t)
+  int rank; const void* first; int64_t ld1; const void* second; int64_t ld2;
+  void* y; int64_t ldy;
+};
+
+// Fifth-generation tensor cores, 16-bit types, both directions.  Returns 0 or -3.
+int32_t launch_product_umma(const hyacinHandle_t* handle, const char* fn, bool trans, hyacinPrecision_t type, const ProductArgs& a);
+
+}  // namespace hyb
