@@ -1,21 +1,23 @@
 // Products with a 4-bit weight matrix on the fifth-generation tensor cores (16-bit types, both directions).
 //
 // Y (out x T) = A X, A = Wq^T or Wq.  A CTA computes 128 outputs x NT tokens (NT <= 256, accumulators in tensor memory) over a
-// range of K steps of 128:
-//   warp 0     TMA producer: the step's codes (128 columns x 64 bytes, 8 KiB) and the step's X tile (NT tokens x 128, K-major)
-//              into a ring, so that the code stream from DRAM never waits for the arithmetic;
-//   warps 2-9  turn codes into the scaled 16-bit weights s (q - zero) of a 128 x 128 operand tile in shared memory;
-//   warp 1     issues tcgen05.mma (M128, N NT, K16) on it.
-// Both directions share the dequantisation: a thread owns one column of W and a word of its codes is eight consecutive rows, one
-// 16-byte chunk.  With opW 'T' the tile's rows are columns of W and the chunk runs along K (K-major operand); with 'N' the rows of
-// shared memory are K and the chunk runs along the outputs (MN-major operand).  Address and swizzle are the same, only the
-// descriptor differs.
+// range of K steps:
+//   warp 0     TMA producer: the step's codes and the step's X tile (NT tokens, K-major) into a ring, so that the code stream from
+//              DRAM never waits for the arithmetic;
+//   warp 1     issues tcgen05.mma (M128, N NT, K16);
+//   warps 2-5  fetch the step's scales and zero points into the ring;
+//   warps 6-21 turn codes into scaled 16-bit weights s (q - zero), in four groups of four warps that take every fourth step, into up
+//              to six operand buffers: from the dequantised tile to the freed buffer takes some 1700 cycles, several steps' worth.
+// opW 'T': a step is 128 rows of W, a thread owns one output and writes its K values to tensor memory, the A operand of the
+// instruction (an instruction with A in shared memory takes 40 cycles for its 4 KiB however small NT is, from tensor memory
+// 10 to 33).  opW 'N': a step is 64 columns of W; a word of codes is eight consecutive outputs at one K, a 16-byte chunk of an
+// MN-major operand in shared memory.
 // The correction V (U^T X) is two more operands of the same product: K steps whose A tile is V and whose X tile is
 // mid = U^T X, kept as two 16-bit parts (value and remainder), so that it adds no rounding of its own.
 // Few tiles: a cluster of up to 8 CTAs splits the K steps of one tile and adds the partial sums through distributed shared memory
 // in a fixed order.
 // Rounding: s (q - zero) has up to 15 significant bits (8 of s, 5 of q for bfloat16) and is rounded to the operand type, which
-// is what the matrix instruction takes; one half step, independent per weight, well below the rounding of Y after a sum.
+// is what the matrix instruction takes; one half step, independent per weight, of the size of the rounding of Y itself.
 #include "w4_product.h"
 #include "ptx_sm100.cuh"
 #include <algorithm>
@@ -26,27 +28,38 @@ namespace {
 using namespace ptx;
 
 constexpr int kOut = 128;                         // outputs per tile
-constexpr int kStep = 128;                        // K per step
-constexpr uint32_t kCodeBytes = 128 * 64;
-constexpr uint32_t kOperandBytes = kOut * kStep * 2;
 constexpr int kMaxRing = 8;
-constexpr int kThreads = 320;
-constexpr int kWorkers = 8;                       // dequantising warps
-constexpr uint32_t kSmemLimit = 232448;
+constexpr int kMaxTokens = 256;                   // per tile
+constexpr int kLoaders = 4;                       // warps that fetch scales
+constexpr int kGroups = 4, kGroupWarps = 4;       // dequantising warps
+constexpr int kMaxBufs = 6;                       // operand buffers
+constexpr int kThreads = 32 * (2 + kLoaders + kGroups * kGroupWarps);
+// More than half of the shared memory, always: one CTA per SM, so tensor memory is not contended for, which clusters whose CTAs
+// wait for one another could not afford.
+constexpr uint32_t kSmemLimit = 232448, kSmemFloor = 120 * 1024;
+template <bool TRANS> struct Geometry {
+  static constexpr int step = TRANS ? 128 : 64;                          // K per step
+  static constexpr int cols = TRANS ? kOut : step;                       // columns of W per step
+  static constexpr uint32_t code_bytes = cols * 64;
+  static constexpr uint32_t scale_bytes = cols * 12;                     // four 16-bit scales and four zero points per column
+  static constexpr uint32_t operand_bytes = TRANS ? 0 : kOut * step * 2; // in shared memory, per group
+  static constexpr uint32_t operand_cols = TRANS ? step / 2 : 0;         // in tensor memory, per group
+};
 
 struct UmmaParams {
   const void* scales; const uint8_t* zeros; int64_t lds;
   int m, n, t, out;
   int segs, seg_sub, seg_shift;                   // 32-row subsets per segment; shift when that is a power of two, else -1
+  int wide;                                       // segments of a block that one aligned load fetches (1, 2, 4)
   int code_steps, steps;                          // K steps of codes, and with those of the correction
   int rank; const void* second; int64_t ld2;
   void* y; int64_t ldy;
-  int nt, ring, splits; uint32_t tmem_cols, idesc;
+  int nt, ring, bufs, groups, splits, second_aligned; uint32_t nt_cols, tmem_cols, idesc;
   uint32_t* status;
 };
 
 struct UmmaBars {
-  uint64_t full[kMaxRing], empty[kMaxRing], a_full[2], a_empty[2], done;
+  uint64_t full[kMaxRing], empty[kMaxRing], a_full[kMaxBufs], done;
   uint32_t tmem_base; uint32_t abort_flag;
 };
 
@@ -54,6 +67,44 @@ __device__ __forceinline__ void umma_f16(uint32_t d, uint64_t adesc, uint64_t bd
   asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
                "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
                ::"r"(d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+               "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+               ::"r"(d), "r"(a), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+      ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+        "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]),
+        "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]),
+        "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+      : "memory");
+}
+// Bounded waits for the pipelines of this kernel, executed by whole warps: a poll by a single lane is not suspended by the
+// hardware, and many warps that poll slow the multiplying warp down (a satisfied wait took it 800 cycles with 20 single-lane
+// pollers).  So few warps poll at a time, the ones that run ahead with pauses in between.
+template <bool PAUSE> __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_flag, uint32_t* status, uint32_t code) {
+  bool ok = false;
+#pragma unroll 1
+  for (uint32_t it = 0; it < (1u << 20); ++it) {
+    uint32_t done;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(done) : "r"(smem_u32(bar)), "r"(parity), "r"(20000u) : "memory");
+    if (__all_sync(~0u, done)) { ok = true; break; }
+    if (__any_sync(~0u, *abort_flag)) break;
+    if (PAUSE) __nanosleep(64);
+  }
+  if (!ok && (threadIdx.x & 31) == 0 && !*abort_flag) { *abort_flag = 1u; *reinterpret_cast<volatile uint32_t*>(status) = code; }
+  return __all_sync(~0u, ok);
+}
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r != 0;
 }
 __device__ __forceinline__ void tmem_ld8(uint32_t addr, float (&v)[8]) {
   uint32_t r[8];
@@ -85,6 +136,15 @@ __device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, ui
   asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
+// Eight consecutive values, the first `valid` of them, zeros behind.
+template <class T> __device__ __forceinline__ uint4 load8(const T* p, int valid, bool aligned) {
+  if (valid >= 8 && aligned) return *reinterpret_cast<const uint4*>(p);
+  uint32_t o[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (int e = 0; e < 8; ++e) if (e < valid) o[e >> 1] |= uint32_t(reinterpret_cast<const uint16_t*>(p)[e]) << (16 * (e & 1));
+  return make_uint4(o[0], o[1], o[2], o[3]);
+}
+
 // Scale and zero point of one (column, segment), as the pairs that the dequantisation multiplies and subtracts.
 template <class T> struct Scale;
 // half: 0x6400 | q is 1024 + q and 0x6400 | 16 q is 1024 + 16 q, both exact
@@ -96,7 +156,7 @@ template <> struct Scale<__half> {
   }
   static __device__ __forceinline__ uint32_t u(__half2 v) { return *reinterpret_cast<uint32_t*>(&v); }
   static __device__ __forceinline__ __half2 h(uint32_t v) { return *reinterpret_cast<__half2*>(&v); }
-  static __device__ __forceinline__ void word(uint32_t w, const Ready& r, uint32_t (&o)[4]) {
+  static __device__ __forceinline__ void word(uint32_t w, const Ready& r, uint32_t* o) {
     const __half2 sixteenth = __float2half2_rn(0.0625f);
     const uint32_t v = w >> 8;
     o[0] = u(__hmul2(__hadd2(h((w & 0x000f000fu) | 0x64006400u), r.low), r.s));
@@ -114,7 +174,7 @@ template <> struct Scale<__nv_bfloat16> {
   }
   static __device__ __forceinline__ uint32_t u(__nv_bfloat162 v) { return *reinterpret_cast<uint32_t*>(&v); }
   static __device__ __forceinline__ __nv_bfloat162 h(uint32_t v) { return *reinterpret_cast<__nv_bfloat162*>(&v); }
-  static __device__ __forceinline__ void word(uint32_t w, const Ready& r, uint32_t (&o)[4]) {
+  static __device__ __forceinline__ void word(uint32_t w, const Ready& r, uint32_t* o) {
 #pragma unroll
     for (int p = 0; p < 4; ++p) o[p] = u(__hmul2(__hadd2(h(((w >> (4 * p)) & 0x000f000fu) | 0x43004300u), r.low), r.s));
   }
@@ -127,20 +187,41 @@ product_umma_kernel(const __grid_constant__ CUtensorMap code_map, const __grid_c
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* aligned = smem_raw + (base - smem_u32(smem_raw));
+  using G = Geometry<TRANS>;
+  constexpr int kStep = G::step;
   const uint32_t x_bytes = uint32_t(p.nt) * kStep * 2;
-  const uint32_t operand = base + p.ring * kCodeBytes, x_ring = operand + 2 * kOperandBytes;
-  UmmaBars* bars = reinterpret_cast<UmmaBars*>(aligned + size_t(p.ring) * kCodeBytes + 2 * kOperandBytes + size_t(p.ring) * x_bytes);
+  const uint32_t operand = base + p.ring * G::code_bytes, x_ring = operand + p.bufs * G::operand_bytes, scale_ring = x_ring + p.ring * x_bytes;
+  UmmaBars* bars = reinterpret_cast<UmmaBars*>(aligned + (scale_ring - base) + p.ring * G::scale_bytes);
   volatile uint32_t* abort_flag = &bars->abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int part = int(blockIdx.x) % p.splits, tile = int(blockIdx.x) / p.splits, t0 = int(blockIdx.y) * p.nt;
   const int step0 = int(int64_t(p.steps) * part / p.splits), step1 = int(int64_t(p.steps) * (part + 1) / p.splits);
 
+  // The first copies start before the block has met: the thread that issues them has initialised their barriers itself.
+  const int early = step1 - step0 < p.ring ? step1 - step0 : p.ring;
+  auto issue = [&](int k, uint32_t stage) {
+    uint64_t* bar = &bars->full[stage];
+    const uint32_t sx = x_ring + stage * x_bytes;
+    if (k < p.code_steps) {
+      mbar_expect_tx(bar, G::code_bytes + x_bytes);
+      if (TRANS) tma_load_2d(base + stage * G::code_bytes, &code_map, bar, k * 64, tile * kOut);
+      else tma_load_2d(base + stage * G::code_bytes, &code_map, bar, tile * 64, k * kStep);
+      tma_load_2d(sx, &x_map, bar, k * kStep, t0);
+      if (TRANS) tma_load_2d(sx + x_bytes / 2, &x_map, bar, k * kStep + 64, t0);
+    } else {
+      mbar_expect_tx(bar, x_bytes);
+      const int c = (k - p.code_steps) * kStep;
+      tma_load_2d(sx, &mid_map, bar, c, t0);
+      if (TRANS) tma_load_2d(sx + x_bytes / 2, &mid_map, bar, c + 64, t0);
+    }
+  };
   if (threadIdx.x == 0) {
-    for (int s = 0; s < p.ring; ++s) { mbar_init(&bars->full[s], 1); mbar_init(&bars->empty[s], 1); }
-    for (int a = 0; a < 2; ++a) { mbar_init(&bars->a_full[a], kWorkers); mbar_init(&bars->a_empty[a], 1); }
+    for (int s = 0; s < p.ring; ++s) { mbar_init(&bars->full[s], 2); mbar_init(&bars->empty[s], 1); }
+    for (int a = 0; a < p.bufs; ++a) mbar_init(&bars->a_full[a], kGroupWarps);
     mbar_init(&bars->done, 1);
     bars->abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    for (int k = step0; k < step0 + early && k < p.code_steps; ++k) issue(k, k - step0);
   }
   if (warp == 1) tmem_alloc(&bars->tmem_base, p.tmem_cols);
   tc_fence_before();
@@ -150,134 +231,232 @@ product_umma_kernel(const __grid_constant__ CUtensorMap code_map, const __grid_c
 
   bool ok = true;
   if (warp == 0) {
-    if (lane == 0) {
-      uint32_t stage = 0, phase = 0; int issued = 0; bool waited = false;
-      for (int k = step0; k < step1; ++k) {
-        if (!(ok = mbar_wait(&bars->empty[stage], phase ^ 1u, abort_flag, p.status, 11u))) break;
-        uint64_t* bar = &bars->full[stage];
-        const uint32_t sx = x_ring + stage * x_bytes;
-        if (k < p.code_steps) {
-          mbar_expect_tx(bar, kCodeBytes + x_bytes);
-          if (TRANS) tma_load_2d(base + stage * kCodeBytes, &code_map, bar, k * 64, tile * kOut);
-          else tma_load_2d(base + stage * kCodeBytes, &code_map, bar, tile * 64, k * kStep);
-          tma_load_2d(sx, &x_map, bar, k * kStep, t0);
-          tma_load_2d(sx + x_bytes / 2, &x_map, bar, k * kStep + 64, t0);
-        } else {
-          // mid comes from the kernel before this one, which may still be running
-          if (!waited) { asm volatile("griddepcontrol.wait;" ::: "memory"); waited = true; }
-          mbar_expect_tx(bar, x_bytes);
-          const int c = (k - p.code_steps) * kStep;
-          tma_load_2d(sx, &mid_map, bar, c, t0);
-          tma_load_2d(sx + x_bytes / 2, &mid_map, bar, c + 64, t0);
-        }
-        ++issued;
-        if (++stage == uint32_t(p.ring)) { stage = 0; phase ^= 1u; }
+    uint32_t stage = 0, phase = 0; int issued = 0; bool waited = false;
+    for (int k = step0; k < step1; ++k) {
+      if (!(issued < early && k < p.code_steps)) {
+        if (issued >= p.ring && !(ok = warp_wait<true>(&bars->empty[stage], phase ^ 1u, abort_flag, p.status, 11u))) break;
+        // mid comes from the kernel before this one, which may still be running
+        if (k >= p.code_steps && !waited) { asm volatile("griddepcontrol.wait;" ::: "memory"); waited = true; }
+        if (lane == 0) issue(k, stage);
+        __syncwarp();
       }
-      if (!ok) {      // some role gave up: let the copies in flight land before the block can end
-        uint32_t ignore = 0;
-        for (int b = 0; b < (issued < p.ring ? issued : p.ring); ++b) {
-          if (stage == 0) { stage = p.ring; phase ^= 1u; }
-          --stage;
-          mbar_wait(&bars->full[stage], phase, &ignore, p.status, 12u);
-        }
+      ++issued;
+      if (++stage == uint32_t(p.ring)) { stage = 0; phase ^= 1u; }
+    }
+    if (!ok && lane == 0) {      // some role gave up: let the copies in flight land before the block can end
+      uint32_t ignore = 0;
+      for (int b = 0; b < (issued < p.ring ? issued : p.ring); ++b) {
+        if (stage == 0) { stage = p.ring; phase ^= 1u; }
+        --stage;
+        mbar_wait(&bars->full[stage], phase, &ignore, p.status, 12u);
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      uint32_t stage = 0, phase = 0, buf = 0, buf_phase = 0;
-      for (int k = step0; k < step1; ++k) {
-        if (!(ok = mbar_wait(&bars->full[stage], phase, abort_flag, p.status, 13u))) break;
-        if (!(ok = mbar_wait(&bars->a_full[buf], buf_phase, abort_flag, p.status, 14u))) break;
-        tc_fence_after();
-        const uint32_t sa = operand + buf * kOperandBytes, sx = x_ring + stage * x_bytes;
+    // The whole warp runs the loop and one elected lane issues: descriptors then stay in uniform registers.  With the loop inside
+    // a single-lane branch an instruction took 69 cycles to issue, more than it runs for with NT <= 128.
+    uint32_t stage = 0, buf = 0, buf_phase = 0;
+    for (int k = step0; k < step1; ++k) {
+      // the group that filled the operand buffer had seen the step's copies land
+      if (!(ok = warp_wait<false>(&bars->a_full[buf], buf_phase, abort_flag, p.status, 14u))) break;
+      tc_fence_after();
+      const uint32_t sx = x_ring + stage * x_bytes, ta = tmem + p.nt_cols + buf * G::operand_cols;
+      const uint64_t a0 = operand_desc(operand + buf * G::operand_bytes, G::operand_bytes / 2), b0 = operand_desc(sx, 16);
+      const uint32_t b_half = x_bytes / 32;
+      if (elect_one()) {
 #pragma unroll
         for (int q = 0; q < kStep / 16; ++q) {
-          const uint64_t ad = TRANS ? operand_desc(sa + (q >> 2) * (kOperandBytes / 2) + (q & 3) * 32, 16)
-                                    : operand_desc(sa + q * 2048, kOperandBytes / 2);
-          const uint64_t bd = operand_desc(sx + (q >> 2) * (x_bytes / 2) + (q & 3) * 32, 16);
-          umma_f16(tmem, ad, bd, p.idesc, (k > step0 || q > 0) ? 1u : 0u);
+          const uint64_t bd = b0 + ((q >> 2) * b_half + (q & 3) * 2);
+          if (TRANS) umma_f16_ts(tmem, ta + q * 8, bd, p.idesc, (k > step0 || q > 0) ? 1u : 0u);
+          else umma_f16(tmem, a0 + q * 128, bd, p.idesc, (k > step0 || q > 0) ? 1u : 0u);
         }
         umma_commit(&bars->empty[stage]);
-        umma_commit(&bars->a_empty[buf]);
-        if (++stage == uint32_t(p.ring)) { stage = 0; phase ^= 1u; }
-        if (++buf == 2) { buf = 0; buf_phase ^= 1u; }
       }
-      umma_commit(&bars->done);
-      if (!ok) { uint32_t ignore = 0; mbar_wait(&bars->done, 0u, &ignore, p.status, 15u); }      // instructions in flight end before tensor memory is freed
+      __syncwarp();
+      if (++stage == uint32_t(p.ring)) stage = 0;
+      if (++buf == uint32_t(p.bufs)) { buf = 0; buf_phase ^= 1u; }
     }
-  } else {
-    const int id = threadIdx.x - 64, row = id & 127, half = id >> 7;      // row: column of W within the step's 128
-    const bool uniform = (p.seg_sub & 3) == 0;
-    Scale<T> cur[4];
-    auto load_scales = [&](int k) {
-      const int col = TRANS ? tile * kOut + row : k * kStep + row;
-      const int sub = (TRANS ? k : tile) * 4;
-      const bool live = col < p.n;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (i > 0 && uniform) { cur[i] = cur[0]; continue; }
-        int s = p.seg_shift >= 0 ? (sub + i) >> p.seg_shift : (sub + i) / p.seg_sub;
-        s = min(s, p.segs - 1);
-        cur[i].bits = live ? static_cast<const uint16_t*>(p.scales)[col * p.lds + s] : uint16_t(0);
-        cur[i].zero = p.zeros ? (live ? int(p.zeros[col * p.lds + s]) : 0) : 8;
-      }
+    if (elect_one()) umma_commit(&bars->done);
+    __syncwarp();
+    if (!ok) { uint32_t ignore = 0; mbar_wait(&bars->done, 0u, &ignore, p.status, 15u); }      // instructions in flight end before tensor memory is freed
+  } else if (warp < 2 + kLoaders) {
+    // Scales and zero points of a step, [column][subset]: they lie one row of the table per column, so every load touches as many
+    // lines as lanes.  Each loader takes every fourth step and has the next one's loads in flight while it hands one over.
+    const int loaders = p.ring < kLoaders ? p.ring : kLoaders;
+    constexpr int kPer = G::cols / 32;                             // columns per lane
+    struct Entry { uint32_t s01, s23, z; } even[kPer], odd[kPer];
+    enum Form { kNothing, kOne, kPair, kFour, kMixed };
+    auto segment = [&](int sub) { return p.seg_shift >= 0 ? sub >> p.seg_shift : sub / p.seg_sub; };
+    auto form = [&](int k) {
+      if (k >= p.code_steps || k >= step1) return kNothing;
+      const int first = segment((TRANS ? k : tile) * 4);
+      return p.wide == 4 && first + 4 <= p.segs ? kFour : p.wide == 2 && first + 2 <= p.segs ? kPair : (p.seg_sub & 3) == 0 ? kOne : kMixed;
     };
-    uint32_t stage = 0, phase = 0, buf = 0, buf_phase = 0;
-    if (step0 < min(step1, p.code_steps)) load_scales(step0);
-    for (int k = step0; k < step1; ++k) {
-      const uint32_t dst = operand + buf * kOperandBytes + row * 128, swz = (row & 7) << 4;
-      if (k < p.code_steps) {
-        ok = __all_sync(~0u, mbar_wait(&bars->full[stage], phase, abort_flag, p.status, 16u));
-        if (!ok) break;
-        uint4 q[2];
+    auto fetch = [&](int k, Entry (&e)[kPer]) {
+      const int sub = (TRANS ? k : tile) * 4, first = segment(sub);
+      const Form f = form(k);
 #pragma unroll
-        for (int c = 0; c < 2; ++c) q[c] = lds128(base + stage * kCodeBytes + row * 64 + (((2 * half + c) ^ ((row >> 1) & 3)) << 4));
-        typename Scale<T>::Ready r[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) r[i] = cur[i].ready();
-        if (k + 1 < min(step1, p.code_steps)) load_scales(k + 1);
-        ok = __all_sync(~0u, mbar_wait(&bars->a_empty[buf], buf_phase ^ 1u, abort_flag, p.status, 17u));
-        if (!ok) break;
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const uint32_t w[4] = {q[c].x, q[c].y, q[c].z, q[c].w};
+      for (int j = 0; j < kPer; ++j) {
+        const int col = (TRANS ? tile * kOut : k * kStep) + 32 * j + lane;
+        e[j].s01 = e[j].s23 = 0; e[j].z = p.zeros ? 0u : 0x08080808u;
+        if (f == kNothing || col >= p.n) continue;
+        const uint16_t* scales = static_cast<const uint16_t*>(p.scales) + col * p.lds;
+        const uint8_t* zeros = p.zeros + col * p.lds;
+        if (f == kFour) {
+          const uint2 v = *reinterpret_cast<const uint2*>(scales + first);
+          e[j].s01 = v.x; e[j].s23 = v.y;
+          if (p.zeros) e[j].z = *reinterpret_cast<const uint32_t*>(zeros + first);
+        } else if (f == kPair) {
+          e[j].s01 = *reinterpret_cast<const uint32_t*>(scales + first);
+          if (p.zeros) e[j].z = *reinterpret_cast<const uint16_t*>(zeros + first);
+        } else if (f == kOne) {
+          e[j].s01 = scales[first];
+          if (p.zeros) e[j].z = zeros[first];
+        } else {
+          uint32_t s[4], z = 0;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            uint32_t o[4]; Scale<T>::word(w[i], r[i], o);
-            sts128(dst + (i >> 1) * (kOperandBytes / 2) + (((4 * (i & 1) + 2 * half + c) << 4) ^ swz), o[0], o[1], o[2], o[3]);
+            const int g = min(segment(sub + i), p.segs - 1);
+            s[i] = scales[g];
+            if (p.zeros) z |= uint32_t(zeros[g]) << (8 * i);
+          }
+          e[j].s01 = s[0] | s[1] << 16; e[j].s23 = s[2] | s[3] << 16;
+          if (p.zeros) e[j].z = z;
+        }
+      }
+    };
+    uint32_t stage = (warp - 2) % p.ring, phase = 0;
+    auto hand_over = [&](int k, const Entry (&e)[kPer]) {
+      if (!warp_wait<true>(&bars->empty[stage], phase ^ 1u, abort_flag, p.status, 20u)) return false;
+      const uint32_t at = scale_ring + stage * G::scale_bytes;
+      const Form f = form(k);
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        uint32_t s01 = e[j].s01, s23 = e[j].s23, z = e[j].z;
+        if (f == kPair) { s23 = __byte_perm(s01, 0, 0x3232); s01 = __byte_perm(s01, 0, 0x1010); if (p.zeros) z = __byte_perm(z, 0, 0x1100); }
+        else if (f == kOne) { s23 = s01 = __byte_perm(s01, 0, 0x1010); if (p.zeros) z = __byte_perm(z, 0, 0x0000); }
+        asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at + (32 * j + lane) * 8), "r"(s01), "r"(s23) : "memory");
+        asm volatile("st.shared.u32 [%0], %1;" ::"r"(at + G::cols * 8 + (32 * j + lane) * 4), "r"(z) : "memory");
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->full[stage]);
+      stage += loaders;
+      while (stage >= uint32_t(p.ring)) { stage -= p.ring; phase ^= 1u; }
+      return true;
+    };
+    // A loader that waits for step k has handed over step k - loaders, so step k - loaders - ring has left the
+    // ring; with loaders <= ring that covers step k - 2 ring, and the parity it waits for cannot be that of the phase before.
+    int k = warp - 2 < loaders ? step0 + warp - 2 : step1;
+    fetch(k, even);
+    while (k < step1) {
+      fetch(k + loaders, odd);
+      if (!(ok = hand_over(k, even))) break;
+      if ((k += loaders) >= step1) break;
+      fetch(k + loaders, even);
+      if (!(ok = hand_over(k, odd))) break;
+      k += loaders;
+    }
+  } else {
+    const int id = threadIdx.x - 32 * (2 + kLoaders), group = id >> 7;
+    // column of W within the step; for 'T' that is the output, which has to be this thread's lane of tensor memory
+    const int row = TRANS ? 32 * (warp & 3) + lane : id & 63, half = (id >> 6) & 1;
+    const uint32_t swz = (row & 7) << 4;
+    // An operand buffer is free when the step before on it, k - bufs, was multiplied: the barrier that also frees that step's ring
+    // stage.  A group waits for its own steps only and a barrier cannot overtake it: step k + ring is not loaded, and step
+    // k - bufs + ring >= k not multiplied, before step k was, which needs this group (bufs <= ring).  It cannot be early either:
+    // after its first wait all steps up to k - bufs are known to be multiplied, so step k's stage is in its last or this phase, and
+    // its wait for step k - groups before told the same of step k - groups - bufs (groups <= ring).
+    // The group's first warp polls, the others wait at a barrier that also tells them whether it gave up.
+    auto group_wait = [&](uint64_t* free, uint32_t free_parity, uint64_t* full, uint32_t full_parity) {
+      uint32_t good = 1;
+      if (((id >> 5) & 3) == 0) {
+        if (free) good = warp_wait<false>(free, free_parity, abort_flag, p.status, 17u);
+        if (good) good = warp_wait<false>(full, full_parity, abort_flag, p.status, 16u);
+      }
+      asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %0, 0;\n\tbar.red.and.pred q, %1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                   : "+r"(good) : "r"(group + 1) : "memory");
+      return good != 0;
+    };
+    uint32_t stage = group, phase = 0, buf = group;
+    for (int k = group < p.groups ? step0 + group : step1; k < step1; k += p.groups) {
+      const int s = k - step0 - p.bufs;
+      if (!(ok = group_wait(s >= 0 ? &bars->empty[s % p.ring] : nullptr, (s / p.ring) & 1, &bars->full[stage], phase))) break;
+      const uint32_t dst = operand + buf * G::operand_bytes + row * 128;
+      const uint32_t tdst = tmem + (uint32_t(32 * (warp & 3)) << 16) + p.nt_cols + buf * G::operand_cols;
+      if (TRANS) tc_fence_after();
+      if (k < p.code_steps) {
+        const uint32_t at = scale_ring + stage * G::scale_bytes, codes = base + stage * G::code_bytes + row * 64, chunk = (row >> 1) & 3;
+        constexpr int kQuarters = TRANS ? 4 : 2;
+        uint32_t s[2], z; uint4 q[kQuarters];
+        asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(s[0]), "=r"(s[1]) : "r"(at + row * 8));
+        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(z) : "r"(at + G::cols * 8 + row * 4));
+#pragma unroll
+        for (int c = 0; c < kQuarters; ++c) q[c] = lds128(codes + (((TRANS ? c : 2 * half + c) ^ chunk) << 4));
+#pragma unroll
+        for (int pair = 0; pair < 2; ++pair) {
+          uint32_t o[2][kQuarters][4];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            Scale<T> sc; sc.bits = uint16_t(s[pair] >> (16 * i)); sc.zero = (z >> (16 * pair + 8 * i)) & 0xff;
+            const typename Scale<T>::Ready r = sc.ready();
+#pragma unroll
+            for (int c = 0; c < kQuarters; ++c) Scale<T>::word(pair == 0 ? (i == 0 ? q[c].x : q[c].y) : (i == 0 ? q[c].z : q[c].w), r, o[i][c]);
+          }
+          if constexpr (TRANS) tmem_st32(tdst + pair * 32, reinterpret_cast<const uint32_t (&)[32]>(o));
+          else {
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+              for (int c = 0; c < kQuarters; ++c)
+                sts128(dst + pair * (G::operand_bytes / 2) + (((4 * i + 2 * half + c) << 4) ^ swz), o[i][c][0], o[i][c][1], o[i][c][2], o[i][c][3]);
           }
         }
       } else {
         // correction step: entry (output, c) of the operand is second(output, c mod rank), c < 2 rank
-        ok = __all_sync(~0u, mbar_wait(&bars->a_empty[buf], buf_phase ^ 1u, abort_flag, p.status, 18u));
-        if (!ok) break;
         const uint16_t* second = static_cast<const uint16_t*>(p.second);
+        const int c0 = (k - p.code_steps) * kStep;
+        if constexpr (TRANS) {
+          const int out = tile * kOut + row;
 #pragma unroll 1
-        for (int j = 0; j < 8; ++j) {
-          uint32_t o[4] = {0, 0, 0, 0};
+          for (int pair = 0; pair < 2; ++pair) {
+            uint32_t o[32];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const int along = 64 * half + 8 * j + e;
-            const int c = (k - p.code_steps) * kStep + (TRANS ? along : row), out = tile * kOut + (TRANS ? row : along);
-            if (c < 2 * p.rank && out < p.out) o[e >> 1] |= uint32_t(second[out + int64_t(c < p.rank ? c : c - p.rank) * p.ld2]) << (16 * (e & 1));
+            for (int e = 0; e < 32; ++e) {
+              const int a = c0 + pair * 64 + 2 * e, b = a + 1;
+              const uint32_t lo = a < 2 * p.rank && out < p.out ? second[out + int64_t(a < p.rank ? a : a - p.rank) * p.ld2] : 0u;
+              const uint32_t hi = b < 2 * p.rank && out < p.out ? second[out + int64_t(b < p.rank ? b : b - p.rank) * p.ld2] : 0u;
+              o[e] = lo | hi << 16;
+            }
+            tmem_st32(tdst + pair * 32, o);
           }
-          sts128(dst + half * (kOperandBytes / 2) + ((j << 4) ^ swz), o[0], o[1], o[2], o[3]);
+        } else {
+          const int c = c0 + row;
+          const uint16_t* from = second + int64_t(c < p.rank ? c : c - p.rank) * p.ld2 + tile * kOut + 64 * half;
+          const int valid = c < 2 * p.rank ? p.out - tile * kOut - 64 * half : 0;
+#pragma unroll 4
+          for (int j = 0; j < 8; ++j) {
+            const uint4 v = load8(reinterpret_cast<const T*>(from) + 8 * j, valid - 8 * j, p.second_aligned != 0);
+            sts128(dst + half * (G::operand_bytes / 2) + ((j << 4) ^ swz), v.x, v.y, v.z, v.w);
+          }
         }
       }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      if (TRANS) {
+        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        tc_fence_before();
+      } else asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars->a_full[buf]);
-      if (++stage == uint32_t(p.ring)) { stage = 0; phase ^= 1u; }
-      if (++buf == 2) { buf = 0; buf_phase ^= 1u; }
+      if ((buf += p.groups) >= uint32_t(p.bufs)) buf -= p.bufs;
+      stage += p.groups;
+      while (stage >= uint32_t(p.ring)) { stage -= p.ring; phase ^= 1u; }
     }
     // ---- accumulators: to Y, or to shared memory for the cluster's sum ----
-    ok = __all_sync(~0u, ok && mbar_wait(&bars->done, 0u, abort_flag, p.status, 19u));
+    ok = ok && warp_wait<true>(&bars->done, 0u, abort_flag, p.status, 19u);
     if (ok) {
       tc_fence_after();
-      const int quarter = warp & 3, side = (warp - 2) >> 2, o = quarter * 32 + lane, out = tile * kOut + o;
+      const int quarter = warp & 3, side = (warp - 2 - kLoaders) >> 2, o = quarter * 32 + lane, out = tile * kOut + o;
       const uint32_t addr = tmem + (uint32_t(quarter * 32) << 16);
       float* red = reinterpret_cast<float*>(aligned);
-      for (int c = side * (p.nt / 2); c < (side + 1) * (p.nt / 2); c += 8) {
+      for (int c = side * 8; c < p.nt; c += 8 * kGroups) {
         if (p.splits == 1 && t0 + c >= p.t) break;
         float v[8];
         tmem_ld8(addr + c, v);
@@ -313,13 +492,6 @@ product_umma_kernel(const __grid_constant__ CUtensorMap code_map, const __grid_c
 }
 
 // ---- mid = first^T X for many tokens, as two 16-bit parts: [token][value 0 .. rank, remainder 0 .. rank] ----------------------
-template <class T> __device__ __forceinline__ uint4 load8(const T* p, int valid, bool aligned) {
-  if (valid >= 8 && aligned) return *reinterpret_cast<const uint4*>(p);
-  uint32_t o[4] = {0, 0, 0, 0};
-#pragma unroll
-  for (int e = 0; e < 8; ++e) if (e < valid) o[e >> 1] |= uint32_t(reinterpret_cast<const uint16_t*>(p)[e]) << (16 * (e & 1));
-  return make_uint4(o[0], o[1], o[2], o[3]);
-}
 template <class T> __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1);
 template <> __device__ __forceinline__ void mma16816<__half>(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -392,12 +564,12 @@ bool encode_2d(CUtensorMap* map, CUtensorMapDataType type, const void* ptr, uint
   return r == CUDA_SUCCESS;
 }
 
-// CTAs that share a tile's K steps: the whole takes ceil(tiles s / SMs) rounds of ceil(steps / s) steps plus about six steps' worth of
+// CTAs that share a tile's K steps: the whole takes ceil(tiles s / slots) rounds of ceil(steps / s) steps plus `overhead` steps' worth of
 // start, drain and exchange.
-int choose_splits(int64_t tiles, int steps, int sms) {
+int choose_splits(int64_t tiles, int steps, int slots, int overhead) {
   int best = 1; double cost = 1e300;
   for (int s = 1; s <= 8 && s * 2 <= std::max(steps, 2); ++s) {
-    const double c = double((tiles * s + sms - 1) / sms) * ((steps + s - 1) / s + 6.);
+    const double c = double((tiles * s + slots - 1) / slots) * ((steps + s - 1) / s + overhead);
     if (c < cost * 0.999) { cost = c; best = s; }
   }
   return best;
@@ -429,25 +601,40 @@ template <class T, bool TRANS> int32_t launch(const hyacinHandle_t* handle, cons
   p.scales = a.scales; p.zeros = a.zeros; p.lds = a.lds; p.m = a.m; p.n = a.n; p.t = a.t; p.out = out;
   p.segs = (a.m + a.seg - 1) / a.seg; p.seg_sub = a.seg / 32; p.seg_shift = -1;
   for (int s = 0; s < 27; ++s) if (p.seg_sub == 1 << s) p.seg_shift = s;
+  // two or four segments per block of 128 rows, fetched at once where the table's rows allow it
+  const int per_block = p.seg_sub == 1 ? 4 : p.seg_sub == 2 ? 2 : 1;
+  p.wide = per_block > 1 && a.lds % per_block == 0 && reinterpret_cast<uintptr_t>(a.scales) % (2 * per_block) == 0 &&
+           reinterpret_cast<uintptr_t>(a.zeros) % per_block == 0 ? per_block : 1;
+  using G = Geometry<TRANS>;
+  constexpr int kStep = G::step;
   p.code_steps = (in + kStep - 1) / kStep;
   p.rank = a.rank; p.second = a.second; p.ld2 = a.ld2; p.y = a.y; p.ldy = a.ldy;
   p.steps = p.code_steps + (2 * a.rank + kStep - 1) / kStep;
-  const int64_t token_tiles = (int64_t(a.t) + 255) / 256;
+  const int64_t token_tiles = (int64_t(a.t) + kMaxTokens - 1) / kMaxTokens;
   p.nt = int((int64_t(a.t) + token_tiles - 1) / token_tiles + 15) / 16 * 16;
+  p.nt_cols = (p.nt + 31) / 32 * 32;
+
+  const uint32_t x_bytes = uint32_t(p.nt) * kStep * 2, stage_bytes = G::code_bytes + x_bytes + G::scale_bytes;
+  // operand buffers: as many as leave the ring as many stages; with 'T' they share the 512 columns with the accumulators
+  const uint32_t fixed = 1024 + sizeof(UmmaBars);
+  p.bufs = TRANS ? std::min<int>(kMaxBufs, (512 - p.nt_cols) / std::max<uint32_t>(G::operand_cols, 1)) : kMaxBufs;
+  for (;; --p.bufs) {
+    p.ring = int(std::min<uint32_t>(kMaxRing, (kSmemLimit - fixed - p.bufs * G::operand_bytes) / stage_bytes));
+    if (p.ring >= p.bufs) break;
+  }
+  p.groups = std::min(kGroups, p.bufs);
   p.tmem_cols = 32;
-  while (p.tmem_cols < uint32_t(p.nt)) p.tmem_cols *= 2;
-  const uint32_t x_bytes = uint32_t(p.nt) * kStep * 2;
-  const uint32_t fixed = 2 * kOperandBytes + 1024 + sizeof(UmmaBars);
-  p.ring = int(std::min<uint32_t>(kMaxRing, (kSmemLimit - fixed) / (kCodeBytes + x_bytes)));
-  const uint32_t smem = fixed + p.ring * (kCodeBytes + x_bytes);
+  while (p.tmem_cols < p.nt_cols + p.bufs * G::operand_cols) p.tmem_cols *= 2;
+  const uint32_t smem = std::max(fixed + p.bufs * G::operand_bytes + p.ring * stage_bytes, kSmemFloor);
+  p.second_aligned = reinterpret_cast<uintptr_t>(a.second) % 16 == 0 && a.ld2 % 8 == 0;
   const int tiles = (out + kOut - 1) / kOut;
-  p.splits = choose_splits(int64_t(tiles) * token_tiles, p.steps, handle->DeviceSMs);
+  p.splits = choose_splits(int64_t(tiles) * token_tiles, p.steps, handle->DeviceSMs, TRANS ? 6 : 12);
   const uint32_t fmt = type == HYACIN_F16 ? 0u : 1u;
   p.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((TRANS ? 0u : 1u) << 15) | (uint32_t(p.nt >> 3) << 17) | (uint32_t(kOut >> 4) << 24);
   p.status = status_word_device(handle->DeviceID);
   const CUtensorMapDataType dt = type == HYACIN_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   CUtensorMap code_map{}, x_map{}, mid_map{};
-  bool fine = encode_2d(&code_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.codes, uint64_t((a.m + 127) / 128) * 64, a.n, a.ldq, 64, 128, CU_TENSOR_MAP_SWIZZLE_64B) &&
+  bool fine = encode_2d(&code_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.codes, uint64_t((a.m + 127) / 128) * 64, a.n, a.ldq, 64, G::cols, CU_TENSOR_MAP_SWIZZLE_64B) &&
               encode_2d(&x_map, dt, x, in, a.t, uint64_t(ldx) * 2, 64, p.nt, CU_TENSOR_MAP_SWIZZLE_128B);
   mid_map = x_map;
   if (fine && a.rank) {
