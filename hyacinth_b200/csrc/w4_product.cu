@@ -89,6 +89,7 @@ extern "C" int32_t hyacinB200ProductW4(const hyacinHandle_t* handle, char opW, i
   if (!trans && opW != 'N' && opW != 'n') return w4_refuse(fn, "opW must be 'T' or 'N'");
   if (!is_w4_type(Xtype)) return w4_refuse(fn, "type not supported");
   if (M < 0 || N < 0 || T < 0 || rank < 0 || segM <= 0 || segM % 32) return w4_refuse(fn, "sizes: M, N, T, rank >= 0 and segM a positive multiple of 32");
+  if (M > 0x7fffff00 || N > 0x7fffff00 || T > 0x7fffff00) return w4_refuse(fn, "sizes: M, N, T at most 2^31 - 256");
   const int in = trans ? M : N, out = trans ? N : M;
   if (T == 0 || out == 0) return 0;
   if (!Y || ldy < out) return w4_refuse(fn, "Y: null or leading dimension too small");
@@ -105,7 +106,11 @@ extern "C" int32_t hyacinB200ProductW4(const hyacinHandle_t* handle, char opW, i
   static_cast<ProductArgs&>(a) = ProductArgs{codes, ldq, M, N, T, segM, scales, zeros, lds, X, ldx, in > 0 ? rank : 0,
                                              trans ? U : V, trans ? ldu : ldv, trans ? V : U, trans ? ldv : ldu, Y, ldy};
   timer_mark(handle, Segment::Replicated);
-  if (in > 0 && Xtype != HYACIN_F32 && (!trans || T > 16)) return launch_product_umma(handle, fn, trans, Xtype, a);
+  if (in > 0 && trans) {
+    const int per = product_stream_vectors(Xtype, a);
+    if (per > 0 && (Xtype == HYACIN_F32 || (T + per - 1) / per <= 2)) return launch_product_stream(handle, fn, Xtype, a);
+  }
+  if (in > 0 && Xtype != HYACIN_F32) return launch_product_umma(handle, fn, trans, Xtype, a);
   float* mid = nullptr;
   int32_t rc = 0;
   with_w4_type(Xtype, [&](auto tag) {

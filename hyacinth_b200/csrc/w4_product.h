@@ -16,4 +16,8 @@ struct ProductArgs {
 // Fifth-generation tensor cores, 16-bit types, both directions.  Returns 0 or -3.
 int32_t launch_product_umma(const hyacinHandle_t* handle, const char* fn, bool trans, hyacinPrecision_t type, const ProductArgs& a);
 
+// Few vectors, opW 'T', all types, any number of passes over W; product_stream_vectors: vectors per pass (0: not even one fits).
+int product_stream_vectors(hyacinPrecision_t type, const ProductArgs& a);
+int32_t launch_product_stream(const hyacinHandle_t* handle, const char* fn, hyacinPrecision_t type, const ProductArgs& a);
+
 }  // namespace hyb
