@@ -108,7 +108,7 @@ extern "C" int32_t hyacinB200ProductW4(const hyacinHandle_t* handle, char opW, i
   timer_mark(handle, Segment::Replicated);
   if (in > 0 && trans) {
     const int per = product_stream_vectors(Xtype, a);
-    if (per > 0 && (Xtype == HYACIN_F32 || (T + per - 1) / per <= 2)) return launch_product_stream(handle, fn, Xtype, a);
+    if (per > 0 && (Xtype == HYACIN_F32 || (T <= 8 && per >= T))) return launch_product_stream(handle, fn, Xtype, a);
   }
   if (in > 0 && Xtype != HYACIN_F32) return launch_product_umma(handle, fn, trans, Xtype, a);
   float* mid = nullptr;

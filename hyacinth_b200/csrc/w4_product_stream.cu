@@ -9,12 +9,13 @@
 // 16 bits is that of Y.  Single-precision x is split into three bfloat16 parts of 8 bits that add up to it exactly, three columns
 // of the right-hand operand, and multiplies the exact whole numbers q - zero: the result is that of 32-bit sums.
 // Layout.  A CTA (one per SM) takes every 148th tile of 16 columns, the rows of the m16n8k16 instruction.  A column's codes are
-// contiguous; a stage of the ring holds 2048 rows of the tile, 1 KiB per column, one TMA box, so the copies for the next
-// stages and tiles are in flight all the time (up to 190 KiB per SM) whatever the arithmetic does.  Each of 8 warps takes two
-// blocks of 128 rows of the stage.  Lane (g, c) reads quarter c of the block's 64 bytes of columns g and g + 8: four words, word i
+// contiguous; a stage of the ring holds 4096 rows of the tile (2048 for more than eight operand columns), one TMA box, so the copies for the next
+// stages and tiles are in flight all the time (up to 190 KiB per SM) whatever the arithmetic does.  Each of 16 warps takes two
+// blocks of 128 rows of the stage (one).  Lane (g, c) reads quarter c of the block's 64 bytes of columns g and g + 8: four words, word i
 // holding rows 32 i + 8 c .. + 7.  The order of K inside an instruction is free as long as both operands use the same one, so the
 // lane's four code pairs of a word meet the lane's 16 bytes of x for those eight rows, read from shared memory in their natural
-// order.  Four more warps fetch scales and zero points, coalesced along a table row, into the same ring.
+// order.  Six more warps fetch scales and zero points, coalesced along a table row, into the
+// same ring, and one adds the partial sums of the multiplying warps.
 // Bound.  DRAM, at 23 bytes per clock and SM: 710 cycles for a stage of 16 KiB, for which the extraction takes 450 cycles of the
 // integer pipe (7 instructions per eight codes at half rate) and the matrix pipe 256 per eight vectors.
 #include "w4_product.h"
@@ -28,13 +29,13 @@ namespace {
 using namespace ptx;
 
 constexpr int kTile = 16;                         // columns
-constexpr int kWarps = 8;                         // multiplying warps
-constexpr int kPer = 2;                           // blocks of 128 rows a warp takes from a stage
-constexpr int kStageBlocks = kWarps * kPer;
-constexpr int kLoaders = 4;                       // warps that fetch scales
-constexpr int kThreads = 32 * (kWarps + kLoaders + 1);
-constexpr int kColumnPitch = kStageBlocks * 64;   // bytes of a column in a stage
-constexpr int kMaxRing = 12;
+constexpr int kWarps = 16;                        // multiplying warps
+// blocks of 128 rows a warp takes from a stage: two while x leaves room for four such stages
+__host__ __device__ constexpr int blocks_per_warp(int tiles) { return tiles == 1 ? 2 : 1; }
+constexpr int kLoaders = 6;                       // warps that fetch scales
+constexpr int kJoints = 2;                        // buffers for the partial sums of a tile
+constexpr int kThreads = 32 * (kWarps + kLoaders + 2);
+constexpr int kMaxRing = 8;
 constexpr int kSmemLimit = 232448;
 
 struct StreamParams {
@@ -49,7 +50,7 @@ struct StreamParams {
   uint32_t* status;
 };
 
-struct StreamBars { uint64_t full[kMaxRing], empty[kMaxRing]; uint32_t abort_flag; };
+struct StreamBars { uint64_t full[kMaxRing], empty[kMaxRing], joint_full[kJoints], joint_empty[kJoints]; uint32_t abort_flag; };
 
 // Two codes each: offset + q as extracted.
 template <bool HALF> struct Codes;
@@ -67,9 +68,15 @@ template <> struct Codes<false> {      // 0x4300 | q = 128 + q
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   }
 };
+// (w & mask) | bits in one instruction: left to the compiler, two constants became two instructions
+__device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask, uint32_t bits) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(w), "r"(mask), "r"(bits));
+  return r;
+}
 template <bool HALF> __device__ __forceinline__ void code_pairs(uint32_t w, uint32_t (&o)[4]) {
 #pragma unroll
-  for (int p = 0; p < 4; ++p) o[p] = ((w >> (4 * p)) & 0x000f000fu) | Codes<HALF>::kBits;
+  for (int p = 0; p < 4; ++p) o[p] = and_or(w >> (4 * p), 0x000f000fu, Codes<HALF>::kBits);
 }
 // bfloat16 pairs q - zero
 __device__ __forceinline__ void subtract_zero(uint32_t (&o)[4], int zero) {
@@ -111,84 +118,36 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volati
   return false;
 }
 
-// X: type of x; TILES: eights of operand columns (vectors, or their parts); FINE: segments shorter than a block or not a multiple of it.
-template <class X, int TILES, bool FINE>
+// X: type of x; TILES: eights of operand columns (vectors, or their parts); GRAIN: 32-row subsets that share a scale for sure: 4 when
+// segments are whole blocks, else 2 or 1.
+template <class X, int TILES, int GRAIN>
 __global__ void __launch_bounds__(kThreads, 1) product_stream_kernel(const __grid_constant__ CUtensorMap code_map, const __grid_constant__ StreamParams p) {
   constexpr bool kSplit = sizeof(X) == 4, kHalf = std::is_same<X, __half>::value;
-  constexpr int kPairs = FINE ? 4 * kStageBlocks + 1 : kStageBlocks + 1;       // scales of a column in a stage; odd, so that columns fall into different banks
+  constexpr int kPer = blocks_per_warp(TILES), kStageBlocks = kWarps * kPer, kColumnPitch = kStageBlocks * 64;      // pitch: bytes of a column in a stage
+  constexpr int kPairs = 4 / GRAIN * kStageBlocks + 1;       // scales of a column in a stage; odd, so that columns fall into different banks
   constexpr int kRed = 8 * TILES + 1;
   extern __shared__ __align__(128) uint8_t smem[];
   uint16_t* xs = reinterpret_cast<uint16_t*>(smem);                // [operand column][row]
   float* sums = reinterpret_cast<float*>(smem + p.sums_at);        // [segment of a block][operand column]: sum of x over it
   uint8_t* ring = smem + p.ring_at;
   Pair<X>* pairs = reinterpret_cast<Pair<X>*>(smem + p.pairs_at);  // [stage][column][segment of the stage]
-  float* red = reinterpret_cast<float*>(smem + p.red_at);          // [parity][warp][column][operand column]
+  float* red = reinterpret_cast<float*>(smem + p.red_at);          // [joint][warp][column][operand column]
   StreamBars* bars = reinterpret_cast<StreamBars*>(smem + p.bars_at);
   volatile uint32_t* abort_flag = &bars->abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int tiles = (p.n + kTile - 1) / kTile, stages = (p.blocks + kStageBlocks - 1) / kStageBlocks;      // stages per tile
 
-  // stage number `at` of this CTA: tile blockIdx.x + (at / stages) gridDim.x, rows (at % stages) 2048 ...
+  // stage number `at` of this CTA: tile blockIdx.x + (at / stages) gridDim.x, chunk at % stages of the rows
   const int my_tiles = (tiles - int(blockIdx.x) + int(gridDim.x) - 1) / int(gridDim.x), total = my_tiles * stages;
   auto copy = [&](int tile, int chunk, int stage) {
     mbar_expect_tx(&bars->full[stage], kTile * kColumnPitch);
     tma_load_2d(smem_u32(ring) + stage * kTile * kColumnPitch, &code_map, &bars->full[stage], chunk * (kColumnPitch / 8), tile * kTile);
   };
-  if (warp == 0) {
-    if (lane == 0) {
-      for (int s = 0; s < p.ring; ++s) { mbar_init(&bars->full[s], 2); mbar_init(&bars->empty[s], kWarps); }
-      bars->abort_flag = 0;
-      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-      // the first copies start before the block has met
-      for (int at = 0, tile = blockIdx.x, chunk = 0; at < total && at < p.ring; ++at) {
-        copy(tile, chunk, at);
-        if (++chunk == stages) { chunk = 0; tile += gridDim.x; }
-      }
-    }
-  } else {
-    // x, one operand column per line, zeros behind the last row, and its sums per segment
-    const int rows = p.blocks * kW4Block, tid = threadIdx.x - 32, step = kThreads - 32;
-    if constexpr (kSplit) {
-      for (int t = 0; t < p.t; ++t)
-        for (int r = tid; r < rows; r += step) {
-          float v = r < p.m ? static_cast<const float*>(p.x)[t * p.ldx + r] : 0.f;
-#pragma unroll
-          for (int k = 0; k < 3; ++k) {
-            const __nv_bfloat16 h = __float2bfloat16_rz(v);
-            xs[(3 * t + k) * p.pitch + r] = __bfloat16_as_ushort(h);
-            v = fabsf(v) <= 3.402823466e38f ? v - __bfloat162float(h) : 0.f;
-          }
-        }
-    } else {
-      // eight rows per thread; sixteen threads share a block and take part together
-#pragma unroll 1
-      for (int t = 0; t < p.t; ++t)
-#pragma unroll 2
-        for (int r = tid * 8; r < rows; r += step * 8) {
-          const int valid = p.m - r;
-          const uint16_t* src = static_cast<const uint16_t*>(p.x) + t * p.ldx + r;
-          uint4 v;
-          if (p.x_aligned && valid >= 8) v = *reinterpret_cast<const uint4*>(src);
-          else {
-            uint32_t o[4] = {0, 0, 0, 0};
-#pragma unroll
-            for (int i = 0; i < 8; ++i) if (i < valid) o[i >> 1] |= uint32_t(src[i]) << (16 * (i & 1));
-            v = make_uint4(o[0], o[1], o[2], o[3]);
-          }
-          *reinterpret_cast<uint4*>(xs + t * p.pitch + r) = v;
-          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-          float s = 0.f;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint16_t lo = uint16_t(w[i]), hi = uint16_t(w[i] >> 16);
-            s += to_f32(*reinterpret_cast<const X*>(&lo)) + to_f32(*reinterpret_cast<const X*>(&hi));
-          }
-          const uint32_t mask = lane < 16 ? 0x0000ffffu : 0xffff0000u;
-#pragma unroll
-          for (int d = 1; d < (FINE ? 4 : 16); d *= 2) s += __shfl_xor_sync(mask, s, d);
-          if ((r / 8) % (FINE ? 4 : 16) == 0) sums[r / (FINE ? 32 : 128) * (8 * TILES) + t] = s;
-        }
-    }
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < p.ring; ++s) { mbar_init(&bars->full[s], 2); mbar_init(&bars->empty[s], kWarps); }
+    for (int j = 0; j < kJoints; ++j) { mbar_init(&bars->joint_full[j], kWarps); mbar_init(&bars->joint_empty[j], 1); }
+    bars->abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   __syncthreads();
 
@@ -197,11 +156,9 @@ __global__ void __launch_bounds__(kThreads, 1) product_stream_kernel(const __gri
     // ---- codes ----
     int tile = blockIdx.x, chunk = 0; uint32_t stage = 0, phase = 0;
     for (int at = 0; at < total; ++at) {
-      if (at >= p.ring) {
-        if (!(ok = warp_wait(&bars->empty[stage], phase ^ 1u, abort_flag, p.status, 31u))) break;
-        if (lane == 0) copy(tile, chunk, stage);
-        __syncwarp();
-      }
+      if (at >= p.ring && !(ok = warp_wait(&bars->empty[stage], phase ^ 1u, abort_flag, p.status, 31u))) break;
+      if (lane == 0) copy(tile, chunk, stage);
+      __syncwarp();
       if (++chunk == stages) { chunk = 0; tile += gridDim.x; }
       if (++stage == uint32_t(p.ring)) { stage = 0; phase ^= 1u; }
     }
@@ -232,17 +189,17 @@ __global__ void __launch_bounds__(kThreads, 1) product_stream_kernel(const __gri
       for (int s0 = 0; s0 < count; s0 += 32) {
         const int s = s0 + (lane & ((1 << log) - 1));
 #pragma unroll 1
-        for (int c0 = 0; c0 < cols; c0 += 8 * step) {
-          X scale[8]; uint8_t zero[8];
+        for (int c0 = 0; c0 < cols; c0 += 16 * step) {
+          X scale[16]; uint8_t zero[16];
 #pragma unroll
-          for (int u = 0; u < 8; ++u) {
+          for (int u = 0; u < 16; ++u) {
             const int col = c0 + first + u * step;
             const int64_t at_table = int64_t(tile * kTile + col) * p.lds + seg0 + s;
             if (col < cols && s < count) { scale[u] = static_cast<const X*>(p.scales)[at_table]; zero[u] = p.zeros ? p.zeros[at_table] : uint8_t(8); }
           }
           if (!waited) { if (!(ok = warp_wait(&bars->empty[stage], phase ^ 1u, abort_flag, p.status, 33u))) break; waited = true; }
 #pragma unroll
-          for (int u = 0; u < 8; ++u) {
+          for (int u = 0; u < 16; ++u) {
             const int col = c0 + first + u * step;
             if (col < cols && s < count) out[col * kPairs + s] = make_pair<X>(scale[u], int(zero[u]));
           }
@@ -253,78 +210,145 @@ __global__ void __launch_bounds__(kThreads, 1) product_stream_kernel(const __gri
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars->full[stage]);
     }
+  } else if (warp == 1 + kLoaders) {
+    // ---- joining: adds the multiplying warps' partial sums of a tile, so that they need not wait for one another ----
+    uint32_t joint = 0, phase = 0;
+    for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+      if (!(ok = warp_wait(&bars->joint_full[joint], phase, abort_flag, p.status, 35u))) break;
+#pragma unroll 2
+      for (int e = lane; e < kTile * p.t; e += 32) {
+        const int col = e & (kTile - 1), t = e / kTile, out = tile * kTile + col;
+        const float* from = red + joint * kWarps * kTile * kRed + col * kRed + (kSplit ? 3 * t : t);
+        float v = 0.f;
+#pragma unroll
+        for (int q = 0; q < kWarps; ++q)
+#pragma unroll
+          for (int i = 0; i < (kSplit ? 3 : 1); ++i) v += from[q * kTile * kRed + i];
+        if (out < p.n) static_cast<X*>(p.y)[int64_t(t) * p.ldy + out] = from_f32<X>(v);
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->joint_empty[joint]);
+      if (++joint == kJoints) { joint = 0; phase ^= 1u; }
+    }
   } else {
     // ---- products ----
-    const int w = warp - 1 - kLoaders, g = lane >> 2, c = lane & 3;
+    const int w = warp - 2 - kLoaders, g = lane >> 2, c = lane & 3;
+    // First x, one operand column per line, zeros behind the last row, and its sums per segment, while the first codes arrive.
+    {
+      const int rows = p.blocks * kW4Block, tid = threadIdx.x - 32 * (2 + kLoaders), step = kWarps * 32;
+      if constexpr (kSplit) {
+        for (int t = 0; t < p.t; ++t)
+#pragma unroll 4
+          for (int r = tid; r < rows; r += step) {
+            float v = r < p.m ? __ldg(static_cast<const float*>(p.x) + t * p.ldx + r) : 0.f;
+#pragma unroll
+            for (int k = 0; k < 3; ++k) {
+              const __nv_bfloat16 h = __float2bfloat16_rz(v);
+              xs[(3 * t + k) * p.pitch + r] = __bfloat16_as_ushort(h);
+              v = fabsf(v) <= 3.402823466e38f ? v - __bfloat162float(h) : 0.f;
+            }
+          }
+      } else {
+        // eight rows per thread and step; the threads of a block are neighbours in one half of a warp (rows / 8 is a multiple of 16)
+        const int per = rows / 8, chunks = p.t * per;
+#pragma unroll 4
+        for (int e = tid; e < chunks; e += step) {
+          const int t = e / per, r = (e - t * per) * 8, valid = p.m - r;
+          const uint16_t* src = static_cast<const uint16_t*>(p.x) + t * p.ldx + r;
+          uint4 v;
+          if (p.x_aligned && valid >= 8) v = __ldg(reinterpret_cast<const uint4*>(src));
+          else {
+            uint32_t o[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < 8; ++i) if (i < valid) o[i >> 1] |= uint32_t(__ldg(src + i)) << (16 * (i & 1));
+            v = make_uint4(o[0], o[1], o[2], o[3]);
+          }
+          *reinterpret_cast<uint4*>(xs + t * p.pitch + r) = v;
+          const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+          float s = 0.f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint16_t lo = uint16_t(u[i]), hi = uint16_t(u[i] >> 16);
+            s += to_f32(*reinterpret_cast<const X*>(&lo)) + to_f32(*reinterpret_cast<const X*>(&hi));
+          }
+          const uint32_t mask = lane < 16 ? 0x0000ffffu : 0xffff0000u;
+#pragma unroll
+          for (int d = 1; d < 4 * GRAIN; d *= 2) s += __shfl_xor_sync(mask, s, d);
+          if ((r / 8) % (4 * GRAIN) == 0) sums[r / (32 * GRAIN) * (8 * TILES) + t] = s;
+        }
+      }
+      asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory");
+    }
     const uint16_t* xl[TILES];
 #pragma unroll
     for (int j = 0; j < TILES; ++j) xl[j] = xs + min(8 * j + g, p.cols - 1) * p.pitch + 8 * c;
-    uint32_t stage = 0, phase = 0, parity = 0;
-    for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x, parity ^= 1u) {
+    uint32_t stage = 0, phase = 0, joint = 0, joint_phase = 0;
+    for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
       float sum[TILES][4] = {};
       for (int chunk = 0; chunk < stages; ++chunk) {
         if (!(ok = warp_wait(&bars->full[stage], phase, abort_flag, p.status, 34u))) break;
-        uint4 qs[kPer][2];
-#pragma unroll
-        for (int u = 0; u < kPer; ++u) {
-          const uint8_t* from = ring + (stage * kTile + g) * kColumnPitch + (u * kWarps + w) * 64 + c * 16;
-          qs[u][0] = *reinterpret_cast<const uint4*>(from); qs[u][1] = *reinterpret_cast<const uint4*>(from + 8 * kColumnPitch);
-        }
+        const uint8_t* from = ring + (stage * kTile + g) * kColumnPitch + w * 64 + c * 16;
         const Pair<X>* pa = pairs + (stage * kTile + g) * kPairs - segment_of(chunk * kStageBlocks * 4, p);
         const Pair<X>* pb = pa + 8 * kPairs;
+        // one block: (offset + q) x in the matrix pipe on top of -(offset + zero) sum x, times the scale
+        auto block = [&](int b, const uint4& qa, const uint4& qb) {
 #pragma unroll
-        for (int u = 0; u < kPer; ++u) {
-          const int b = chunk * kStageBlocks + u * kWarps + w;
-          if (b >= p.blocks) break;
-          const uint4 qa = qs[u][0], qb = qs[u][1];
-          float acc[TILES][4] = {}, odd[TILES][4] = {};            // two chains of instructions that do not wait for each other
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint32_t a[4], e[4];
-            code_pairs<kHalf>(i == 0 ? qa.x : i == 1 ? qa.y : i == 2 ? qa.z : qa.w, a);
-            code_pairs<kHalf>(i == 0 ? qb.x : i == 1 ? qb.y : i == 2 ? qb.z : qb.w, e);
+          for (int i0 = 0; i0 < 4; i0 += GRAIN) {
             // rows behind the last one meet zeros of x under the last segment's scale
-            const int seg = FINE ? min(segment_of(4 * b + i, p), p.segs - 1) : segment_of(4 * b, p);
-            if constexpr (kSplit) { subtract_zero(a, pa[seg].zero); subtract_zero(e, pb[seg].zero); }
+            const int seg = GRAIN < 4 ? min(segment_of(4 * b + i0, p), p.segs - 1) : segment_of(4 * b, p);
+            const Pair<X> va = pa[seg], vb = pb[seg];
+            float acc[TILES][4] = {}, odd[TILES][4] = {};          // two chains of instructions that do not wait for each other
+            float sa, sb;
+            if constexpr (kSplit) { sa = va.scale; sb = vb.scale; }
+            else {
+              const float2 fa = unpack_pair(va), fb = unpack_pair(vb);
+              sa = fa.x; sb = fb.x;
+#pragma unroll
+              for (int j = 0; j < TILES; ++j) {
+                const float2 sx = *reinterpret_cast<const float2*>(sums + (4 * b + i0) / GRAIN * (8 * TILES) + 8 * j + 2 * c);
+                acc[j][0] = -fa.y * sx.x; acc[j][1] = -fa.y * sx.y; acc[j][2] = -fb.y * sx.x; acc[j][3] = -fb.y * sx.y;
+              }
+            }
+#pragma unroll
+            for (int i = i0; i < i0 + GRAIN; ++i) {
+              uint32_t a[4], e[4];
+              code_pairs<kHalf>(i == 0 ? qa.x : i == 1 ? qa.y : i == 2 ? qa.z : qa.w, a);
+              code_pairs<kHalf>(i == 0 ? qb.x : i == 1 ? qb.y : i == 2 ? qb.z : qb.w, e);
+              if constexpr (kSplit) { subtract_zero(a, va.zero); subtract_zero(e, vb.zero); }
+#pragma unroll
+              for (int j = 0; j < TILES; ++j) {
+                const uint4 x = *reinterpret_cast<const uint4*>(xl[j] + b * kW4Block + 32 * i);
+                Codes<kHalf>::mma(acc[j], a[0], e[0], a[1], e[1], x.x, x.y);
+                if (GRAIN > 1) Codes<kHalf>::mma(odd[j], a[2], e[2], a[3], e[3], x.z, x.w);
+                else Codes<kHalf>::mma(acc[j], a[2], e[2], a[3], e[3], x.z, x.w);
+              }
+            }
 #pragma unroll
             for (int j = 0; j < TILES; ++j) {
-              const uint4 x = *reinterpret_cast<const uint4*>(xl[j] + b * kW4Block + 32 * i);
-              Codes<kHalf>::mma(acc[j], a[0], e[0], a[1], e[1], x.x, x.y);
-              Codes<kHalf>::mma(odd[j], a[2], e[2], a[3], e[3], x.z, x.w);
-            }
-            if (FINE || i == 3) {
-#pragma unroll
-              for (int j = 0; j < TILES; ++j)
+              if (GRAIN > 1)
 #pragma unroll
                 for (int q = 0; q < 4; ++q) acc[j][q] += odd[j][q];
-              if constexpr (kSplit) {
-                const float sa = pa[seg].scale, sb = pb[seg].scale;
-#pragma unroll
-                for (int j = 0; j < TILES; ++j) {
-                  sum[j][0] += sa * acc[j][0]; sum[j][1] += sa * acc[j][1]; sum[j][2] += sb * acc[j][2]; sum[j][3] += sb * acc[j][3];
-                }
-              } else {
-                const float2 fa = unpack_pair(pa[seg]), fb = unpack_pair(pb[seg]);
-#pragma unroll
-                for (int j = 0; j < TILES; ++j) {
-                  const float2 sx = *reinterpret_cast<const float2*>(sums + (FINE ? 4 * b + i : b) * (8 * TILES) + 8 * j + 2 * c);
-                  sum[j][0] += fa.x * (acc[j][0] - fa.y * sx.x); sum[j][1] += fa.x * (acc[j][1] - fa.y * sx.y);
-                  sum[j][2] += fb.x * (acc[j][2] - fb.y * sx.x); sum[j][3] += fb.x * (acc[j][3] - fb.y * sx.y);
-                }
-              }
-              if (FINE) {
-#pragma unroll
-                for (int j = 0; j < TILES; ++j)
-#pragma unroll
-                  for (int q = 0; q < 4; ++q) acc[j][q] = odd[j][q] = 0.f;
-              }
+              sum[j][0] += sa * acc[j][0]; sum[j][1] += sa * acc[j][1]; sum[j][2] += sb * acc[j][2]; sum[j][3] += sb * acc[j][3];
             }
           }
+        };
+        const int b0 = chunk * kStageBlocks + w;
+        if (b0 + (kPer - 1) * kWarps < p.blocks) {
+          uint4 q[kPer][2];
+#pragma unroll
+          for (int u = 0; u < kPer; ++u) { q[u][0] = *reinterpret_cast<const uint4*>(from + u * kWarps * 64); q[u][1] = *reinterpret_cast<const uint4*>(from + u * kWarps * 64 + 8 * kColumnPitch); }
+#pragma unroll
+          for (int u = 0; u < kPer; ++u) block(b0 + u * kWarps, q[u][0], q[u][1]);
+        } else {
+#pragma unroll 1
+          for (int u = 0; b0 + u * kWarps < p.blocks; ++u)
+            block(b0 + u * kWarps, *reinterpret_cast<const uint4*>(from + u * kWarps * 64), *reinterpret_cast<const uint4*>(from + u * kWarps * 64 + 8 * kColumnPitch));
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars->empty[stage]);
         if (++stage == uint32_t(p.ring)) { stage = 0; phase ^= 1u; }
       }
+      if (!ok) break;
       // correction: this warp's share of the rank, straight into its partial sums (the first of the parts of a vector)
       if (p.rank) {
         asm volatile("griddepcontrol.wait;" ::: "memory");         // mid comes from the kernel before this one
@@ -345,26 +369,16 @@ __global__ void __launch_bounds__(kThreads, 1) product_stream_kernel(const __gri
             }
         }
       }
-      // the warps' partial sums meet in shared memory, in buffers that alternate from tile to tile
-      float* mine = red + (parity * kWarps + w) * kTile * kRed;
+      // the warps' partial sums meet in shared memory
+      if (!(ok = warp_wait(&bars->joint_empty[joint], joint_phase ^ 1u, abort_flag, p.status, 36u))) break;
+      float* mine = red + (joint * kWarps + w) * kTile * kRed;
 #pragma unroll
       for (int j = 0; j < TILES; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) mine[(g + 8 * (e >> 1)) * kRed + 8 * j + 2 * c + (e & 1)] = sum[j][e];
-      // the barrier also tells every warp whether one gave up: all leave at the same tile
-      uint32_t good = ok;
-      asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %0, 0;\n\tbar.red.and.pred q, 1, %1, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "+r"(good) : "n"(kWarps * 32) : "memory");
-      ok = good != 0;
-      for (int e = threadIdx.x - 32 * (1 + kLoaders); e < kTile * p.t; e += kWarps * 32) {
-        const int col = e & (kTile - 1), t = e / kTile, out = tile * kTile + col;
-        const float* from = red + parity * kWarps * kTile * kRed + col * kRed + (kSplit ? 3 * t : t);
-        float v = 0.f;
-#pragma unroll
-        for (int q = 0; q < kWarps; ++q)
-#pragma unroll
-          for (int i = 0; i < (kSplit ? 3 : 1); ++i) v += from[q * kTile * kRed + i];
-        if (out < p.n) static_cast<X*>(p.y)[int64_t(t) * p.ldy + out] = from_f32<X>(v);
-      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->joint_full[joint]);
+      if (++joint == kJoints) { joint = 0; joint_phase ^= 1u; }
     }
   }
 }
@@ -413,8 +427,8 @@ template <class X> __global__ void __launch_bounds__(256) mid_kernel(const X* fi
   }
 }
 
-template <class X, int TILES, bool FINE> cudaError_t start(const hyacinHandle_t* handle, const CUtensorMap& map, const StreamParams& p, int smem) {
-  auto* kernel = product_stream_kernel<X, TILES, FINE>;
+template <class X, int TILES, int GRAIN> cudaError_t start(const hyacinHandle_t* handle, const CUtensorMap& map, const StreamParams& p, int smem) {
+  auto* kernel = product_stream_kernel<X, TILES, GRAIN>;
   static std::atomic<uint64_t> ready{0};                           // per device: shared memory limit raised
   const uint64_t bit = uint64_t(1) << (handle->DeviceID & 63);
   if (!(ready.load() & bit)) {
@@ -431,8 +445,8 @@ template <class X, int TILES, bool FINE> cudaError_t start(const hyacinHandle_t*
   return cudaLaunchKernelEx(&cfg, kernel, map, p);
 }
 
-template <class X, bool FINE> cudaError_t dispatch(const hyacinHandle_t* handle, const CUtensorMap& map, const StreamParams& p, int smem) {
-  return p.cols <= 8 ? start<X, 1, FINE>(handle, map, p, smem) : start<X, 2, FINE>(handle, map, p, smem);
+template <class X, int GRAIN> cudaError_t dispatch(const hyacinHandle_t* handle, const CUtensorMap& map, const StreamParams& p, int smem) {
+  return p.cols <= 8 ? start<X, 1, GRAIN>(handle, map, p, smem) : start<X, 2, GRAIN>(handle, map, p, smem);
 }
 
 constexpr int kMaxColumns = 16;
@@ -444,14 +458,14 @@ int place(StreamParams& p, hyacinPrecision_t type, const ProductArgs& a, int vec
   p.segs = (a.m + a.seg - 1) / a.seg; p.seg_sub = a.seg / 32; p.seg_shift = -1;
   for (int s = 0; s < 27; ++s) if (p.seg_sub == 1 << s) p.seg_shift = s;
   p.blocks = (a.m + kW4Block - 1) / kW4Block;
-  const bool fine = p.seg_sub % 4 != 0;
-  const int64_t tiles = p.cols > 8 ? 2 : 1, pitch = int64_t(p.blocks) * kW4Block + 32;      // 64 bytes over a multiple of 256: lanes g, g + 1 in different halves of the banks
-  const int64_t x_bytes = (p.cols * pitch * 2 + 127) / 128 * 128, sums = type == HYACIN_F32 ? 0 : (int64_t(p.blocks) * (fine ? 4 : 1) * 8 * tiles * 4 + 127) / 128 * 128;
-  const int64_t red = 2 * kWarps * kTile * (8 * tiles + 1) * 4, pair_stage = int64_t(kTile) * (fine ? 4 * kStageBlocks + 1 : kStageBlocks + 1) * (type == HYACIN_F32 ? 8 : 4);
-  const int64_t fixed = x_bytes + sums + red + int64_t(sizeof(StreamBars)), stage = kTile * kColumnPitch + pair_stage;
+  const int per_block = p.seg_sub % 4 == 0 ? 1 : p.seg_sub % 2 == 0 ? 2 : 4;
+  const int64_t tiles = p.cols > 8 ? 2 : 1, stage_blocks = kWarps * blocks_per_warp(int(tiles)), pitch = int64_t(p.blocks) * kW4Block + 32;      // 64 bytes over a multiple of 256: lanes g, g + 1 in different halves of the banks
+  const int64_t x_bytes = (p.cols * pitch * 2 + 127) / 128 * 128, sums = type == HYACIN_F32 ? 0 : (int64_t(p.blocks) * per_block * 8 * tiles * 4 + 127) / 128 * 128;
+  const int64_t red = kJoints * kWarps * kTile * (8 * tiles + 1) * 4, pair_stage = int64_t(kTile) * (per_block * stage_blocks + 1) * (type == HYACIN_F32 ? 8 : 4);
+  const int64_t fixed = x_bytes + sums + red + int64_t(sizeof(StreamBars)), stage_codes = kTile * stage_blocks * 64, stage = stage_codes + pair_stage;
   const int64_t ring = std::min<int64_t>(kMaxRing, (kSmemLimit - fixed) / stage);
   if (fixed > kSmemLimit || ring < 4) return 0;
-  p.ring = int(ring); p.pitch = int(pitch); p.sums_at = int(x_bytes); p.ring_at = int(x_bytes + sums); p.pairs_at = int(p.ring_at + ring * kTile * kColumnPitch);
+  p.ring = int(ring); p.pitch = int(pitch); p.sums_at = int(x_bytes); p.ring_at = int(x_bytes + sums); p.pairs_at = int(p.ring_at + ring * stage_codes);
   p.red_at = int(p.pairs_at + ring * pair_stage); p.bars_at = int(p.red_at + red);
   return int(fixed + ring * stage);
 }
@@ -470,16 +484,6 @@ int32_t launch_product_stream(const hyacinHandle_t* handle, const char* fn, hyac
   float* mid = nullptr;
   int32_t rc = 0;
   const int per = product_stream_vectors(type, a);
-  // the codes as eight-byte elements: a box row of 1 KiB
-  EncodeTiledFn encode = encode_tiled();
-  CUtensorMap map{};
-  const cuuint64_t dims[2] = {cuuint64_t((int64_t(a.m) + 127) / 128 * 8), cuuint64_t(a.n)}, strides[1] = {cuuint64_t(a.ldq)};
-  const cuuint32_t box[2] = {kColumnPitch / 8, kTile}, elem[2] = {1, 1};
-  if (!encode || encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT64, 2, const_cast<uint8_t*>(a.codes), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
-                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS) {
-    std::fprintf(stderr, "hyacin-b200: %s: cuTensorMapEncodeTiled failed\n", fn);
-    return -3;
-  }
   with_w4_type(type, [&](auto tag) {
     using X = decltype(tag);
     if (a.rank) {
@@ -489,6 +493,16 @@ int32_t launch_product_stream(const hyacinHandle_t* handle, const char* fn, hyac
     for (int64_t t0 = 0; t0 < a.t && rc == 0; t0 += per) {
       StreamParams p{};
       const int smem = place(p, type, a, int(std::min<int64_t>(per, a.t - t0)));
+      // the codes as eight-byte elements: a box row is a column's share of a stage
+      EncodeTiledFn encode = encode_tiled();
+      CUtensorMap map{};
+      const cuuint64_t dims[2] = {cuuint64_t(p.blocks) * 8, cuuint64_t(a.n)}, strides[1] = {cuuint64_t(a.ldq)};
+      const cuuint32_t box[2] = {cuuint32_t(kWarps * blocks_per_warp(p.cols > 8 ? 2 : 1) * 8), kTile}, elem[2] = {1, 1};
+      if (!encode || encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT64, 2, const_cast<uint8_t*>(a.codes), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS) {
+        std::fprintf(stderr, "hyacin-b200: %s: cuTensorMapEncodeTiled failed\n", fn);
+        rc = -3; return;
+      }
       p.codes = a.codes; p.ldq = a.ldq; p.scales = a.scales; p.zeros = a.zeros; p.lds = a.lds;
       p.x = static_cast<const X*>(a.x) + t0 * a.ldx; p.ldx = a.ldx; p.y = static_cast<X*>(a.y) + t0 * a.ldy; p.ldy = a.ldy;
       p.second = a.second; p.ld2 = a.ld2; p.mid = mid ? mid + t0 * a.rank : nullptr;
@@ -500,7 +514,7 @@ int32_t launch_product_stream(const hyacinHandle_t* handle, const char* fn, hyac
         mid_kernel<X><<<dim3(a.rank, (p.t + 7) / 8), 256, 0, stream>>>(static_cast<const X*>(a.first), a.ld1, a.m, a.rank, static_cast<const X*>(p.x), a.ldx, p.t, mid + t0 * a.rank,
                                                                       wide && reinterpret_cast<uintptr_t>(a.first) % 16 == 0 && a.ld1 * sizeof(X) % 16 == 0);
       }
-      const cudaError_t e = p.seg_sub % 4 ? dispatch<X, true>(handle, map, p, smem) : dispatch<X, false>(handle, map, p, smem);
+      const cudaError_t e = p.seg_sub % 4 == 0 ? dispatch<X, 4>(handle, map, p, smem) : p.seg_sub % 2 == 0 ? dispatch<X, 2>(handle, map, p, smem) : dispatch<X, 1>(handle, map, p, smem);
       if (e != cudaSuccess) { report_cuda_error(e, fn, __FILE__, __LINE__); rc = -3; }
       else rc = w4_launched(fn);
     }
