@@ -9,15 +9,24 @@
 // The sum over the classes outside is accumulated without the listed ones, so p_r / q_r never comes from a difference, and
 // what concerns the list (K terms) is done in 64 bits: where student and teacher agree, q - p is the difference of two numbers
 // close to one.
+//
+// Two kernels.  distill_cluster_kernel keeps a token's logits in the shared memory of a cluster of one to eight CTAs: they are read
+// from DRAM once, with bulk copies, and the gradient is written from there; one exchange of (maximum, sum) per CTA is all the
+// communication.  Slices of at most 72 KiB leave three CTAs per SM, whose loads, arithmetic and stores overlap.
+// distill_plain_kernel (one block per token, passes over global memory) takes rows that do not fit a cluster.
+// exp is taken as 2^(z scale - c), scale = log2(e) / tau and c = float(top scale), one fused multiply-add and one ex2 per entry;
+// what rounding c loses, kappa = top scale - c, is known in 64 bits and put back into the sum, so the loss does not see it.
 #include "w4.cuh"
+#include "ptx_sm100.cuh"
+#include <atomic>
 #include <algorithm>
+#include <type_traits>
 
 namespace hyb {
 namespace {
 
 constexpr int kMaxList = 1024;
 constexpr int kMaxClasses = 1 << 20;
-constexpr float kLog2e = 1.4426950408889634f;
 
 struct DistillArgs {
   const void* z; int64_t ldz; int n, t, k;
@@ -25,6 +34,19 @@ struct DistillArgs {
   const float* teacher_lse; const float* weight;
   float* loss; float* stats_out; const float* stats_in;
   void* dz; int64_t lddz;
+  int splits, list_at;      // cluster kernel: CTAs per token, start of the list in shared memory
+};
+
+__device__ __forceinline__ float ex2(float x) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
+// 2^(z scale - c) relative to top: c and the factor that puts kappa back.  top = 0 stands for "nothing there".
+struct Exponent {
+  float scale, c; double fix;
+  __device__ Exponent(double tau, float top) {
+    scale = float(1.4426950408889634 / tau); c = top * scale;
+    fix = exp2(double(c) - double(top) * double(scale));
+    if (!(fabsf(c) <= 3.402823466e38f)) fix = 1.;
+  }
+  __device__ __forceinline__ float operator()(float z) const { return ex2(fmaf(z, scale, -c)); }
 };
 
 // Sum / maximum over the block, the same in every thread.  buf: 32 entries.
@@ -40,20 +62,25 @@ template <class V, class F> __device__ V block_reduce(V v, F f, V* buf) {
 struct Add { template <class V> __device__ V operator()(V a, V b) const { return a + b; } };
 struct Max { template <class V> __device__ V operator()(V a, V b) const { return a > b ? a : b; } };
 
-// The list of one token in shared memory.
+// The list of one token in shared memory, `k` entries each.
 struct List {
-  double p[kMaxList];        // teacher probability
-  double logp[kMaxList];
-  double psum[kMaxList];     // sum over the entries of the same class, at the first of them
-  float z[kMaxList];         // student logit
-  int id[kMaxList];          // class, -1 when skipped
-  int first[kMaxList];       // 1: first entry of its class
-  double buf[32]; float fbuf[32];
+  double *p, *logp, *psum;   // teacher probability, its logarithm, sum over the entries of the same class
+  float* z;                  // student logit
+  int *id, *first;           // class, -1 when skipped; 1 for the first entry of its class
+  double* buf; float* fbuf;  // 32 entries each, for reductions
+  __device__ List(uint8_t* at, int k) {
+    buf = reinterpret_cast<double*>(at); p = buf + 32; logp = p + k; psum = logp + k;
+    fbuf = reinterpret_cast<float*>(psum + k); z = fbuf + 32; id = reinterpret_cast<int*>(z + k); first = id + k;
+  }
 };
+__host__ __device__ constexpr size_t list_bytes(int k) { return 32 * 12 + size_t(k) * 36; }
 
-// Reads the list; returns p_r and the mass.  Ends with a barrier.
-template <class T> __device__ void load_list(const DistillArgs& a, int64_t token, const T* z, List& s, double& rest, double& mass) {
-  double top = -INFINITY;
+// What is known of the teacher, and of the student's listed classes, before the rest of the row has been seen.
+struct Listed { double rest, mass, top, sum; };      // p_r, sum p + p_r; log-sum-exp of the student's listed classes as top + log(sum), top = -inf without any
+
+// Reads the list.  Ends with a barrier.
+template <class T> __device__ Listed load_list(const DistillArgs& a, int64_t token, const T* z, List& s) {
+  double top = -INFINITY, student = -INFINITY;
   for (int i = threadIdx.x; i < a.k; i += blockDim.x) {
     const int id = a.ids[token * a.ldk + i];
     const bool ok = id >= 0 && id < a.n;
@@ -61,6 +88,7 @@ template <class T> __device__ void load_list(const DistillArgs& a, int64_t token
     const double t = ok ? double(a.teacher[token * a.ldk + i]) / a.tau : -INFINITY;
     s.logp[i] = t; s.z[i] = ok ? to_f32(z[id]) : 0.f;
     top = fmax(top, t);
+    if (ok) student = fmax(student, double(s.z[i]) / a.tau);
   }
   double norm;
   if (a.teacher_lse) norm = double(a.teacher_lse[token]);
@@ -77,21 +105,57 @@ template <class T> __device__ void load_list(const DistillArgs& a, int64_t token
     sum += s.p[i];
   }
   sum = block_reduce(sum, Add{}, s.buf);
+  Listed r;
+  r.rest = a.teacher_lse ? fmax(0., 1. - sum) : 0.;
+  r.mass = sum + r.rest;
+  r.top = block_reduce(student, Max{}, s.buf);
+  double e = 0.;
   for (int i = threadIdx.x; i < a.k; i += blockDim.x) {
     int first = s.id[i] >= 0; double ps = 0.;
     for (int j = 0; j < a.k; ++j) if (s.id[j] == s.id[i]) { ps += s.p[j]; if (j < i) first = 0; }
     s.first[i] = first; s.psum[i] = ps;
+    if (first && r.top > -INFINITY) e += exp(double(s.z[i]) / a.tau - r.top);
   }
-  rest = a.teacher_lse ? fmax(0., 1. - sum) : 0.;
-  mass = sum + rest;
+  r.sum = block_reduce(e, Add{}, s.buf);
   __syncthreads();
+  return r;
+}
+
+// The student's normalisers from the listed classes and the sum over the others, outside 2^(top scale).
+struct Student {
+  double lse, lse_out; bool empty, no_outside;
+  __device__ Student(const DistillArgs& a, const Listed& l, float top, float outside) {
+    no_outside = outside == 0.f;
+    lse_out = no_outside ? -INFINITY : log(double(outside)) + double(top) / a.tau;
+    double ref = fmax(l.top, lse_out);
+    if (ref == -INFINITY) ref = 0.;
+    const double total = (l.top > -INFINITY || l.top != l.top ? l.sum * exp(l.top - ref) : 0.) + (no_outside ? 0. : exp(lse_out - ref));
+    empty = total == 0.;
+    lse = ref + log(total);
+  }
+};
+// Weighted loss (same in every thread; all threads of the block take part).
+__device__ double distill_loss(const DistillArgs& a, const List& s, const Listed& l, const Student& st, float weight) {
+  double kl = 0.;
+  for (int i = threadIdx.x; i < a.k; i += blockDim.x) if (s.p[i] != 0.) kl += s.p[i] * (s.logp[i] - (st.empty ? -INFINITY : double(s.z[i]) / a.tau - st.lse));
+  kl = block_reduce(kl, Add{}, s.buf);
+  if (l.rest > 0.) kl += l.rest * (log(l.rest) - (st.no_outside ? -INFINITY : st.lse_out - st.lse));
+  return kl * weight;
+}
+// dKL/dz = factor * 2^(z scale - top scale) outside the list
+__device__ __forceinline__ double outside_factor(const DistillArgs& a, const Listed& l, const Student& st, float outside, float weight) {
+  return st.no_outside ? 0. : double(weight) / a.tau * (l.mass * exp(st.lse_out - st.lse) - l.rest) / double(outside);
+}
+__device__ __forceinline__ float listed_gradient(const DistillArgs& a, const List& s, const Listed& l, const Student& st, float weight, int i) {
+  return float(double(weight) / a.tau * (l.mass * (st.empty ? 0. : exp(double(s.z[i]) / a.tau - st.lse)) - s.psum[i]));
 }
 
 // Plain form: one block per token, two passes over the logits, a bit per class for the list.
 // Mode: loss from this pass's sums, or gradient from saved ones.
 template <class T> __global__ void __launch_bounds__(512) distill_plain_kernel(DistillArgs a) {
-  extern __shared__ uint32_t listed[];
-  __shared__ List s;
+  extern __shared__ __align__(16) uint8_t smem[];
+  uint32_t* listed = reinterpret_cast<uint32_t*>(smem + (list_bytes(a.k) + 15) / 16 * 16);
+  List s(smem, a.k);
   const T* z_all = static_cast<const T*>(a.z);
   for (int64_t token = blockIdx.x; token < a.t; token += gridDim.x) {
     const T* z = z_all + token * a.ldz;
@@ -107,11 +171,9 @@ template <class T> __global__ void __launch_bounds__(512) distill_plain_kernel(D
       continue;
     }
     for (int j = threadIdx.x; j < (a.n + 31) / 32; j += blockDim.x) listed[j] = 0;
-    double rest, mass;
-    load_list<T>(a, token, z, s, rest, mass);
+    const Listed l = load_list<T>(a, token, z, s);
     for (int i = threadIdx.x; i < a.k; i += blockDim.x) if (s.id[i] >= 0) atomicOr(&listed[s.id[i] >> 5], 1u << (s.id[i] & 31));
     __syncthreads();
-    const float scale = kLog2e / float(a.tau);
     float top, outside;
     if (a.stats_in) { top = a.stats_in[2 * token]; outside = a.stats_in[2 * token + 1]; }
     else {
@@ -119,56 +181,235 @@ template <class T> __global__ void __launch_bounds__(512) distill_plain_kernel(D
       for (int j = threadIdx.x; j < a.n; j += blockDim.x) if (!(listed[j >> 5] >> (j & 31) & 1)) top = fmaxf(top, to_f32(z[j]));
       top = block_reduce(top, Max{}, s.fbuf);
       if (top == -INFINITY) top = 0.f;
+      const Exponent e(a.tau, top);
       double sum = 0.;
-      for (int j = threadIdx.x; j < a.n; j += blockDim.x) if (!(listed[j >> 5] >> (j & 31) & 1)) sum += exp2f((to_f32(z[j]) - top) * scale);
-      outside = float(block_reduce(sum, Add{}, s.buf));
+      for (int j = threadIdx.x; j < a.n; j += blockDim.x) if (!(listed[j >> 5] >> (j & 31) & 1)) sum += e(to_f32(z[j]));
+      outside = float(block_reduce(sum, Add{}, s.buf) * e.fix);
     }
-    // log-sum-exps in 64 bits, relative to the larger of the two maxima
-    double ltop = -INFINITY;
-    for (int i = threadIdx.x; i < a.k; i += blockDim.x) if (s.id[i] >= 0) ltop = fmax(ltop, double(s.z[i]) / a.tau);
-    ltop = block_reduce(ltop, Max{}, s.buf);
-    const double lse_out = log(double(outside)) + double(top) / a.tau;
-    double ref = fmax(ltop, lse_out);
-    if (ref == -INFINITY) ref = 0.;
-    double e = 0.;
-    for (int i = threadIdx.x; i < a.k; i += blockDim.x) if (s.first[i]) e += exp(double(s.z[i]) / a.tau - ref);
-    const double total = block_reduce(e, Add{}, s.buf) + (outside == 0.f ? 0. : exp(lse_out - ref));
-    const double lse = ref + log(total);
+    const Student st(a, l, top, outside);
     if (a.loss || a.stats_out) {
-      double kl = 0.;
-      for (int i = threadIdx.x; i < a.k; i += blockDim.x) if (s.p[i] != 0.) kl += s.p[i] * (s.logp[i] - (total == 0. ? -INFINITY : double(s.z[i]) / a.tau - lse));
-      kl = block_reduce(kl, Add{}, s.buf);
-      if (rest > 0.) kl += rest * (log(rest) - (outside == 0.f ? -INFINITY : lse_out - lse));
+      const double loss = distill_loss(a, s, l, st, weight);
       if (threadIdx.x == 0) {
-        if (a.loss) a.loss[token] = float(kl * weight);
+        if (a.loss) a.loss[token] = float(loss);
         if (a.stats_out) { a.stats_out[2 * token] = top; a.stats_out[2 * token + 1] = outside; }
       }
     }
     if (dz) {
-      const double w = double(weight) / a.tau;
-      const float factor = outside == 0.f ? 0.f : float(w * (mass * exp(double(top) / a.tau - lse) - rest / double(outside)));
+      const Exponent e(a.tau, top);
+      const float factor = float(outside_factor(a, l, st, outside, weight) * e.fix);
       for (int j = threadIdx.x; j < a.n; j += blockDim.x)
-        if (!(listed[j >> 5] >> (j & 31) & 1)) dz[j] = from_f32<T>(factor * exp2f((to_f32(z[j]) - top) * scale));
-      for (int i = threadIdx.x; i < a.k; i += blockDim.x)
-        if (s.first[i]) dz[s.id[i]] = from_f32<T>(float(w * (mass * (total == 0. ? 0. : exp(double(s.z[i]) / a.tau - lse)) - s.psum[i])));
+        if (!(listed[j >> 5] >> (j & 31) & 1)) dz[j] = from_f32<T>(factor * e(to_f32(z[j])));
+      for (int i = threadIdx.x; i < a.k; i += blockDim.x) if (s.first[i]) dz[s.id[i]] = from_f32<T>(listed_gradient(a, s, l, st, weight, i));
     }
   }
 }
 
-int32_t launch_distill(const char* fn, const hyacinHandle_t* handle, hyacinPrecision_t type, const DistillArgs& a) {
-  const size_t bits = size_t((a.n + 31) / 32) * 4;
-  int32_t rc = 0;
-  with_w4_type(type, [&](auto tag) {
-    auto* kernel = distill_plain_kernel<decltype(tag)>;
-    if (bits > 8192) {
-      const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxClasses / 8);
-      if (e != cudaSuccess) { report_cuda_error(e, "cudaFuncSetAttribute", __FILE__, __LINE__); rc = -3; return; }
+// ---- cluster kernel ------------------------------------------------------------------------------------------------
+constexpr int kClusterThreads = 256;
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ float ld_cluster(const void* at, uint32_t rank) {
+  uint32_t remote; float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(ptx::smem_u32(at)), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote) : "memory");
+  return v;
+}
+// The entries of a 16-byte vector as floats, and back.
+template <class T> __device__ __forceinline__ void unpack(const uint4& v, float (&f)[16 / sizeof(T)]) {
+  const T* p = reinterpret_cast<const T*>(&v);
+#pragma unroll
+  for (int i = 0; i < int(16 / sizeof(T)); ++i) f[i] = to_f32(p[i]);
+}
+template <class T> __device__ __forceinline__ uint4 pack(const float (&f)[16 / sizeof(T)]) {
+  uint4 v;
+  if constexpr (sizeof(T) == 4) v = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+  else {
+    uint32_t* o = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (std::is_same<T, __half>::value) { const __half2 h = __floats2half2_rn(f[2 * i], f[2 * i + 1]); o[i] = *reinterpret_cast<const uint32_t*>(&h); }
+      else { const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]); o[i] = *reinterpret_cast<const uint32_t*>(&h); }
     }
-    count_launch();
-    kernel<<<unsigned(std::min(a.t, 1 << 20)), 512, bits, handle->cudaStream>>>(a);
-    rc = w4_launched(fn);
-  });
-  return rc;
+  }
+  return v;
+}
+
+// A token's row is cut at the 16-byte boundaries of its address: up to V - 1 entries before the first one belong to CTA 0, those behind
+// the last one to the last CTA (both kept as floats in `edge`), the vectors between are shared out evenly.
+template <class T> __global__ void __launch_bounds__(kClusterThreads, 3) distill_cluster_kernel(const __grid_constant__ DistillArgs a, uint32_t* status) {
+  constexpr int V = 16 / sizeof(T);
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ float edge[2 * V], part[2];
+  __shared__ uint64_t bar; __shared__ uint32_t abort_flag;
+  uint4* slice = reinterpret_cast<uint4*>(smem);
+  List s(smem + a.list_at, a.k);
+  const int rank = int(blockIdx.x % unsigned(a.splits)); const int64_t token = blockIdx.x / unsigned(a.splits);
+  const T* z = static_cast<const T*>(a.z) + token * a.ldz;
+  T* dz = a.dz ? static_cast<T*>(a.dz) + token * a.lddz : nullptr;
+  const int mis = int(reinterpret_cast<uintptr_t>(z) / sizeof(T) % V), head = min((V - mis) % V, a.n), vectors = (a.n - head) / V, tail0 = head + vectors * V;
+  const int v0 = int(int64_t(vectors) * rank / a.splits), v1 = int(int64_t(vectors) * (rank + 1) / a.splits);
+  const bool first = rank == 0, last = rank == a.splits - 1;
+  const bool same = dz && int(reinterpret_cast<uintptr_t>(dz) / sizeof(T) % V) == mis;      // gradient and logits share their alignment
+  const float weight = a.weight ? a.weight[token] : 1.f;
+  if (weight == 0.f) {                               // the same for the whole cluster: nobody waits
+    if (first && threadIdx.x == 0) {
+      if (a.loss) a.loss[token] = 0.f;
+      if (a.stats_out) a.stats_out[2 * token] = a.stats_out[2 * token + 1] = __int_as_float(0x7fc00000);
+    }
+    if (dz) {
+      if (same) for (int v = v0 + threadIdx.x; v < v1; v += kClusterThreads) *reinterpret_cast<uint4*>(dz + head + v * V) = make_uint4(0, 0, 0, 0);
+      else for (int j = head + v0 * V + threadIdx.x; j < head + v1 * V; j += kClusterThreads) dz[j] = from_f32<T>(0.f);
+      if (first && int(threadIdx.x) < head) dz[threadIdx.x] = from_f32<T>(0.f);
+      if (last && tail0 + int(threadIdx.x) < a.n) dz[tail0 + threadIdx.x] = from_f32<T>(0.f);
+    }
+    return;
+  }
+  if (threadIdx.x == 0) {
+    ptx::mbar_init(&bar, 1); abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    const uint32_t bytes = uint32_t(v1 - v0) * 16;
+    ptx::mbar_expect_tx(&bar, bytes);
+    for (uint32_t at = 0; at < bytes; at += 32768) ptx::bulk_load(ptx::smem_u32(smem) + at, reinterpret_cast<const uint8_t*>(z + head + v0 * V) + at, min(32768u, bytes - at), &bar);
+  }
+  if (threadIdx.x < 2 * V) {
+    const int j = int(threadIdx.x) < V ? int(threadIdx.x) : tail0 + int(threadIdx.x) - V;
+    const bool mine = int(threadIdx.x) < V ? first && j < head : last && j < a.n;
+    edge[threadIdx.x] = mine ? to_f32(z[j]) : -INFINITY;
+  }
+  const Listed l = load_list<T>(a, token, z, s);
+  bool ok = ptx::mbar_wait(&bar, 0u, &abort_flag, status, 41u);
+  __syncthreads();                                   // every thread has seen the copy land before an entry is overwritten
+  for (int i = threadIdx.x; i < a.k; i += kClusterThreads) {      // listed classes leave the row (equal values for a class listed twice)
+    const int id = s.id[i], v = id < head ? -1 : (id - head) / V;
+    if (id < 0) continue;
+    if (id < head) { if (first) edge[id] = -INFINITY; }
+    else if (id >= tail0) { if (last) edge[V + id - tail0] = -INFINITY; }
+    else if (v >= v0 && v < v1) reinterpret_cast<T*>(slice)[id - head - v0 * V] = from_f32<T>(-INFINITY);
+  }
+  __syncthreads();
+  float top, outside;
+  if (!a.stats_in) {
+    // maximum and sum of this slice, then one exchange
+    float m = threadIdx.x < 2 * V ? edge[threadIdx.x] : -INFINITY;
+    for (int v = threadIdx.x; v < v1 - v0; v += kClusterThreads) {
+      float f[V]; unpack<T>(slice[v], f);
+#pragma unroll
+      for (int i = 0; i < V; ++i) m = fmaxf(m, f[i]);
+    }
+    m = block_reduce(m, Max{}, s.fbuf);
+    const Exponent e(a.tau, m == -INFINITY ? 0.f : m);
+    float sum = threadIdx.x < 2 * V ? e(edge[threadIdx.x]) : 0.f;
+    for (int v = threadIdx.x; v < v1 - v0; v += kClusterThreads) {
+      float f[V]; unpack<T>(slice[v], f);
+      float q[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) q[i] = e(f[i]);
+#pragma unroll
+      for (int d = V / 2; d; d /= 2)
+#pragma unroll
+        for (int i = 0; i < d; ++i) q[i] += q[i + d];
+      sum += q[0];
+    }
+    const double mine = block_reduce(double(sum), Add{}, s.buf) * e.fix;
+    if (a.splits > 1) {
+      if (threadIdx.x == 0) { part[0] = m; part[1] = float(mine); }
+      cluster_arrive(); cluster_wait();
+      top = -INFINITY;
+      for (int r = 0; r < a.splits; ++r) top = fmaxf(top, ld_cluster(&part[0], r));
+      if (top == -INFINITY) top = 0.f;
+      double total = 0.;
+      for (int r = 0; r < a.splits; ++r) {
+        const float pm = ld_cluster(&part[0], r), ps = ld_cluster(&part[1], r);
+        total += pm == -INFINITY ? 0. : pm == top ? double(ps) : double(ps) * exp2((double(pm) - double(top)) * double(e.scale));
+      }
+      outside = float(total);
+      cluster_arrive();                              // peers may leave once everybody has read
+    } else { top = m == -INFINITY ? 0.f : m; outside = float(mine); }
+  } else {
+    top = a.stats_in[2 * token]; outside = a.stats_in[2 * token + 1];
+    if (a.splits > 1) { cluster_arrive(); cluster_wait(); cluster_arrive(); }      // in place: every CTA has read the listed logits
+  }
+  const Student st(a, l, top, outside);
+  if (first && (a.loss || a.stats_out)) {
+    const double loss = distill_loss(a, s, l, st, weight);
+    if (threadIdx.x == 0) {
+      if (a.loss) a.loss[token] = float(loss);
+      if (a.stats_out) { a.stats_out[2 * token] = top; a.stats_out[2 * token + 1] = outside; }
+    }
+  }
+  if (dz) {
+    const Exponent e(a.tau, top);
+    const float factor = float(outside_factor(a, l, st, outside, weight) * e.fix);
+    for (int v = threadIdx.x; v < v1 - v0; v += kClusterThreads) {
+      float f[V]; unpack<T>(slice[v], f);
+#pragma unroll
+      for (int i = 0; i < V; ++i) f[i] = factor * e(f[i]);
+      T* to = dz + head + (v0 + v) * V;
+      if (same) *reinterpret_cast<uint4*>(to) = pack<T>(f);
+      else
+#pragma unroll
+        for (int i = 0; i < V; ++i) to[i] = from_f32<T>(f[i]);
+    }
+    if (threadIdx.x < 2 * V) {
+      const int j = int(threadIdx.x) < V ? int(threadIdx.x) : tail0 + int(threadIdx.x) - V;
+      if (int(threadIdx.x) < V ? first && j < head : last && j < a.n) dz[j] = from_f32<T>(factor * e(edge[threadIdx.x]));
+    }
+    __syncthreads();                                 // the listed classes are written last
+    for (int i = threadIdx.x; i < a.k; i += kClusterThreads) {
+      const int id = s.id[i];
+      if (!s.first[i]) continue;
+      const bool mine = id < head ? first : id >= tail0 ? last : (id - head) / V >= v0 && (id - head) / V < v1;
+      if (mine) dz[id] = from_f32<T>(listed_gradient(a, s, l, st, weight, i));
+    }
+  }
+  if (a.splits > 1) cluster_wait();
+  (void)ok;                                          // an expired wait is in the status word; the values are then undefined
+}
+
+// Slices of at most 72 KiB where eight CTAs allow it (three CTAs per SM), otherwise what one CTA per SM takes.
+constexpr int kSliceBytes = 72 * 1024, kSmemMost = 225 * 1024;
+
+template <class T> cudaError_t raise_limit(const hyacinHandle_t* handle, T* kernel, std::atomic<uint64_t>& ready) {
+  const uint64_t bit = uint64_t(1) << (handle->DeviceID & 63);      // per device
+  if (ready.load() & bit) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost);
+  if (e == cudaSuccess) ready.fetch_or(bit);
+  return e;
+}
+
+int32_t launch_distill(const char* fn, const hyacinHandle_t* handle, hyacinPrecision_t type, DistillArgs a) {
+  const int64_t row = int64_t(a.n) * int64_t(w4_type_bytes(type)) + 16;
+  int splits = 1;
+  while (splits < 8 && (row + splits - 1) / splits > kSliceBytes) splits *= 2;
+  cudaError_t e = cudaSuccess;
+  count_launch();
+  const int64_t slice = ((row / 16 + splits - 1) / splits + 1) * 16;
+  if (slice + int64_t(list_bytes(a.k)) <= kSmemMost && int64_t(a.t) * splits <= 0x7fffffff) {
+    a.splits = splits; a.list_at = int(slice);
+    const size_t smem = size_t(slice) + list_bytes(a.k);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(unsigned(a.t) * splits); cfg.blockDim = dim3(kClusterThreads); cfg.dynamicSmemBytes = smem; cfg.stream = handle->cudaStream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension; attr[0].val.clusterDim.x = splits; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr; cfg.numAttrs = splits > 1 ? 1 : 0;
+    uint32_t* status = status_word_device(handle->DeviceID);
+    with_w4_type(type, [&](auto tag) {
+      auto* kernel = distill_cluster_kernel<decltype(tag)>;
+      static std::atomic<uint64_t> ready{0};
+      e = raise_limit(handle, kernel, ready);
+      if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, kernel, a, status);
+    });
+  } else {
+    const size_t smem = (list_bytes(a.k) + 15) / 16 * 16 + size_t((a.n + 31) / 32) * 4;
+    with_w4_type(type, [&](auto tag) {
+      auto* kernel = distill_plain_kernel<decltype(tag)>;
+      static std::atomic<uint64_t> ready{0};
+      e = raise_limit(handle, kernel, ready);
+      if (e == cudaSuccess) kernel<<<unsigned(std::min(a.t, 1 << 20)), 512, smem, handle->cudaStream>>>(a);
+    });
+  }
+  if (e != cudaSuccess) { report_cuda_error(e, fn, __FILE__, __LINE__); return -3; }
+  return w4_launched(fn);
 }
 
 int32_t check_distill(const char* fn, const hyacinHandle_t* handle, hyacinPrecision_t type, const DistillArgs& a) {
@@ -193,7 +434,7 @@ extern "C" int32_t hyacinB200DistillLoss(const hyacinHandle_t* handle, hyacinPre
                                          const float* teacherLse, const float* weight, float* loss, float* stats, void* dZ, int32_t lddz) {
   using namespace hyb;
   const char* fn = "hyacinB200DistillLoss";
-  DistillArgs a{Z, ldz, N, T, K, ids, teacher, ldk, tau, teacherLse, weight, loss, stats, nullptr, dZ, lddz};
+  DistillArgs a{Z, ldz, N, T, K, ids, teacher, ldk, tau, teacherLse, weight, loss, stats, nullptr, dZ, lddz, 1, 0};
   const int32_t rc = check_distill(fn, handle, Ztype, a);
   if (rc) return rc < 0 ? rc : 0;
   if (!loss && !stats && !dZ) return 0;
@@ -206,7 +447,7 @@ extern "C" int32_t hyacinB200DistillGrad(const hyacinHandle_t* handle, hyacinPre
                                          const float* teacherLse, const float* weight, const float* stats, void* dZ, int32_t lddz) {
   using namespace hyb;
   const char* fn = "hyacinB200DistillGrad";
-  DistillArgs a{Z, ldz, N, T, K, ids, teacher, ldk, tau, teacherLse, weight, nullptr, nullptr, stats, dZ, lddz};
+  DistillArgs a{Z, ldz, N, T, K, ids, teacher, ldk, tau, teacherLse, weight, nullptr, nullptr, stats, dZ, lddz, 1, 0};
   const int32_t rc = check_distill(fn, handle, Ztype, a);
   if (rc) return rc < 0 ? rc : 0;
   if (!stats || !dZ) return w4_refuse(fn, "null pointer");
