@@ -40,12 +40,9 @@ struct DistillArgs {
 __device__ __forceinline__ float ex2(float x) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
 // 2^(z scale - c) relative to top: c and the factor that puts kappa back.  top = 0 stands for "nothing there".
 struct Exponent {
-  float scale, c; double fix;
-  __device__ Exponent(double tau, float top) {
-    scale = float(1.4426950408889634 / tau); c = top * scale;
-    fix = exp2(double(c) - double(top) * double(scale));
-    if (!(fabsf(c) <= 3.402823466e38f)) fix = 1.;
-  }
+  float scale, c, top;
+  __device__ __forceinline__ Exponent(double tau, float t) : scale(float(1.4426950408889634 / tau)), c(t * scale), top(t) {}
+  __device__ double fix() const { return fabsf(c) <= 3.402823466e38f ? exp2(double(c) - double(top) * double(scale)) : 1.; }
   __device__ __forceinline__ float operator()(float z) const { return ex2(fmaf(z, scale, -c)); }
 };
 
@@ -184,7 +181,7 @@ template <class T> __global__ void __launch_bounds__(512) distill_plain_kernel(D
       const Exponent e(a.tau, top);
       double sum = 0.;
       for (int j = threadIdx.x; j < a.n; j += blockDim.x) if (!(listed[j >> 5] >> (j & 31) & 1)) sum += e(to_f32(z[j]));
-      outside = float(block_reduce(sum, Add{}, s.buf) * e.fix);
+      outside = float(block_reduce(sum, Add{}, s.buf) * e.fix());
     }
     const Student st(a, l, top, outside);
     if (a.loss || a.stats_out) {
@@ -196,7 +193,7 @@ template <class T> __global__ void __launch_bounds__(512) distill_plain_kernel(D
     }
     if (dz) {
       const Exponent e(a.tau, top);
-      const float factor = float(outside_factor(a, l, st, outside, weight) * e.fix);
+      const float factor = float(outside_factor(a, l, st, outside, weight) * e.fix());
       for (int j = threadIdx.x; j < a.n; j += blockDim.x)
         if (!(listed[j >> 5] >> (j & 31) & 1)) dz[j] = from_f32<T>(factor * e(to_f32(z[j])));
       for (int i = threadIdx.x; i < a.k; i += blockDim.x) if (s.first[i]) dz[s.id[i]] = from_f32<T>(listed_gradient(a, s, l, st, weight, i));
@@ -205,16 +202,23 @@ template <class T> __global__ void __launch_bounds__(512) distill_plain_kernel(D
 }
 
 // ---- cluster kernel ------------------------------------------------------------------------------------------------
-constexpr int kClusterThreads = 256;
+constexpr int kMainThreads = 256, kClusterThreads = kMainThreads + 32;      // the last warp works on the list
+constexpr int kHashWords = 2048;                  // 65536 bits: finds out cheaply that no class is listed twice
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ void main_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kMainThreads) : "memory"); }
 __device__ __forceinline__ float ld_cluster(const void* at, uint32_t rank) {
   uint32_t remote; float v;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(ptx::smem_u32(at)), "r"(rank));
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote) : "memory");
   return v;
 }
-// The entries of a 16-byte vector as floats, and back.
+template <class V, class F> __device__ __forceinline__ V warp_reduce(V v, F f) {
+#pragma unroll
+  for (int d = 16; d; d >>= 1) v = f(v, __shfl_xor_sync(~0u, v, d));
+  return v;
+}
+// The entries of a 16-byte vector as floats, and back; their maximum together with m, two at a time for the 16-bit types.
 template <class T> __device__ __forceinline__ void unpack(const uint4& v, float (&f)[16 / sizeof(T)]) {
   const T* p = reinterpret_cast<const T*>(&v);
 #pragma unroll
@@ -233,17 +237,80 @@ template <class T> __device__ __forceinline__ uint4 pack(const float (&f)[16 / s
   }
   return v;
 }
+template <class T> struct RowMax;
+template <> struct RowMax<float> {
+  float m = -INFINITY;
+  __device__ __forceinline__ void add(const uint4& v) { m = fmaxf(fmaxf(m, fmaxf(__uint_as_float(v.x), __uint_as_float(v.y))), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w))); }
+  __device__ __forceinline__ float value() const { return m; }
+};
+template <> struct RowMax<__half> {
+  __half2 m = __float2half2_rn(-INFINITY);
+  __device__ __forceinline__ void add(const uint4& v) {
+    const __half2* h = reinterpret_cast<const __half2*>(&v);
+    m = __hmax2(__hmax2(m, __hmax2(h[0], h[1])), __hmax2(h[2], h[3]));
+  }
+  __device__ __forceinline__ float value() const { return fmaxf(__low2float(m), __high2float(m)); }
+};
+template <> struct RowMax<__nv_bfloat16> {
+  __nv_bfloat162 m = __float2bfloat162_rn(-INFINITY);
+  __device__ __forceinline__ void add(const uint4& v) {
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
+    m = __hmax2(__hmax2(m, __hmax2(h[0], h[1])), __hmax2(h[2], h[3]));
+  }
+  __device__ __forceinline__ float value() const { return fmaxf(__low2float(m), __high2float(m)); }
+};
+
+// The teacher's probabilities and the student's listed classes, by one warp; id and z (and the teacher's logits in logp) are there.
+__device__ Listed list_by_warp(const DistillArgs& a, int64_t token, List& s, bool twice) {
+  const int lane = threadIdx.x & 31;
+  double top = -INFINITY, student = -INFINITY;
+  for (int i = lane; i < a.k; i += 32) if (s.id[i] >= 0) { top = fmax(top, s.logp[i]); student = fmax(student, double(s.z[i]) / a.tau); }
+  double norm;
+  if (a.teacher_lse) norm = double(a.teacher_lse[token]);
+  else {
+    top = warp_reduce(top, Max{});
+    double e = 0.;
+    for (int i = lane; i < a.k; i += 32) if (s.id[i] >= 0) e += exp(s.logp[i] - top);
+    norm = top + log(warp_reduce(e, Add{}));
+  }
+  Listed r;
+  r.top = warp_reduce(student, Max{});
+  double sum = 0., e = 0.;
+  for (int i = lane; i < a.k; i += 32) {
+    const bool ok = s.id[i] >= 0;
+    const double l = s.logp[i] - norm, p = ok ? exp(l) : 0.;
+    s.logp[i] = l; s.p[i] = s.psum[i] = p; s.first[i] = ok;
+    sum += p;
+  }
+  __syncwarp();
+  if (twice)                                         // some class may be listed twice
+    for (int i = lane; i < a.k; i += 32) {
+      int first = s.id[i] >= 0; double ps = 0.;
+      for (int j = 0; j < a.k; ++j) if (s.id[j] == s.id[i]) { ps += s.p[j]; if (j < i) first = 0; }
+      s.first[i] = first; s.psum[i] = ps;
+    }
+  for (int i = lane; i < a.k; i += 32) if (s.first[i] && r.top > -INFINITY) e += exp(double(s.z[i]) / a.tau - r.top);
+  r.sum = warp_reduce(e, Add{});
+  sum = warp_reduce(sum, Add{});
+  r.rest = a.teacher_lse ? fmax(0., 1. - sum) : 0.;
+  r.mass = sum + r.rest;
+  return r;
+}
 
 // A token's row is cut at the 16-byte boundaries of its address: up to V - 1 entries before the first one belong to CTA 0, those behind
 // the last one to the last CTA (both kept as floats in `edge`), the vectors between are shared out evenly.
+// Eight warps run over the slice; a ninth does the list's 64-bit arithmetic meanwhile.
 template <class T> __global__ void __launch_bounds__(kClusterThreads, 3) distill_cluster_kernel(const __grid_constant__ DistillArgs a, uint32_t* status) {
   constexpr int V = 16 / sizeof(T);
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ float edge[2 * V], part[2];
+  __shared__ float edge[2 * V], part[2], warp_max[8], shared_top, shared_factor;
+  __shared__ double warp_sum[8];
   __shared__ uint64_t bar; __shared__ uint32_t abort_flag;
+  __shared__ __align__(16) uint32_t hash[kHashWords];
   uint4* slice = reinterpret_cast<uint4*>(smem);
   List s(smem + a.list_at, a.k);
   const int rank = int(blockIdx.x % unsigned(a.splits)); const int64_t token = blockIdx.x / unsigned(a.splits);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const T* z = static_cast<const T*>(a.z) + token * a.ldz;
   T* dz = a.dz ? static_cast<T*>(a.dz) + token * a.lddz : nullptr;
   const int mis = int(reinterpret_cast<uintptr_t>(z) / sizeof(T) % V), head = min((V - mis) % V, a.n), vectors = (a.n - head) / V, tail0 = head + vectors * V;
@@ -269,105 +336,139 @@ template <class T> __global__ void __launch_bounds__(kClusterThreads, 3) distill
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     const uint32_t bytes = uint32_t(v1 - v0) * 16;
     ptx::mbar_expect_tx(&bar, bytes);
-    for (uint32_t at = 0; at < bytes; at += 32768) ptx::bulk_load(ptx::smem_u32(smem) + at, reinterpret_cast<const uint8_t*>(z + head + v0 * V) + at, min(32768u, bytes - at), &bar);
+    for (uint32_t at = 0; at < bytes; at += 16384) ptx::bulk_load(ptx::smem_u32(smem) + at, reinterpret_cast<const uint8_t*>(z + head + v0 * V) + at, min(16384u, bytes - at), &bar);
+  }
+  for (int i = threadIdx.x; i < kHashWords / 4; i += kClusterThreads) reinterpret_cast<uint4*>(hash)[i] = make_uint4(0, 0, 0, 0);
+  __syncthreads();
+  int twice = 0;
+  for (int i = threadIdx.x; i < a.k; i += kClusterThreads) {
+    const int id = a.ids[token * a.ldk + i];
+    const bool ok = id >= 0 && id < a.n;
+    const float t = a.teacher[token * a.ldk + i];
+    s.id[i] = ok ? id : -1; s.logp[i] = ok ? double(t) / a.tau : -INFINITY; s.z[i] = ok ? to_f32(z[id]) : 0.f;
+    if (ok) { const uint32_t bit = 1u << (id & 31); twice |= (atomicOr(&hash[(id >> 5) & (kHashWords - 1)], bit) & bit) != 0; }
   }
   if (threadIdx.x < 2 * V) {
     const int j = int(threadIdx.x) < V ? int(threadIdx.x) : tail0 + int(threadIdx.x) - V;
     const bool mine = int(threadIdx.x) < V ? first && j < head : last && j < a.n;
     edge[threadIdx.x] = mine ? to_f32(z[j]) : -INFINITY;
   }
-  const Listed l = load_list<T>(a, token, z, s);
-  bool ok = ptx::mbar_wait(&bar, 0u, &abort_flag, status, 41u);
-  __syncthreads();                                   // every thread has seen the copy land before an entry is overwritten
+  ptx::mbar_wait(&bar, 0u, &abort_flag, status, 41u);      // expired: the status word says so, the values are then undefined
+  twice = __syncthreads_or(twice);                   // every thread has seen the copy land before an entry is overwritten
   for (int i = threadIdx.x; i < a.k; i += kClusterThreads) {      // listed classes leave the row (equal values for a class listed twice)
-    const int id = s.id[i], v = id < head ? -1 : (id - head) / V;
+    const int id = s.id[i];
     if (id < 0) continue;
     if (id < head) { if (first) edge[id] = -INFINITY; }
     else if (id >= tail0) { if (last) edge[V + id - tail0] = -INFINITY; }
-    else if (v >= v0 && v < v1) reinterpret_cast<T*>(slice)[id - head - v0 * V] = from_f32<T>(-INFINITY);
+    else { const int v = (id - head) / V; if (v >= v0 && v < v1) reinterpret_cast<T*>(slice)[id - head - v0 * V] = from_f32<T>(-INFINITY); }
   }
   __syncthreads();
-  float top, outside;
-  if (!a.stats_in) {
-    // maximum and sum of this slice, then one exchange
-    float m = threadIdx.x < 2 * V ? edge[threadIdx.x] : -INFINITY;
-    for (int v = threadIdx.x; v < v1 - v0; v += kClusterThreads) {
-      float f[V]; unpack<T>(slice[v], f);
+
+  Listed l{};
+  if (warp == 8) l = list_by_warp(a, token, s, twice != 0);
+  else if (!a.stats_in) {
+    // maximum and sum of this slice
+    RowMax<T> row_max;
+    for (int v = threadIdx.x; v < v1 - v0; v += kMainThreads) row_max.add(slice[v]);
+    float m = row_max.value();
+    if (threadIdx.x < 2 * V) m = fmaxf(m, edge[threadIdx.x]);
+    m = warp_reduce(m, Max{});
+    if (lane == 0) warp_max[warp] = m;
+    main_sync();
 #pragma unroll
-      for (int i = 0; i < V; ++i) m = fmaxf(m, f[i]);
-    }
-    m = block_reduce(m, Max{}, s.fbuf);
+    for (int w = 0; w < 8; ++w) m = fmaxf(m, warp_max[w]);
     const Exponent e(a.tau, m == -INFINITY ? 0.f : m);
     float sum = threadIdx.x < 2 * V ? e(edge[threadIdx.x]) : 0.f;
-    for (int v = threadIdx.x; v < v1 - v0; v += kClusterThreads) {
+#pragma unroll 2
+    for (int v = threadIdx.x; v < v1 - v0; v += kMainThreads) {
       float f[V]; unpack<T>(slice[v], f);
-      float q[V];
 #pragma unroll
-      for (int i = 0; i < V; ++i) q[i] = e(f[i]);
+      for (int i = 0; i < V; ++i) f[i] = e(f[i]);
 #pragma unroll
       for (int d = V / 2; d; d /= 2)
 #pragma unroll
-        for (int i = 0; i < d; ++i) q[i] += q[i + d];
-      sum += q[0];
+        for (int i = 0; i < d; ++i) f[i] += f[i + d];
+      sum += f[0];
     }
-    const double mine = block_reduce(double(sum), Add{}, s.buf) * e.fix;
-    if (a.splits > 1) {
-      if (threadIdx.x == 0) { part[0] = m; part[1] = float(mine); }
-      cluster_arrive(); cluster_wait();
-      top = -INFINITY;
-      for (int r = 0; r < a.splits; ++r) top = fmaxf(top, ld_cluster(&part[0], r));
-      if (top == -INFINITY) top = 0.f;
-      double total = 0.;
-      for (int r = 0; r < a.splits; ++r) {
-        const float pm = ld_cluster(&part[0], r), ps = ld_cluster(&part[1], r);
-        total += pm == -INFINITY ? 0. : pm == top ? double(ps) : double(ps) * exp2((double(pm) - double(top)) * double(e.scale));
-      }
-      outside = float(total);
-      cluster_arrive();                              // peers may leave once everybody has read
-    } else { top = m == -INFINITY ? 0.f : m; outside = float(mine); }
-  } else {
-    top = a.stats_in[2 * token]; outside = a.stats_in[2 * token + 1];
-    if (a.splits > 1) { cluster_arrive(); cluster_wait(); cluster_arrive(); }      // in place: every CTA has read the listed logits
-  }
-  const Student st(a, l, top, outside);
-  if (first && (a.loss || a.stats_out)) {
-    const double loss = distill_loss(a, s, l, st, weight);
+    const double mine = warp_reduce(double(sum), Add{});
+    if (lane == 0) warp_sum[warp] = mine;
+    main_sync();
     if (threadIdx.x == 0) {
-      if (a.loss) a.loss[token] = float(loss);
-      if (a.stats_out) { a.stats_out[2 * token] = top; a.stats_out[2 * token + 1] = outside; }
+      double total = 0.;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) total += warp_sum[w];
+      part[0] = m; part[1] = float(total * e.fix());
     }
   }
-  if (dz) {
+  if (a.splits > 1) { __syncwarp(); cluster_arrive(); cluster_wait(); }      // also: every CTA has read the listed logits, the gradient may go in their place
+  else __syncthreads();
+  if (warp == 8) {
+    float top, outside;
+    if (a.stats_in) { top = a.stats_in[2 * token]; outside = a.stats_in[2 * token + 1]; }
+    else {
+      // one CTA's part per lane
+      const float pm = lane >= a.splits ? -INFINITY : a.splits > 1 ? ld_cluster(&part[0], lane) : part[0];
+      const float ps = lane >= a.splits ? 0.f : a.splits > 1 ? ld_cluster(&part[1], lane) : part[1];
+      top = warp_reduce(pm, Max{});
+      if (top == -INFINITY) top = 0.f;
+      const double scale = double(float(1.4426950408889634 / a.tau));
+      const double share = pm == -INFINITY ? 0. : pm == top ? double(ps) : double(ps) * exp2((double(pm) - double(top)) * scale);
+      outside = float(warp_reduce(share, Add{}));
+    }
+    const Student st(a, l, top, outside);
     const Exponent e(a.tau, top);
-    const float factor = float(outside_factor(a, l, st, outside, weight) * e.fix);
-    for (int v = threadIdx.x; v < v1 - v0; v += kClusterThreads) {
-      float f[V]; unpack<T>(slice[v], f);
-#pragma unroll
-      for (int i = 0; i < V; ++i) f[i] = factor * e(f[i]);
-      T* to = dz + head + (v0 + v) * V;
-      if (same) *reinterpret_cast<uint4*>(to) = pack<T>(f);
-      else
-#pragma unroll
-        for (int i = 0; i < V; ++i) to[i] = from_f32<T>(f[i]);
+    if (lane == 0) { shared_top = top; shared_factor = float(outside_factor(a, l, st, outside, weight) * e.fix()); }
+    __syncthreads();
+    if (a.splits > 1) cluster_arrive();              // peers may leave once everybody has read
+    if (first && (a.loss || a.stats_out)) {
+      double kl = 0.;
+      for (int i = lane; i < a.k; i += 32) if (s.p[i] != 0.) kl += s.p[i] * (s.logp[i] - (st.empty ? -INFINITY : double(s.z[i]) / a.tau - st.lse));
+      kl = warp_reduce(kl, Add{});
+      if (l.rest > 0.) kl += l.rest * (log(l.rest) - (st.no_outside ? -INFINITY : st.lse_out - st.lse));
+      if (lane == 0) {
+        if (a.loss) a.loss[token] = float(kl * weight);
+        if (a.stats_out) { a.stats_out[2 * token] = top; a.stats_out[2 * token + 1] = outside; }
+      }
     }
-    if (threadIdx.x < 2 * V) {
-      const int j = int(threadIdx.x) < V ? int(threadIdx.x) : tail0 + int(threadIdx.x) - V;
-      if (int(threadIdx.x) < V ? first && j < head : last && j < a.n) dz[j] = from_f32<T>(factor * e(edge[threadIdx.x]));
+    if (dz) {
+      for (int i = lane; i < a.k; i += 32) if (s.first[i]) s.psum[i] = double(listed_gradient(a, s, l, st, weight, i));
+      __syncthreads();                               // the listed classes are written last
+      for (int i = lane; i < a.k; i += 32) {
+        const int id = s.id[i];
+        if (!s.first[i]) continue;
+        const bool mine = id < head ? first : id >= tail0 ? last : (id - head) / V >= v0 && (id - head) / V < v1;
+        if (mine) dz[id] = from_f32<T>(float(s.psum[i]));
+      }
     }
-    __syncthreads();                                 // the listed classes are written last
-    for (int i = threadIdx.x; i < a.k; i += kClusterThreads) {
-      const int id = s.id[i];
-      if (!s.first[i]) continue;
-      const bool mine = id < head ? first : id >= tail0 ? last : (id - head) / V >= v0 && (id - head) / V < v1;
-      if (mine) dz[id] = from_f32<T>(listed_gradient(a, s, l, st, weight, i));
+  } else {
+    __syncthreads();
+    if (a.splits > 1) cluster_arrive();
+    if (dz) {
+      const Exponent e(a.tau, shared_top);
+      const float factor = shared_factor;
+#pragma unroll 2
+      for (int v = threadIdx.x; v < v1 - v0; v += kMainThreads) {
+        float f[V]; unpack<T>(slice[v], f);
+#pragma unroll
+        for (int i = 0; i < V; ++i) f[i] = factor * e(f[i]);
+        T* to = dz + head + (v0 + v) * V;
+        if (same) __stcs(reinterpret_cast<uint4*>(to), pack<T>(f));
+        else
+#pragma unroll
+          for (int i = 0; i < V; ++i) to[i] = from_f32<T>(f[i]);
+      }
+      if (threadIdx.x < 2 * V) {
+        const int j = int(threadIdx.x) < V ? int(threadIdx.x) : tail0 + int(threadIdx.x) - V;
+        if (int(threadIdx.x) < V ? first && j < head : last && j < a.n) dz[j] = from_f32<T>(factor * e(edge[threadIdx.x]));
+      }
+      __syncthreads();
     }
   }
   if (a.splits > 1) cluster_wait();
-  (void)ok;                                          // an expired wait is in the status word; the values are then undefined
 }
 
 // Slices of at most 72 KiB where eight CTAs allow it (three CTAs per SM), otherwise what one CTA per SM takes.
-constexpr int kSliceBytes = 72 * 1024, kSmemMost = 225 * 1024;
+constexpr int kSliceBytes = 72 * 1024, kSmemMost = 216 * 1024;
 
 template <class T> cudaError_t raise_limit(const hyacinHandle_t* handle, T* kernel, std::atomic<uint64_t>& ready) {
   const uint64_t bit = uint64_t(1) << (handle->DeviceID & 63);      // per device

@@ -4,6 +4,7 @@
 // The quotient decides a whole number, so it is taken in 64 bits: w and s carry at most 24 bits, a quotient that is not
 // exactly a half differs from it by at least 2^-28 relative, and rint of the 64-bit quotient is that of the exact one.
 #include "w4.cuh"
+#include <algorithm>
 
 namespace hyb {
 namespace {
@@ -23,18 +24,145 @@ struct SegmentCode {        // what a segment's codes are computed with
   }
 };
 
-// lo, hi: extremes of the segment together with 0; bad: it holds a NaN or an infinity.
+// rint(v / s), ties to even, as if the quotient were exact.  v * inverse is off by at most 2^-22 of itself, so its nearest whole number
+// is wrong by one at most and only next to a half.  The remainder v - whole s is exact in 32 bits (a multiple of the smaller of
+// the two last places, and at most about s / 2), and twice that against s decides.  Quotients of 32 and more, which only a scale that
+// was rounded to next to nothing leaves, go through 64 bits.  Adding and subtracting 1.5 * 2^23 rounds to the nearest whole number
+// on the floating-point pipe: the conversion instructions, four per weight, took longer than DRAM.
+constexpr float kRound = 12582912.f;
+__device__ __forceinline__ float rounded_quotient(float v, float s, float inverse) {
+  const float t = v * inverse;
+  if (!(fabsf(t) < 32.f)) return float(fmin(fmax(rint(double(v) / double(s)), -64.), 64.));
+  const float m = __fadd_rn(t, kRound);
+  float whole = __fadd_rn(m, -kRound);
+  const float r = fmaf(-whole, s, v), twice = 2.f * fabsf(r);
+  if (twice >= s && (twice > s || (__float_as_int(m) & 1))) whole += copysignf(1.f, r);
+  return whole;
+}
+
+// lo, hi: extremes of the segment together with 0; bad: it holds a NaN or an infinity.  float(double / 7) is the 32-bit quotient;
+// so is float(double / 15) of a difference that 32 bits hold.
 template <class S> __device__ __forceinline__ SegmentCode segment_code(float lo, float hi, bool bad, bool symmetric, S* scale) {
   SegmentCode c;
-  const double span = symmetric ? double(fmaxf(-lo, hi)) / 7. : (double(hi) - double(lo)) / 15.;
-  *scale = bad ? from_f32<S>(__int_as_float(0x7fc00000)) : from_f32<S>(float(span));
-  c.s = double(to_f32(*scale));
-  c.live = c.s > 0.;                                   // false for NaN as well
-  c.zero = symmetric ? 8 : c.live ? int(fmin(fmax(rint(-double(lo) / c.s), 0.), 15.)) : 0;
+  float span;
+  if (symmetric) span = __fdiv_rn(fmaxf(-lo, hi), 7.f);
+  else {
+    const double d = double(hi) - double(lo); const float f = float(d);
+    span = double(f) == d ? __fdiv_rn(f, 15.f) : float(d / 15.);
+  }
+  *scale = from_f32<S>(bad ? __int_as_float(0x7fc00000) : span);
+  const float s = to_f32(*scale);
+  c.s = double(s);
+  c.live = s > 0.f;                                    // false for NaN as well
+  if (symmetric) c.zero = 8;
+  else if (!c.live) c.zero = 0;
+  else {
+    c.zero = int(fminf(fmaxf(rounded_quotient(-lo, s, 1.f / s), 0.f), 15.f));
+  }
   return c;
 }
 
-// One warp per (column, segment): a pass for the extremes, a pass for the codes.
+// Segments of 32, 64, 128 or 256 rows: a lane owns eight consecutive rows, one word of codes, a warp 256 rows of a column; a
+// segment's lanes are neighbours and find its extremes with shuffles, so W is read once and everything stays in registers.
+// Rows that are not 16-byte aligned pass through shared memory, so that DRAM sees whole lines all the same.
+// Bound: DRAM (read W, write half a byte per weight, and 4 bytes of residual where asked for).
+// A warp walks down the columns of its row group with the next column's load in flight.
+template <class T, class S> __global__ void __launch_bounds__(256) quantize_w4_warp_kernel(QuantizeArgs a, int w_aligned, int r_aligned) {
+  __shared__ float turns[8][256];
+  constexpr int kWords = int(sizeof(T)) * 8 / 16;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  float* turn = turns[warp];
+  const int row0 = blockIdx.x * 256, row = row0 + lane * 8, valid = a.m - row, all = a.m - row0;
+  const bool wide = w_aligned && all >= 256, symmetric = a.zeros == nullptr;
+  const int step = gridDim.y * 8, lanes = a.seg / 8, r8 = row / 8;
+  const bool writes = r8 < (a.m + kW4Block - 1) / kW4Block * 16, leads = lane % lanes == 0 && valid > 0;
+  const int64_t code_at = int64_t(r8 / 16) * 64 + (4 * (r8 & 3) + ((r8 >> 2) & 3)) * 4;
+  const T* w = static_cast<const T*>(a.w) + row0;
+  uint4 raw[kWords]; T part[8];
+  auto fetch = [&](int col) {
+    if (col >= a.n) return;
+    const T* from = w + col * a.ldw;
+    if (wide) {
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) raw[i] = __ldcs(reinterpret_cast<const uint4*>(from + lane * 8) + i);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) if (i * 32 + lane < all) part[i] = from[i * 32 + lane];
+    }
+  };
+  int col = blockIdx.y * 8 + warp;
+  fetch(col);
+  for (; col < a.n; col += step) {
+    float v[8];
+    if (wide) {
+      const T* e = reinterpret_cast<const T*>(raw);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = to_f32(e[i]);
+    } else {
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 8; ++i) turn[i * 32 + lane] = i * 32 + lane < all ? to_f32(part[i]) : 0.f;
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = turn[lane * 8 + i];
+      __syncwarp();
+    }
+    fetch(col + step);
+    // the largest magnitude as an integer finds infinities and NaNs as well
+    int size = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) size = max(size, __float_as_int(v[i]) & 0x7fffffff);
+    float lo = 0.f, hi = 0.f;
+    if (symmetric) {
+      for (int d = 1; d < lanes; d *= 2) size = max(size, __shfl_xor_sync(~0u, size, d));
+      hi = __int_as_float(size);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) { lo = fminf(lo, v[i]); hi = fmaxf(hi, v[i]); }
+      for (int d = 1; d < lanes; d *= 2) {
+        size = max(size, __shfl_xor_sync(~0u, size, d)); lo = fminf(lo, __shfl_xor_sync(~0u, lo, d)); hi = fmaxf(hi, __shfl_xor_sync(~0u, hi, d));
+      }
+    }
+    S scale; const SegmentCode c = segment_code<S>(lo, hi, size >= 0x7f800000, symmetric, &scale);
+    if (leads) {
+      const int64_t at = col * a.lds + row / a.seg;
+      static_cast<S*>(a.scales)[at] = scale;
+      if (!symmetric) a.zeros[at] = uint8_t(c.zero);
+    }
+    const float s = to_f32(scale), inverse = 1.f / s;
+    // codes minus their zero point lie in [low, high]; 0 for a segment without a scale
+    const float zero = float(c.zero), low = !c.live ? 0.f : symmetric ? -7.f : -zero, high = !c.live ? 0.f : symmetric ? 7.f : 15.f - zero;
+    uint32_t word = 0;
+    float r[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float whole = c.live ? fminf(fmaxf(rounded_quotient(v[i], s, inverse), low), high) : 0.f;
+      const uint32_t q = __float_as_uint(whole + (kRound + zero)) & 15u;
+      word |= q << (4 * w4_row_nibble(i));
+      r[i] = fmaf(-s, whole, v[i]);
+    }
+    if (valid < 8) {                                 // rows behind the last one are stored as 0
+#pragma unroll
+      for (int i = 0; i < 8; ++i) if (i >= valid) word &= ~(15u << (4 * w4_row_nibble(i)));
+    }
+    if (writes) *reinterpret_cast<uint32_t*>(a.codes + col * a.ldq + code_at) = word;
+    if (a.r) {
+      float* to = a.r + col * a.ldr + row0;
+      if (r_aligned && all >= 256) {
+        __stcs(reinterpret_cast<float4*>(to + lane * 8), make_float4(r[0], r[1], r[2], r[3]));
+        __stcs(reinterpret_cast<float4*>(to + lane * 8) + 1, make_float4(r[4], r[5], r[6], r[7]));
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) turn[lane * 8 + i] = r[i];
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) if (i * 32 + lane < all) __stcs(to + i * 32 + lane, turn[i * 32 + lane]);
+      }
+    }
+  }
+}
+
+// Any other segment length: one warp per (column, segment), a pass for the extremes, a pass for the codes.
 template <class T, class S> __global__ void __launch_bounds__(256) quantize_w4_kernel(QuantizeArgs a) {
   const int lane = threadIdx.x & 31;
   const int64_t task = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5);
@@ -93,6 +221,17 @@ extern "C" int32_t hyacinB200QuantizeW4(const hyacinHandle_t* handle, hyacinPrec
   if (blocks > 0x7fffffff) return w4_refuse(fn, "too many segments");
   timer_mark(handle, Segment::Replicated);
   count_launch();
+  if (segM == 32 || segM == 64 || segM == 128 || segM == 256) {
+    const int64_t groups = (int64_t(M) + 255) / 256;
+    const int w_aligned = reinterpret_cast<uintptr_t>(W) % 16 == 0 && int64_t(ldw) * int64_t(w4_type_bytes(Wtype)) % 16 == 0;
+    const int r_aligned = reinterpret_cast<uintptr_t>(R) % 16 == 0 && ldr % 4 == 0;
+    // about six blocks per SM, so that a warp sees several columns
+    const int64_t chunks = std::max<int64_t>(1, std::min<int64_t>({(int64_t(N) + 7) / 8, 6 * int64_t(handle->DeviceSMs) / groups, 65535}));
+    with_w4_type(Wtype, [&](auto t) { with_w4_type(Stype, [&](auto s) {
+      quantize_w4_warp_kernel<decltype(t), decltype(s)><<<dim3(unsigned(groups), unsigned(chunks)), 256, 0, handle->cudaStream>>>(a, w_aligned, r_aligned);
+    }); });
+    return w4_launched("quantize_w4_warp_kernel");
+  }
   with_w4_type(Wtype, [&](auto t) { with_w4_type(Stype, [&](auto s) {
     quantize_w4_kernel<decltype(t), decltype(s)><<<unsigned(blocks), 256, 0, handle->cudaStream>>>(a);
   }); });
