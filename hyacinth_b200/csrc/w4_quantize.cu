@@ -24,21 +24,20 @@ struct SegmentCode {        // what a segment's codes are computed with
   }
 };
 
-// rint(v / s), ties to even, as if the quotient were exact.  v * inverse is off by at most 2^-22 of itself, so its nearest whole number
-// is wrong by one at most and only next to a half.  The remainder v - whole s is exact in 32 bits (a multiple of the smaller of
-// the two last places, and at most about s / 2), and twice that against s decides.  Quotients of 32 and more, which only a scale that
-// was rounded to next to nothing leaves, go through 64 bits.  Adding and subtracting 1.5 * 2^23 rounds to the nearest whole number
-// on the floating-point pipe: the conversion instructions, four per weight, took longer than DRAM.
+// rint(v / s), ties to even, as if the quotient were exact, given `inverse` = 1 / s to within 2^-22.  v * inverse then finds the nearest
+// whole number, or next to a half its neighbour.  The remainder v - whole s is exact in 32 bits (a multiple of the smaller of
+// the two last places, and at most about s / 2), and twice that against s decides.  Adding and subtracting 1.5 * 2^23 rounds to
+// a whole number on the floating-point pipe: the conversion instructions, four per weight, took longer than DRAM.
 constexpr float kRound = 12582912.f;
 __device__ __forceinline__ float rounded_quotient(float v, float s, float inverse) {
-  const float t = v * inverse;
-  if (!(fabsf(t) < 32.f)) return float(fmin(fmax(rint(double(v) / double(s)), -64.), 64.));
-  const float m = __fadd_rn(t, kRound);
-  float whole = __fadd_rn(m, -kRound);
-  const float r = fmaf(-whole, s, v), twice = 2.f * fabsf(r);
-  if (twice >= s && (twice > s || (__float_as_int(m) & 1))) whole += copysignf(1.f, r);
-  return whole;
+  const float m = __fmaf_rn(v, inverse, kRound), whole = __fadd_rn(m, -kRound), r = __fmaf_rn(-whole, s, v), twice = 2.f * fabsf(r);
+  const bool off = twice > s || (twice == s && (__float_as_int(m) & 1));
+  return off ? whole + copysignf(1.f, r) : whole;
 }
+// That holds for ordinary scales and quotients below 32 in magnitude; `largest`: of the segment's weights.
+__device__ __forceinline__ bool ordinary(float s, float inverse, float largest) { return s > 1e-30f && s < 1e30f && largest * inverse < 32.f; }
+__device__ __noinline__ float quotient_in_64_bits(float v, float s) { return float(fmin(fmax(rint(double(v) / double(s)), -64.), 64.)); }
+__device__ __forceinline__ float reciprocal(float s) { float r; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s)); return r; }
 
 // lo, hi: extremes of the segment together with 0; bad: it holds a NaN or an infinity.  float(double / 7) is the 32-bit quotient;
 // so is float(double / 15) of a difference that 32 bits hold.
@@ -57,7 +56,8 @@ template <class S> __device__ __forceinline__ SegmentCode segment_code(float lo,
   if (symmetric) c.zero = 8;
   else if (!c.live) c.zero = 0;
   else {
-    c.zero = int(fminf(fmaxf(rounded_quotient(-lo, s, 1.f / s), 0.f), 15.f));
+    const float inverse = reciprocal(s);
+    c.zero = int(fminf(fmaxf(ordinary(s, inverse, -lo) ? rounded_quotient(-lo, s, inverse) : quotient_in_64_bits(-lo, s), 0.f), 15.f));
   }
   return c;
 }
@@ -67,7 +67,7 @@ template <class S> __device__ __forceinline__ SegmentCode segment_code(float lo,
 // Rows that are not 16-byte aligned pass through shared memory, so that DRAM sees whole lines all the same.
 // Bound: DRAM (read W, write half a byte per weight, and 4 bytes of residual where asked for).
 // A warp walks down the columns of its row group with the next column's load in flight.
-template <class T, class S> __global__ void __launch_bounds__(256) quantize_w4_warp_kernel(QuantizeArgs a, int w_aligned, int r_aligned) {
+template <class T, class S> __global__ void __launch_bounds__(256, 4) quantize_w4_warp_kernel(QuantizeArgs a, int w_aligned, int r_aligned) {
   __shared__ float turns[8][256];
   constexpr int kWords = int(sizeof(T)) * 8 / 16;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -129,17 +129,27 @@ template <class T, class S> __global__ void __launch_bounds__(256) quantize_w4_w
       static_cast<S*>(a.scales)[at] = scale;
       if (!symmetric) a.zeros[at] = uint8_t(c.zero);
     }
-    const float s = to_f32(scale), inverse = 1.f / s;
-    // codes minus their zero point lie in [low, high]; 0 for a segment without a scale
+    const float s = to_f32(scale), inverse = reciprocal(s);
+    const bool slow = c.live && !ordinary(s, inverse, __int_as_float(size));
+    // codes minus their zero point lie in [low, high]: 0 for a segment without a scale (also where the quotient is a NaN)
     const float zero = float(c.zero), low = !c.live ? 0.f : symmetric ? -7.f : -zero, high = !c.live ? 0.f : symmetric ? 7.f : 15.f - zero;
     uint32_t word = 0;
     float r[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float whole = c.live ? fminf(fmaxf(rounded_quotient(v[i], s, inverse), low), high) : 0.f;
+      const float whole = fminf(fmaxf(rounded_quotient(v[i], s, inverse), low), high);
       const uint32_t q = __float_as_uint(whole + (kRound + zero)) & 15u;
       word |= q << (4 * w4_row_nibble(i));
       r[i] = fmaf(-s, whole, v[i]);
+    }
+    if (slow) {                                      // the same with quotients in 64 bits
+      word = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float whole = fminf(fmaxf(quotient_in_64_bits(v[i], s), low), high);
+        word |= (__float_as_uint(whole + (kRound + zero)) & 15u) << (4 * w4_row_nibble(i));
+        r[i] = fmaf(-s, whole, v[i]);
+      }
     }
     if (valid < 8) {                                 // rows behind the last one are stored as 0
 #pragma unroll
