@@ -1,6 +1,7 @@
 // Products of a few vectors with a 4-bit weight matrix, Y = Wq^T X + V (U^T X) and Y = Wq X + U (V^T X), with
 // Wq(r, j) = s(j, r / segM) (q(r, j) - zero(j, r / segM)).
 #include "w4_product.h"
+#include <algorithm>
 
 namespace hyb {
 namespace {
@@ -108,7 +109,10 @@ extern "C" int32_t hyacinB200ProductW4(const hyacinHandle_t* handle, char opW, i
   timer_mark(handle, Segment::Replicated);
   if (in > 0 && trans) {
     const int per = product_stream_vectors(Xtype, a);
-    if (per > 0 && (Xtype == HYACIN_F32 || (T <= 8 && per >= T))) return launch_product_stream(handle, fn, Xtype, a);
+    // Up to eight vectors stream (17 against 23 us, 4096 x 16384); up to sixteen where the tensor-core kernel cannot fetch a block's
+    // scales at once (24 against 58 us, 5001 x 6003, segments of 32 rows, odd table pitch).
+    const bool scattered = segM % 128 != 0 && (segM == 96 || lds % (128 / std::min(segM, 64)) != 0 || reinterpret_cast<uintptr_t>(scales) % (256 / std::min(segM, 64)) != 0);
+    if (per > 0 && (Xtype == HYACIN_F32 || (per >= T && (T <= 8 || scattered)))) return launch_product_stream(handle, fn, Xtype, a);
   }
   if (in > 0 && Xtype != HYACIN_F32) return launch_product_umma(handle, fn, trans, Xtype, a);
   float* mid = nullptr;

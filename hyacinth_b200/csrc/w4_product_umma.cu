@@ -52,7 +52,7 @@ struct UmmaParams {
   int segs, seg_sub, seg_shift;                   // 32-row subsets per segment; shift when that is a power of two, else -1
   int wide;                                       // segments of a block that one aligned load fetches (1, 2, 4)
   int code_steps, steps;                          // K steps of codes, and with those of the correction
-  int rank; const void* second; int64_t ld2;
+  int rank, rank16; const void* second; int64_t ld2;      // rank16: rank rounded up to 16, the width of either part of mid
   void* y; int64_t ldy;
   int nt, ring, bufs, groups, splits, second_aligned; uint32_t nt_cols, tmem_cols, idesc;
   uint32_t* status;
@@ -331,6 +331,11 @@ product_umma_kernel(const __grid_constant__ CUtensorMap code_map, const __grid_c
         }
       }
     };
+    if (p.rank && step1 == p.steps) {                // the correction's factor comes last: into the L2 meanwhile
+      const char* from = static_cast<const char*>(p.second) + int64_t(tile) * kOut * 2;
+      for (int k = threadIdx.x - 64; k < 2 * p.rank; k += 32 * kLoaders)
+        if (tile * kOut + 64 * (k & 1) < p.out) asm volatile("prefetch.global.L2 [%0];" ::"l"(from + int64_t(k >> 1) * p.ld2 * 2 + 128 * (k & 1)));
+    }
     uint32_t stage = (warp - 2) % p.ring, phase = 0;
     auto hand_over = [&](int k, const Entry (&e)[kPer]) {
       if (!warp_wait<true>(&bars->empty[stage], phase ^ 1u, abort_flag, p.status, 20u)) return false;
@@ -383,6 +388,7 @@ product_umma_kernel(const __grid_constant__ CUtensorMap code_map, const __grid_c
                    : "+r"(good) : "r"(group + 1) : "memory");
       return good != 0;
     };
+    auto group_sync = [&] { asm volatile("bar.sync %0, 128;" ::"r"(group + 1) : "memory"); };
     uint32_t stage = group, phase = 0, buf = group;
     for (int k = group < p.groups ? step0 + group : step1; k < step1; k += p.groups) {
       const int s = k - step0 - p.bufs;
@@ -418,27 +424,57 @@ product_umma_kernel(const __grid_constant__ CUtensorMap code_map, const __grid_c
           }
         }
       } else {
-        // correction step: entry (output, c) of the operand is second(output, c mod rank), c < 2 rank
+        // correction step: entry (output, c) of the operand is second(output, c mod rank16), c < 2 rank16; mid is zero behind the rank
         const uint16_t* second = static_cast<const uint16_t*>(p.second);
         const int c0 = (k - p.code_steps) * kStep;
         if constexpr (TRANS) {
-          const int out = tile * kOut + row;
-#pragma unroll 1
-          for (int pair = 0; pair < 2; ++pair) {
-            uint32_t o[32];
+          // 32 columns from c at a time through the stage's own, now idle, code buffer: rows of 128 outputs in, one output's values out
+          uint32_t o[32];
+          const uint32_t turn = base + stage * G::code_bytes;
+          const uint16_t* from = second + tile * kOut;
+          const int valid = p.out - tile * kOut;
+          auto gather = [&](int c, uint32_t* to) {
+            uint4 v[4];
 #pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              const int a = c0 + pair * 64 + 2 * e, b = a + 1;
-              const uint32_t lo = a < 2 * p.rank && out < p.out ? second[out + int64_t(a < p.rank ? a : a - p.rank) * p.ld2] : 0u;
-              const uint32_t hi = b < 2 * p.rank && out < p.out ? second[out + int64_t(b < p.rank ? b : b - p.rank) * p.ld2] : 0u;
-              o[e] = lo | hi << 16;
+            for (int i = 0; i < 4; ++i) {
+              const int e = (id & 127) + 128 * i, chunk = e & 15;
+              int a = c + (e >> 4);
+              if (a >= 2 * p.rank16) a -= 2 * p.rank16;
+              if (a >= p.rank16) a -= p.rank16;
+              v[i] = load8(reinterpret_cast<const T*>(from + int64_t(a) * p.ld2) + chunk * 8, a < p.rank ? valid - chunk * 8 : 0, p.second_aligned != 0);
             }
-            tmem_st32(tdst + pair * 32, o);
+            group_sync();
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sts128(turn + ((id & 127) + 128 * i) * 16, v[i].x, v[i].y, v[i].z, v[i].w);
+            group_sync();
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              uint16_t lo, hi;
+              asm volatile("ld.shared.u16 %0, [%1];" : "=h"(lo) : "r"(turn + (2 * e) * 256 + row * 2));
+              asm volatile("ld.shared.u16 %0, [%1];" : "=h"(hi) : "r"(turn + (2 * e + 1) * 256 + row * 2));
+              to[e] = uint32_t(lo) | uint32_t(hi) << 16;
+            }
+          };
+          if (p.rank16 <= 64 && 64 % p.rank16 == 0) {                // the pattern repeats every 64 columns
+            gather(0, o);
+            if (p.rank16 == 64) gather(32, o + 16);
+            else {
+#pragma unroll
+              for (int e = 0; e < 16; ++e) o[16 + e] = o[e];
+            }
+            tmem_st32(tdst, o); tmem_st32(tdst + 32, o);
+          } else {
+#pragma unroll 1
+            for (int pair = 0; pair < 2; ++pair) {
+              const int c = (c0 + pair * 64) % (2 * p.rank16);
+              gather(c, o); gather((c + 32) % (2 * p.rank16), o + 16);
+              tmem_st32(tdst + pair * 32, o);
+            }
           }
         } else {
-          const int c = c0 + row;
-          const uint16_t* from = second + int64_t(c < p.rank ? c : c - p.rank) * p.ld2 + tile * kOut + 64 * half;
-          const int valid = c < 2 * p.rank ? p.out - tile * kOut - 64 * half : 0;
+          const int c = c0 + row, of = c < p.rank16 ? c : c - p.rank16;
+          const uint16_t* from = second + int64_t(of) * p.ld2 + tile * kOut + 64 * half;
+          const int valid = c < 2 * p.rank16 && of < p.rank ? p.out - tile * kOut - 64 * half : 0;
 #pragma unroll 4
           for (int j = 0; j < 8; ++j) {
             const uint4 v = load8(reinterpret_cast<const T*>(from) + 8 * j, valid - 8 * j, p.second_aligned != 0);
@@ -498,7 +534,7 @@ product_umma_kernel(const __grid_constant__ CUtensorMap code_map, const __grid_c
   }
 }
 
-// ---- mid = first^T X for many tokens, as two 16-bit parts: [token][value 0 .. rank, remainder 0 .. rank] ----------------------
+// ---- mid = first^T X for many tokens, as two 16-bit parts: [token][value, remainder], each padded with zeros to a multiple of 16 ----------------------
 template <class T> __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1);
 template <> __device__ __forceinline__ void mma16816<__half>(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -509,22 +545,25 @@ template <> __device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&d)[4
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-constexpr int kMidWarps = 16;
-// A block: 16 entries of the rank x 16 tokens; its warps split the rows.  A lane feeds eight consecutive rows of each operand
-// row to two instructions: the order of K inside an instruction is free as long as both operands agree.
+constexpr int kMidWarps = 4, kMidSplits = 8;
+// A cluster of eight blocks: 16 entries of the rank x 16 tokens, the blocks and their warps split the rows, sums joined in shared memory
+// and across the cluster in a fixed order.  A lane feeds eight consecutive rows of each operand row to two instructions: the
+// order of K inside an instruction is free as long as both operands agree.  The product waits for this kernel, so what counts is
+// its latency: 4096 rows, rank 64, 256 tokens took 9 us with one block per tile.
 template <class T> __global__ void __launch_bounds__(kMidWarps * 32)
 mid_split_kernel(const T* first, int64_t ld1, int rows, int rank, const T* x, int64_t ldx, int t, T* mid, int64_t ldm, int aligned) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   __shared__ float red[kMidWarps][16][17];
+  __shared__ __align__(16) float part[256];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-  const int k0 = blockIdx.x * 16; const int64_t t0 = int64_t(blockIdx.y) * 16;
+  const int split = blockIdx.x % kMidSplits, k0 = blockIdx.x / kMidSplits * 16; const int64_t t0 = int64_t(blockIdx.y) * 16;
   const T* fp[2] = {first + int64_t(k0 + g) * ld1, first + int64_t(k0 + g + 8) * ld1};
   const T* xp[2] = {x + (t0 + g) * ldx, x + (t0 + g + 8) * ldx};
   const bool fl[2] = {k0 + g < rank, k0 + g + 8 < rank}, xl[2] = {t0 + g < t, t0 + g + 8 < t};
   float acc[2][4] = {};
 #pragma unroll 4
-  for (int r = warp * 32 + c * 8; r < (rows + 31) / 32 * 32; r += kMidWarps * 32) {
-    const int valid = rows - r;
+  for (int64_t r0 = (split * kMidWarps + warp) * 32; r0 < rows; r0 += kMidSplits * kMidWarps * 32) {
+    const int64_t r = r0 + c * 8; const int valid = int(rows - r);
     uint4 a[2], b[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -541,17 +580,33 @@ mid_split_kernel(const T* first, int64_t ld1, int rows, int rank, const T* x, in
 #pragma unroll
     for (int e = 0; e < 4; ++e) red[warp][g + 8 * (e >> 1)][8 * i + 2 * c + (e & 1)] = acc[i][e];
   __syncthreads();
-  if (threadIdx.x < 256) {
-    const int k = threadIdx.x & 15, tok = threadIdx.x >> 4;
-    float s = 0.f;
+  {
+    for (int e = threadIdx.x; e < 256; e += kMidWarps * 32) {
+      float s = 0.f;
 #pragma unroll
-    for (int w = 0; w < kMidWarps; ++w) s += red[w][k][tok];
-    if (k0 + k < rank && t0 + tok < t) {
-      T* m = mid + (t0 + tok) * ldm + k0 + k;
-      const T value = from_f32<T>(s);
-      m[0] = value; m[rank] = from_f32<T>(s - to_f32(value));
+      for (int w = 0; w < kMidWarps; ++w) s += red[w][e & 15][e >> 4];
+      part[e] = s;
     }
   }
+  cluster_sync_all();
+  if (threadIdx.x < 256 / kMidSplits / 4) {
+    const int e = split * (256 / kMidSplits) + threadIdx.x * 4;
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int r = 0; r < kMidSplits; ++r) { const float4 v = ld_cluster4(smem_u32(part + e), r); s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w; }
+    const float v[4] = {s.x, s.y, s.z, s.w};
+    const int tok = e >> 4;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int k = k0 + (e & 15) + i;
+      if (t0 + tok < t) {                            // zeros behind the rank
+        T* m = mid + (t0 + tok) * ldm + k;
+        const T value = from_f32<T>(v[i]);
+        m[0] = value; m[ldm / 2] = from_f32<T>(v[i] - to_f32(value));
+      }
+    }
+  }
+  cluster_sync_all();
 }
 
 // X with rows that TMA can address (16-byte pitch and start).
@@ -615,8 +670,8 @@ template <class T, bool TRANS> int32_t launch(const hyacinHandle_t* handle, cons
   using G = Geometry<TRANS>;
   constexpr int kStep = G::step;
   p.code_steps = (in + kStep - 1) / kStep;
-  p.rank = a.rank; p.second = a.second; p.ld2 = a.ld2; p.y = a.y; p.ldy = a.ldy;
-  p.steps = p.code_steps + (2 * a.rank + kStep - 1) / kStep;
+  p.rank = a.rank; p.rank16 = (a.rank + 15) / 16 * 16; p.second = a.second; p.ld2 = a.ld2; p.y = a.y; p.ldy = a.ldy;
+  p.steps = p.code_steps + (2 * p.rank16 + kStep - 1) / kStep;
   const int64_t token_tiles = (int64_t(a.t) + kMaxTokens - 1) / kMaxTokens;
   p.nt = int((int64_t(a.t) + token_tiles - 1) / token_tiles + 15) / 16 * 16;
   p.nt_cols = (p.nt + 31) / 32 * 32;
@@ -645,13 +700,18 @@ template <class T, bool TRANS> int32_t launch(const hyacinHandle_t* handle, cons
               encode_2d(&x_map, dt, x, in, a.t, uint64_t(ldx) * 2, 64, p.nt, CU_TENSOR_MAP_SWIZZLE_128B);
   mid_map = x_map;
   if (fine && a.rank) {
-    const int64_t ldm = (2 * int64_t(a.rank) + 7) / 8 * 8;
+    const int64_t ldm = 2 * int64_t(p.rank16);
     if (!allocate(&mid, size_t(ldm) * a.t * 2)) { cleanup(); return -3; }
-    fine = encode_2d(&mid_map, dt, mid, 2 * uint64_t(a.rank), a.t, uint64_t(ldm) * 2, 64, p.nt, CU_TENSOR_MAP_SWIZZLE_128B);
+    fine = encode_2d(&mid_map, dt, mid, uint64_t(ldm), a.t, uint64_t(ldm) * 2, 64, p.nt, CU_TENSOR_MAP_SWIZZLE_128B);
     const int aligned = reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx % 8 == 0 && reinterpret_cast<uintptr_t>(a.first) % 16 == 0 && a.ld1 % 8 == 0;
+    cudaLaunchConfig_t mc{};
+    mc.gridDim = dim3(unsigned((a.rank + 15) / 16) * kMidSplits, unsigned((int64_t(a.t) + 15) / 16)); mc.blockDim = dim3(kMidWarps * 32); mc.stream = stream;
+    cudaLaunchAttribute ma[1];
+    ma[0].id = cudaLaunchAttributeClusterDimension; ma[0].val.clusterDim.x = kMidSplits; ma[0].val.clusterDim.y = 1; ma[0].val.clusterDim.z = 1;
+    mc.attrs = ma; mc.numAttrs = 1;
     count_launch();
-    mid_split_kernel<T><<<dim3((a.rank + 15) / 16, unsigned((int64_t(a.t) + 15) / 16)), kMidWarps * 32, 0, stream>>>(
-        static_cast<const T*>(a.first), a.ld1, in, a.rank, static_cast<const T*>(x), ldx, a.t, static_cast<T*>(mid), ldm, aligned);
+    const cudaError_t e = cudaLaunchKernelEx(&mc, mid_split_kernel<T>, static_cast<const T*>(a.first), a.ld1, in, a.rank, static_cast<const T*>(x), ldx, a.t, static_cast<T*>(mid), ldm, aligned);
+    if (e != cudaSuccess) { report_cuda_error(e, fn, __FILE__, __LINE__); fine = false; }
   }
   if (!fine) { cleanup(); return -3; }
   auto* kernel = product_umma_kernel<T, TRANS>;
