@@ -384,7 +384,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_stream_kernel(const __gri
 }
 
 // mid(k, t) = sum_r first(r, k) x(r, t): one block per k and up to eight vectors, its threads share the rows, eight at a time where
-// both operands allow it.
+// both operands allow it.  For one vector two warps: the block then fits beside the product's, which starts meanwhile.
 template <class X> __global__ void __launch_bounds__(256) mid_kernel(const X* first, int64_t ld1, int rows, int rank, const X* x, int64_t ldx, int t, float* mid, int aligned) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   __shared__ float red[8][8];
@@ -392,27 +392,39 @@ template <class X> __global__ void __launch_bounds__(256) mid_kernel(const X* fi
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, k = blockIdx.x, t0 = blockIdx.y * 8;
   float s[8] = {};
   const X* f = first + int64_t(k) * ld1;
-  int r0 = 0;
-  if (aligned) {
-    r0 = rows / kWide * kWide;
+  const X* xt = x + int64_t(t0) * ldx;
+  const int r0 = aligned ? rows / kWide * kWide : 0;
+  auto wide = [&](int count) {
+    if (count == 1) {
+#pragma unroll 8
+      for (int r = threadIdx.x * kWide; r < r0; r += int(blockDim.x) * kWide) {
+        const uint4 fw = __ldg(reinterpret_cast<const uint4*>(f + r)), xw = __ldg(reinterpret_cast<const uint4*>(xt + r));
+        const X *fv = reinterpret_cast<const X*>(&fw), *xv = reinterpret_cast<const X*>(&xw);
+#pragma unroll
+        for (int e = 0; e < kWide; ++e) s[0] += to_f32(fv[e]) * to_f32(xv[e]);
+      }
+      return;
+    }
 #pragma unroll 2
-    for (int r = threadIdx.x * kWide; r < r0; r += 256 * kWide) {
-      const uint4 fw = *reinterpret_cast<const uint4*>(f + r);
+    for (int r = threadIdx.x * kWide; r < r0; r += int(blockDim.x) * kWide) {
+      const uint4 fw = __ldg(reinterpret_cast<const uint4*>(f + r));
       const X* fv = reinterpret_cast<const X*>(&fw);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) if (t0 + i < t) {
-        const uint4 xw = *reinterpret_cast<const uint4*>(x + (t0 + i) * ldx + r);
+      for (int i = 0; i < 8; ++i) if (i < count) {
+        const uint4 xw = __ldg(reinterpret_cast<const uint4*>(xt + i * ldx + r));
         const X* xv = reinterpret_cast<const X*>(&xw);
 #pragma unroll
         for (int e = 0; e < kWide; ++e) s[i] += to_f32(fv[e]) * to_f32(xv[e]);
       }
     }
-  }
+  };
+  const int count = min(8, t - t0);
+  wide(count);
 #pragma unroll 4
-  for (int r = r0 + threadIdx.x; r < rows; r += 256) {
+  for (int r = r0 + threadIdx.x; r < rows; r += int(blockDim.x)) {
     const float v = to_f32(f[r]);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) if (t0 + i < t) s[i] += v * to_f32(x[(t0 + i) * ldx + r]);
+    for (int i = 0; i < 8; ++i) if (i < count) s[i] += v * to_f32(xt[i * ldx + r]);
   }
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
@@ -420,9 +432,9 @@ template <class X> __global__ void __launch_bounds__(256) mid_kernel(const X* fi
     if (lane == 0) red[warp][i] = s[i];
   }
   __syncthreads();
-  if (threadIdx.x < 8 && t0 + int(threadIdx.x) < t) {
+  if (int(threadIdx.x) < count) {
     float v = 0.f;
-    for (int w = 0; w < 8; ++w) v += red[w][threadIdx.x];
+    for (int w = 0; w < int(blockDim.x) / 32; ++w) v += red[w][threadIdx.x];
     mid[int64_t(t0 + threadIdx.x) * rank + k] = v;
   }
 }
@@ -510,8 +522,12 @@ int32_t launch_product_stream(const hyacinHandle_t* handle, const char* fn, hyac
       const bool wide = reinterpret_cast<uintptr_t>(p.x) % 16 == 0 && (p.ldx * sizeof(X) % 16 == 0 || p.t == 1);
       p.x_aligned = sizeof(X) == 2 && wide;
       if (a.rank) {
+        // the product's blocks move in beside this kernel's only if the SM is already split between cache and shared memory their way
+        static std::atomic<uint64_t> carved{0};
+        const uint64_t mine = uint64_t(1) << (handle->DeviceID & 63);
+        if (!(carved.load() & mine)) { HYB_CUDA(cudaFuncSetAttribute(mid_kernel<X>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared)); carved.fetch_or(mine); }
         count_launch();
-        mid_kernel<X><<<dim3(a.rank, (p.t + 7) / 8), 256, 0, stream>>>(static_cast<const X*>(a.first), a.ld1, a.m, a.rank, static_cast<const X*>(p.x), a.ldx, p.t, mid + t0 * a.rank,
+        mid_kernel<X><<<dim3(a.rank, (p.t + 7) / 8), p.t == 1 ? 64 : 256, 0, stream>>>(static_cast<const X*>(a.first), a.ld1, a.m, a.rank, static_cast<const X*>(p.x), a.ldx, p.t, mid + t0 * a.rank,
                                                                       wide && reinterpret_cast<uintptr_t>(a.first) % 16 == 0 && a.ld1 * sizeof(X) % 16 == 0);
       }
       const cudaError_t e = p.seg_sub % 4 == 0 ? dispatch<X, 4>(handle, map, p, smem) : p.seg_sub % 2 == 0 ? dispatch<X, 2>(handle, map, p, smem) : dispatch<X, 1>(handle, map, p, smem);

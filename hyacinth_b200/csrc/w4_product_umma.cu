@@ -545,7 +545,7 @@ template <> __device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&d)[4
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-constexpr int kMidWarps = 4, kMidSplits = 8;
+constexpr int kMidWarps = 8, kMidSplits = 8;
 // A cluster of eight blocks: 16 entries of the rank x 16 tokens, the blocks and their warps split the rows, sums joined in shared memory
 // and across the cluster in a fixed order.  A lane feeds eight consecutive rows of each operand row to two instructions: the
 // order of K inside an instruction is free as long as both operands agree.  The product waits for this kernel, so what counts is
@@ -709,6 +709,13 @@ template <class T, bool TRANS> int32_t launch(const hyacinHandle_t* handle, cons
     cudaLaunchAttribute ma[1];
     ma[0].id = cudaLaunchAttributeClusterDimension; ma[0].val.clusterDim.x = kMidSplits; ma[0].val.clusterDim.y = 1; ma[0].val.clusterDim.z = 1;
     mc.attrs = ma; mc.numAttrs = 1;
+    // the product's blocks move in beside this kernel's only if the SM is already split between cache and shared memory their way
+    static std::atomic<uint64_t> carved{0};
+    const uint64_t mine = uint64_t(1) << (handle->DeviceID & 63);
+    if (!(carved.load() & mine)) {
+      HYB_CUDA(cudaFuncSetAttribute(mid_split_kernel<T>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
+      carved.fetch_or(mine);
+    }
     count_launch();
     const cudaError_t e = cudaLaunchKernelEx(&mc, mid_split_kernel<T>, static_cast<const T*>(a.first), a.ld1, in, a.rank, static_cast<const T*>(x), ldx, a.t, static_cast<T*>(mid), ldm, aligned);
     if (e != cudaSuccess) { report_cuda_error(e, fn, __FILE__, __LINE__); fine = false; }
