@@ -42,7 +42,10 @@ __device__ __forceinline__ float ex2(float x) { float r; asm("ex2.approx.ftz.f32
 struct Exponent {
   float scale, c, top;
   __device__ __forceinline__ Exponent(double tau, float t) : scale(float(1.4426950408889634 / tau)), c(t * scale), top(t) {}
-  __device__ double fix() const { return fabsf(c) <= 3.402823466e38f ? exp2(double(c) - double(top) * double(scale)) : 1.; }
+  __device__ double fix() const {
+    const double x = (double(c) - double(top) * double(scale)) * 0.69314718055994530942;
+    return !(fabsf(c) <= 3.402823466e38f) ? 1. : fabs(x) < 1e-4 ? 1. + x * (1. + x * (0.5 + x * (1. / 6.))) : exp(x);
+  }
   __device__ __forceinline__ float operator()(float z) const { return ex2(fmaf(z, scale, -c)); }
 };
 
@@ -62,15 +65,16 @@ struct Max { template <class V> __device__ V operator()(V a, V b) const { return
 // The list of one token in shared memory, `k` entries each.
 struct List {
   double *p, *logp, *psum;   // teacher probability, its logarithm, sum over the entries of the same class
+  double* e;                 // exp(z / tau - top of the list), 0 for entries that are skipped
   float* z;                  // student logit
   int *id, *first;           // class, -1 when skipped; 1 for the first entry of its class
   double* buf; float* fbuf;  // 32 entries each, for reductions
   __device__ List(uint8_t* at, int k) {
-    buf = reinterpret_cast<double*>(at); p = buf + 32; logp = p + k; psum = logp + k;
-    fbuf = reinterpret_cast<float*>(psum + k); z = fbuf + 32; id = reinterpret_cast<int*>(z + k); first = id + k;
+    buf = reinterpret_cast<double*>(at); p = buf + 32; logp = p + k; psum = logp + k; e = psum + k;
+    fbuf = reinterpret_cast<float*>(e + k); z = fbuf + 32; id = reinterpret_cast<int*>(z + k); first = id + k;
   }
 };
-__host__ __device__ constexpr size_t list_bytes(int k) { return 32 * 12 + size_t(k) * 36; }
+__host__ __device__ constexpr size_t list_bytes(int k) { return 32 * 12 + size_t(k) * 44; }
 
 // What is known of the teacher, and of the student's listed classes, before the rest of the row has been seen.
 struct Listed { double rest, mass, top, sum; };      // p_r, sum p + p_r; log-sum-exp of the student's listed classes as top + log(sum), top = -inf without any
@@ -111,44 +115,47 @@ template <class T> __device__ Listed load_list(const DistillArgs& a, int64_t tok
     int first = s.id[i] >= 0; double ps = 0.;
     for (int j = 0; j < a.k; ++j) if (s.id[j] == s.id[i]) { ps += s.p[j]; if (j < i) first = 0; }
     s.first[i] = first; s.psum[i] = ps;
-    if (first && r.top > -INFINITY) e += exp(double(s.z[i]) / a.tau - r.top);
+    s.e[i] = s.id[i] >= 0 && r.top > -INFINITY ? exp(double(s.z[i]) / a.tau - r.top) : 0.;
+    if (first) e += s.e[i];
   }
   r.sum = block_reduce(e, Add{}, s.buf);
   __syncthreads();
   return r;
 }
 
-// The student's normalisers from the listed classes and the sum over the others, outside 2^(top scale).
+// The student's normaliser from the listed classes and the sum over the others, outside 2^(top scale), everything relative to the larger of
+// the two references: total = listed + outside shares.  Logarithms are left to the loss.
 struct Student {
-  double lse, lse_out; bool empty, no_outside;
-  __device__ Student(const DistillArgs& a, const Listed& l, float top, float outside) {
+  double ref, list_share, outside_share, total; bool no_outside;      // exp(l.top - ref), exp(top / tau - ref)
+  __device__ __forceinline__ Student(const DistillArgs& a, const Listed& l, float top, float outside) {
     no_outside = outside == 0.f;
-    lse_out = no_outside ? -INFINITY : log(double(outside)) + double(top) / a.tau;
-    double ref = fmax(l.top, lse_out);
+    const double out = double(top) / a.tau;
+    ref = no_outside ? l.top : fmax(l.top, out);
     if (ref == -INFINITY) ref = 0.;
-    const double total = (l.top > -INFINITY || l.top != l.top ? l.sum * exp(l.top - ref) : 0.) + (no_outside ? 0. : exp(lse_out - ref));
-    empty = total == 0.;
-    lse = ref + log(total);
+    list_share = l.top == -INFINITY ? 0. : exp(l.top - ref);
+    outside_share = no_outside ? 0. : exp(out - ref);
+    total = l.sum * list_share + double(outside) * outside_share;
   }
+  // log q of a listed class, and of everything outside
+  __device__ __forceinline__ double log_q(double u, double log_total) const { return total == 0. ? -INFINITY : u - ref - log_total; }
 };
-// Weighted loss (same in every thread; all threads of the block take part).
-__device__ double distill_loss(const DistillArgs& a, const List& s, const Listed& l, const Student& st, float weight) {
+// This thread's part of the loss over its entries of the list.
+__device__ __forceinline__ double listed_loss(const DistillArgs& a, const List& s, const Student& st, double log_total, int first, int step) {
   double kl = 0.;
-  for (int i = threadIdx.x; i < a.k; i += blockDim.x) if (s.p[i] != 0.) kl += s.p[i] * (s.logp[i] - (st.empty ? -INFINITY : double(s.z[i]) / a.tau - st.lse));
-  kl = block_reduce(kl, Add{}, s.buf);
-  if (l.rest > 0.) kl += l.rest * (log(l.rest) - (st.no_outside ? -INFINITY : st.lse_out - st.lse));
-  return kl * weight;
+  for (int i = first; i < a.k; i += step) if (s.p[i] != 0.) kl += s.p[i] * (s.logp[i] - st.log_q(double(s.z[i]) / a.tau, log_total));
+  return kl;
+}
+__device__ __forceinline__ double outside_loss(const DistillArgs& a, const Listed& l, const Student& st, double log_total, float top, float outside) {
+  return l.rest > 0. ? l.rest * (log(l.rest) - (st.no_outside ? -INFINITY : log(double(outside)) + double(top) / a.tau - st.ref - log_total)) : 0.;
 }
 // dKL/dz = factor * 2^(z scale - top scale) outside the list
 __device__ __forceinline__ double outside_factor(const DistillArgs& a, const Listed& l, const Student& st, float outside, float weight) {
-  return st.no_outside ? 0. : double(weight) / a.tau * (l.mass * exp(st.lse_out - st.lse) - l.rest) / double(outside);
+  return st.no_outside ? 0. : double(weight) / a.tau * (l.mass * st.outside_share / st.total - l.rest / double(outside));
 }
 __device__ __forceinline__ float listed_gradient(const DistillArgs& a, const List& s, const Listed& l, const Student& st, float weight, int i) {
-  return float(double(weight) / a.tau * (l.mass * (st.empty ? 0. : exp(double(s.z[i]) / a.tau - st.lse)) - s.psum[i]));
+  return float(double(weight) / a.tau * ((st.total == 0. ? 0. : l.mass * s.e[i] * st.list_share / st.total) - s.psum[i]));
 }
 
-// Plain form: one block per token, two passes over the logits, a bit per class for the list.
-// Mode: loss from this pass's sums, or gradient from saved ones.
 template <class T> __global__ void __launch_bounds__(512) distill_plain_kernel(DistillArgs a) {
   extern __shared__ __align__(16) uint8_t smem[];
   uint32_t* listed = reinterpret_cast<uint32_t*>(smem + (list_bytes(a.k) + 15) / 16 * 16);
@@ -185,9 +192,10 @@ template <class T> __global__ void __launch_bounds__(512) distill_plain_kernel(D
     }
     const Student st(a, l, top, outside);
     if (a.loss || a.stats_out) {
-      const double loss = distill_loss(a, s, l, st, weight);
+      const double log_total = log(st.total);
+      const double loss = block_reduce(listed_loss(a, s, st, log_total, threadIdx.x, blockDim.x), Add{}, s.buf) + outside_loss(a, l, st, log_total, top, outside);
       if (threadIdx.x == 0) {
-        if (a.loss) a.loss[token] = float(loss);
+        if (a.loss) a.loss[token] = float(loss * weight);
         if (a.stats_out) { a.stats_out[2 * token] = top; a.stats_out[2 * token + 1] = outside; }
       }
     }
@@ -260,11 +268,28 @@ template <> struct RowMax<__nv_bfloat16> {
   __device__ __forceinline__ float value() const { return fmaxf(__low2float(m), __high2float(m)); }
 };
 
-// The teacher's probabilities and the student's listed classes, by one warp; id and z (and the teacher's logits in logp) are there.
-__device__ Listed list_by_warp(const DistillArgs& a, int64_t token, List& s, bool twice) {
+// The list by one warp: first the classes, for the warps that wait to take them out of the row, then the arithmetic.
+template <class T> __device__ __forceinline__ bool list_classes(const DistillArgs& a, int64_t token, List& s, uint32_t* hash) {
+  bool twice = false;                                // some class may be listed twice
+  for (int i = threadIdx.x & 31; i < a.k; i += 32) {
+    const int id = a.ids[token * a.ldk + i];
+    const bool ok = id >= 0 && id < a.n;
+    s.id[i] = ok ? id : -1;
+    if (ok) { const uint32_t bit = 1u << (id & 31); twice |= (atomicOr(&hash[(id >> 5) & (kHashWords - 1)], bit) & bit) != 0; }
+  }
+  return __any_sync(~0u, twice);
+}
+template <class T> __device__ Listed list_by_warp(const DistillArgs& a, int64_t token, const T* z, List& s, bool twice) {
   const int lane = threadIdx.x & 31;
   double top = -INFINITY, student = -INFINITY;
-  for (int i = lane; i < a.k; i += 32) if (s.id[i] >= 0) { top = fmax(top, s.logp[i]); student = fmax(student, double(s.z[i]) / a.tau); }
+#pragma unroll 2
+  for (int i = lane; i < a.k; i += 32) {
+    const int id = s.id[i];
+    const double t = id >= 0 ? double(a.teacher[token * a.ldk + i]) / a.tau : -INFINITY;
+    const float v = id >= 0 ? to_f32(z[id]) : 0.f;
+    s.logp[i] = t; s.z[i] = v;
+    if (id >= 0) { top = fmax(top, t); student = fmax(student, double(v) / a.tau); }
+  }
   double norm;
   if (a.teacher_lse) norm = double(a.teacher_lse[token]);
   else {
@@ -280,16 +305,17 @@ __device__ Listed list_by_warp(const DistillArgs& a, int64_t token, List& s, boo
     const bool ok = s.id[i] >= 0;
     const double l = s.logp[i] - norm, p = ok ? exp(l) : 0.;
     s.logp[i] = l; s.p[i] = s.psum[i] = p; s.first[i] = ok;
+    s.e[i] = ok && r.top > -INFINITY ? exp(double(s.z[i]) / a.tau - r.top) : 0.;
     sum += p;
   }
   __syncwarp();
-  if (twice)                                         // some class may be listed twice
+  if (twice)
     for (int i = lane; i < a.k; i += 32) {
       int first = s.id[i] >= 0; double ps = 0.;
       for (int j = 0; j < a.k; ++j) if (s.id[j] == s.id[i]) { ps += s.p[j]; if (j < i) first = 0; }
       s.first[i] = first; s.psum[i] = ps;
     }
-  for (int i = lane; i < a.k; i += 32) if (s.first[i] && r.top > -INFINITY) e += exp(double(s.z[i]) / a.tau - r.top);
+  for (int i = lane; i < a.k; i += 32) if (s.first[i]) e += s.e[i];
   r.sum = warp_reduce(e, Add{});
   sum = warp_reduce(sum, Add{});
   r.rest = a.teacher_lse ? fmax(0., 1. - sum) : 0.;
@@ -339,34 +365,30 @@ template <class T> __global__ void __launch_bounds__(kClusterThreads, 3) distill
     for (uint32_t at = 0; at < bytes; at += 16384) ptx::bulk_load(ptx::smem_u32(smem) + at, reinterpret_cast<const uint8_t*>(z + head + v0 * V) + at, min(16384u, bytes - at), &bar);
   }
   for (int i = threadIdx.x; i < kHashWords / 4; i += kClusterThreads) reinterpret_cast<uint4*>(hash)[i] = make_uint4(0, 0, 0, 0);
-  __syncthreads();
-  int twice = 0;
-  for (int i = threadIdx.x; i < a.k; i += kClusterThreads) {
-    const int id = a.ids[token * a.ldk + i];
-    const bool ok = id >= 0 && id < a.n;
-    const float t = a.teacher[token * a.ldk + i];
-    s.id[i] = ok ? id : -1; s.logp[i] = ok ? double(t) / a.tau : -INFINITY; s.z[i] = ok ? to_f32(z[id]) : 0.f;
-    if (ok) { const uint32_t bit = 1u << (id & 31); twice |= (atomicOr(&hash[(id >> 5) & (kHashWords - 1)], bit) & bit) != 0; }
-  }
   if (threadIdx.x < 2 * V) {
     const int j = int(threadIdx.x) < V ? int(threadIdx.x) : tail0 + int(threadIdx.x) - V;
     const bool mine = int(threadIdx.x) < V ? first && j < head : last && j < a.n;
     edge[threadIdx.x] = mine ? to_f32(z[j]) : -INFINITY;
   }
-  ptx::mbar_wait(&bar, 0u, &abort_flag, status, 41u);      // expired: the status word says so, the values are then undefined
-  twice = __syncthreads_or(twice);                   // every thread has seen the copy land before an entry is overwritten
-  for (int i = threadIdx.x; i < a.k; i += kClusterThreads) {      // listed classes leave the row (equal values for a class listed twice)
-    const int id = s.id[i];
-    if (id < 0) continue;
-    if (id < head) { if (first) edge[id] = -INFINITY; }
-    else if (id >= tail0) { if (last) edge[V + id - tail0] = -INFINITY; }
-    else { const int v = (id - head) / V; if (v >= v0 && v < v1) reinterpret_cast<T*>(slice)[id - head - v0 * V] = from_f32<T>(-INFINITY); }
-  }
   __syncthreads();
-
   Listed l{};
-  if (warp == 8) l = list_by_warp(a, token, s, twice != 0);
-  else if (!a.stats_in) {
+  if (warp == 8) {
+    const bool twice = list_classes<T>(a, token, s, hash);
+    asm volatile("bar.arrive 2, %0;" ::"n"(kClusterThreads) : "memory");      // the classes are there
+    l = list_by_warp<T>(a, token, z, s, twice);
+  } else {
+    ptx::mbar_wait(&bar, 0u, &abort_flag, status, 41u);      // expired: the status word says so, the values are then undefined
+    asm volatile("bar.sync 2, %0;" ::"n"(kClusterThreads) : "memory");        // every thread has seen the copy land, and the classes
+    for (int i = threadIdx.x; i < a.k; i += kMainThreads) {  // listed classes leave the row (equal values for a class listed twice)
+      const int id = s.id[i];
+      if (id < 0) continue;
+      if (id < head) { if (first) edge[id] = -INFINITY; }
+      else if (id >= tail0) { if (last) edge[V + id - tail0] = -INFINITY; }
+      else { const int v = (id - head) / V; if (v >= v0 && v < v1) reinterpret_cast<T*>(slice)[id - head - v0 * V] = from_f32<T>(-INFINITY); }
+    }
+    main_sync();
+  }
+  if (warp < 8 && !a.stats_in) {
     // maximum and sum of this slice
     RowMax<T> row_max;
     for (int v = threadIdx.x; v < v1 - v0; v += kMainThreads) row_max.add(slice[v]);
@@ -421,10 +443,8 @@ template <class T> __global__ void __launch_bounds__(kClusterThreads, 3) distill
     __syncthreads();
     if (a.splits > 1) cluster_arrive();              // peers may leave once everybody has read
     if (first && (a.loss || a.stats_out)) {
-      double kl = 0.;
-      for (int i = lane; i < a.k; i += 32) if (s.p[i] != 0.) kl += s.p[i] * (s.logp[i] - (st.empty ? -INFINITY : double(s.z[i]) / a.tau - st.lse));
-      kl = warp_reduce(kl, Add{});
-      if (l.rest > 0.) kl += l.rest * (log(l.rest) - (st.no_outside ? -INFINITY : st.lse_out - st.lse));
+      const double log_total = log(st.total);
+      const double kl = warp_reduce(listed_loss(a, s, st, log_total, lane, 32), Add{}) + outside_loss(a, l, st, log_total, top, outside);
       if (lane == 0) {
         if (a.loss) a.loss[token] = float(kl * weight);
         if (a.stats_out) { a.stats_out[2 * token] = top; a.stats_out[2 * token + 1] = outside; }
