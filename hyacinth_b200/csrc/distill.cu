@@ -30,7 +30,7 @@ constexpr int kMaxClasses = 1 << 20;
 
 struct DistillArgs {
   const void* z; int64_t ldz; int n, t, k;
-  const int32_t* ids; const float* teacher; int64_t ldk; double tau;
+  const int32_t* ids; const float* teacher; int64_t ldk; double tau, inv_tau;
   const float* teacher_lse; const float* weight;
   float* loss; float* stats_out; const float* stats_in;
   void* dz; int64_t lddz;
@@ -86,10 +86,10 @@ template <class T> __device__ Listed load_list(const DistillArgs& a, int64_t tok
     const int id = a.ids[token * a.ldk + i];
     const bool ok = id >= 0 && id < a.n;
     s.id[i] = ok ? id : -1;
-    const double t = ok ? double(a.teacher[token * a.ldk + i]) / a.tau : -INFINITY;
+    const double t = ok ? double(a.teacher[token * a.ldk + i]) * a.inv_tau : -INFINITY;
     s.logp[i] = t; s.z[i] = ok ? to_f32(z[id]) : 0.f;
     top = fmax(top, t);
-    if (ok) student = fmax(student, double(s.z[i]) / a.tau);
+    if (ok) student = fmax(student, double(s.z[i]) * a.inv_tau);
   }
   double norm;
   if (a.teacher_lse) norm = double(a.teacher_lse[token]);
@@ -115,7 +115,7 @@ template <class T> __device__ Listed load_list(const DistillArgs& a, int64_t tok
     int first = s.id[i] >= 0; double ps = 0.;
     for (int j = 0; j < a.k; ++j) if (s.id[j] == s.id[i]) { ps += s.p[j]; if (j < i) first = 0; }
     s.first[i] = first; s.psum[i] = ps;
-    s.e[i] = s.id[i] >= 0 && r.top > -INFINITY ? exp(double(s.z[i]) / a.tau - r.top) : 0.;
+    s.e[i] = s.id[i] >= 0 && r.top > -INFINITY ? exp(double(s.z[i]) * a.inv_tau - r.top) : 0.;
     if (first) e += s.e[i];
   }
   r.sum = block_reduce(e, Add{}, s.buf);
@@ -129,7 +129,7 @@ struct Student {
   double ref, list_share, outside_share, total; bool no_outside;      // exp(l.top - ref), exp(top / tau - ref)
   __device__ __forceinline__ Student(const DistillArgs& a, const Listed& l, float top, float outside) {
     no_outside = outside == 0.f;
-    const double out = double(top) / a.tau;
+    const double out = double(top) * a.inv_tau;
     ref = no_outside ? l.top : fmax(l.top, out);
     if (ref == -INFINITY) ref = 0.;
     list_share = l.top == -INFINITY ? 0. : exp(l.top - ref);
@@ -142,18 +142,18 @@ struct Student {
 // This thread's part of the loss over its entries of the list.
 __device__ __forceinline__ double listed_loss(const DistillArgs& a, const List& s, const Student& st, double log_total, int first, int step) {
   double kl = 0.;
-  for (int i = first; i < a.k; i += step) if (s.p[i] != 0.) kl += s.p[i] * (s.logp[i] - st.log_q(double(s.z[i]) / a.tau, log_total));
+  for (int i = first; i < a.k; i += step) if (s.p[i] != 0.) kl += s.p[i] * (s.logp[i] - st.log_q(double(s.z[i]) * a.inv_tau, log_total));
   return kl;
 }
 __device__ __forceinline__ double outside_loss(const DistillArgs& a, const Listed& l, const Student& st, double log_total, float top, float outside) {
-  return l.rest > 0. ? l.rest * (log(l.rest) - (st.no_outside ? -INFINITY : log(double(outside)) + double(top) / a.tau - st.ref - log_total)) : 0.;
+  return l.rest > 0. ? l.rest * (log(l.rest) - (st.no_outside ? -INFINITY : log(double(outside)) + double(top) * a.inv_tau - st.ref - log_total)) : 0.;
 }
 // dKL/dz = factor * 2^(z scale - top scale) outside the list
 __device__ __forceinline__ double outside_factor(const DistillArgs& a, const Listed& l, const Student& st, float outside, float weight) {
-  return st.no_outside ? 0. : double(weight) / a.tau * (l.mass * st.outside_share / st.total - l.rest / double(outside));
+  return st.no_outside ? 0. : double(weight) * a.inv_tau * (l.mass * st.outside_share / st.total - l.rest / double(outside));
 }
 __device__ __forceinline__ float listed_gradient(const DistillArgs& a, const List& s, const Listed& l, const Student& st, float weight, int i) {
-  return float(double(weight) / a.tau * ((st.total == 0. ? 0. : l.mass * s.e[i] * st.list_share / st.total) - s.psum[i]));
+  return float(double(weight) * a.inv_tau * ((st.total == 0. ? 0. : l.mass * s.e[i] * st.list_share / st.total) - s.psum[i]));
 }
 
 template <class T> __global__ void __launch_bounds__(512) distill_plain_kernel(DistillArgs a) {
@@ -269,45 +269,49 @@ template <> struct RowMax<__nv_bfloat16> {
 };
 
 // The list by one warp: first the classes, for the warps that wait to take them out of the row, then the arithmetic.
-template <class T> __device__ __forceinline__ bool list_classes(const DistillArgs& a, int64_t token, List& s, uint32_t* hash) {
+__device__ __forceinline__ bool list_classes(const DistillArgs& a, int64_t token, List& s, uint32_t* hash) {
+  const int lane = threadIdx.x & 31;
+  const int32_t* ids = a.ids + token * a.ldk;
+  int id = lane < a.k ? ids[lane] : -1;
+#pragma unroll
+  for (int i = 0; i < kHashWords / 128; ++i) reinterpret_cast<uint4*>(hash)[i * 32 + lane] = make_uint4(0, 0, 0, 0);
+  __syncwarp();
   bool twice = false;                                // some class may be listed twice
-  for (int i = threadIdx.x & 31; i < a.k; i += 32) {
-    const int id = a.ids[token * a.ldk + i];
+  for (int i = lane; i < a.k; i += 32) {
+    const int next = i + 32 < a.k ? ids[i + 32] : -1;
     const bool ok = id >= 0 && id < a.n;
     s.id[i] = ok ? id : -1;
     if (ok) { const uint32_t bit = 1u << (id & 31); twice |= (atomicOr(&hash[(id >> 5) & (kHashWords - 1)], bit) & bit) != 0; }
+    id = next;
   }
   return __any_sync(~0u, twice);
 }
 template <class T> __device__ Listed list_by_warp(const DistillArgs& a, int64_t token, const T* z, List& s, bool twice) {
   const int lane = threadIdx.x & 31;
-  double top = -INFINITY, student = -INFINITY;
-#pragma unroll 2
+  float top32 = -INFINITY, student32 = -INFINITY;
+#pragma unroll 4
   for (int i = lane; i < a.k; i += 32) {
     const int id = s.id[i];
-    const double t = id >= 0 ? double(a.teacher[token * a.ldk + i]) / a.tau : -INFINITY;
-    const float v = id >= 0 ? to_f32(z[id]) : 0.f;
-    s.logp[i] = t; s.z[i] = v;
-    if (id >= 0) { top = fmax(top, t); student = fmax(student, double(v) / a.tau); }
+    const float t = id >= 0 ? a.teacher[token * a.ldk + i] : -INFINITY, v = id >= 0 ? to_f32(z[id]) : -INFINITY;
+    s.logp[i] = double(t) * a.inv_tau; s.z[i] = v;
+    top32 = fmaxf(top32, t); student32 = fmaxf(student32, v);
   }
-  double norm;
-  if (a.teacher_lse) norm = double(a.teacher_lse[token]);
-  else {
-    top = warp_reduce(top, Max{});
-    double e = 0.;
-    for (int i = lane; i < a.k; i += 32) if (s.id[i] >= 0) e += exp(s.logp[i] - top);
-    norm = top + log(warp_reduce(e, Add{}));
-  }
+  top32 = warp_reduce(top32, Max{}); student32 = warp_reduce(student32, Max{});
   Listed r;
-  r.top = warp_reduce(student, Max{});
-  double sum = 0., e = 0.;
+  r.top = double(student32) * a.inv_tau;
+  // with the teacher's log-sum-exp p = exp(t - lse), without it the exponentials over their sum
+  const double norm = a.teacher_lse ? double(a.teacher_lse[token]) : top32 == -INFINITY ? 0. : double(top32) * a.inv_tau;
+  double sum = 0.;
   for (int i = lane; i < a.k; i += 32) {
     const bool ok = s.id[i] >= 0;
     const double l = s.logp[i] - norm, p = ok ? exp(l) : 0.;
-    s.logp[i] = l; s.p[i] = s.psum[i] = p; s.first[i] = ok;
-    s.e[i] = ok && r.top > -INFINITY ? exp(double(s.z[i]) / a.tau - r.top) : 0.;
+    s.logp[i] = l; s.p[i] = p; s.first[i] = ok;
+    s.e[i] = ok && student32 != -INFINITY ? exp(double(s.z[i]) * a.inv_tau - r.top) : 0.;
     sum += p;
   }
+  sum = warp_reduce(sum, Add{});
+  const double share = a.teacher_lse ? 1. : 1. / sum, log_sum = a.teacher_lse ? 0. : log(sum);
+  for (int i = lane; i < a.k; i += 32) { s.p[i] = s.psum[i] = s.id[i] >= 0 ? s.p[i] * share : 0.; s.logp[i] -= log_sum; }
   __syncwarp();
   if (twice)
     for (int i = lane; i < a.k; i += 32) {
@@ -315,11 +319,11 @@ template <class T> __device__ Listed list_by_warp(const DistillArgs& a, int64_t 
       for (int j = 0; j < a.k; ++j) if (s.id[j] == s.id[i]) { ps += s.p[j]; if (j < i) first = 0; }
       s.first[i] = first; s.psum[i] = ps;
     }
+  double e = 0.;
   for (int i = lane; i < a.k; i += 32) if (s.first[i]) e += s.e[i];
   r.sum = warp_reduce(e, Add{});
-  sum = warp_reduce(sum, Add{});
-  r.rest = a.teacher_lse ? fmax(0., 1. - sum) : 0.;
-  r.mass = sum + r.rest;
+  if (a.teacher_lse) { r.rest = fmax(0., 1. - sum); r.mass = sum + r.rest; }
+  else { r.rest = 0.; r.mass = sum > 0. ? 1. : sum == 0. ? 0. : sum; }
   return r;
 }
 
@@ -364,19 +368,18 @@ template <class T> __global__ void __launch_bounds__(kClusterThreads, 3) distill
     ptx::mbar_expect_tx(&bar, bytes);
     for (uint32_t at = 0; at < bytes; at += 16384) ptx::bulk_load(ptx::smem_u32(smem) + at, reinterpret_cast<const uint8_t*>(z + head + v0 * V) + at, min(16384u, bytes - at), &bar);
   }
-  for (int i = threadIdx.x; i < kHashWords / 4; i += kClusterThreads) reinterpret_cast<uint4*>(hash)[i] = make_uint4(0, 0, 0, 0);
-  if (threadIdx.x < 2 * V) {
-    const int j = int(threadIdx.x) < V ? int(threadIdx.x) : tail0 + int(threadIdx.x) - V;
-    const bool mine = int(threadIdx.x) < V ? first && j < head : last && j < a.n;
-    edge[threadIdx.x] = mine ? to_f32(z[j]) : -INFINITY;
-  }
-  __syncthreads();
   Listed l{};
   if (warp == 8) {
-    const bool twice = list_classes<T>(a, token, s, hash);
+    const bool twice = list_classes(a, token, s, hash);
     asm volatile("bar.arrive 2, %0;" ::"n"(kClusterThreads) : "memory");      // the classes are there
     l = list_by_warp<T>(a, token, z, s, twice);
   } else {
+    if (threadIdx.x < 2 * V) {
+      const int j = int(threadIdx.x) < V ? int(threadIdx.x) : tail0 + int(threadIdx.x) - V;
+      const bool mine = int(threadIdx.x) < V ? first && j < head : last && j < a.n;
+      edge[threadIdx.x] = mine ? to_f32(z[j]) : -INFINITY;
+    }
+    main_sync();
     ptx::mbar_wait(&bar, 0u, &abort_flag, status, 41u);      // expired: the status word says so, the values are then undefined
     asm volatile("bar.sync 2, %0;" ::"n"(kClusterThreads) : "memory");        // every thread has seen the copy land, and the classes
     for (int i = threadIdx.x; i < a.k; i += kMainThreads) {  // listed classes leave the row (equal values for a class listed twice)
@@ -433,7 +436,7 @@ template <class T> __global__ void __launch_bounds__(kClusterThreads, 3) distill
       const float ps = lane >= a.splits ? 0.f : a.splits > 1 ? ld_cluster(&part[1], lane) : part[1];
       top = warp_reduce(pm, Max{});
       if (top == -INFINITY) top = 0.f;
-      const double scale = double(float(1.4426950408889634 / a.tau));
+      const double scale = double(float(1.4426950408889634 * a.inv_tau));
       const double share = pm == -INFINITY ? 0. : pm == top ? double(ps) : double(ps) * exp2((double(pm) - double(top)) * scale);
       outside = float(warp_reduce(share, Add{}));
     }
@@ -555,7 +558,7 @@ extern "C" int32_t hyacinB200DistillLoss(const hyacinHandle_t* handle, hyacinPre
                                          const float* teacherLse, const float* weight, float* loss, float* stats, void* dZ, int32_t lddz) {
   using namespace hyb;
   const char* fn = "hyacinB200DistillLoss";
-  DistillArgs a{Z, ldz, N, T, K, ids, teacher, ldk, tau, teacherLse, weight, loss, stats, nullptr, dZ, lddz, 1, 0};
+  DistillArgs a{Z, ldz, N, T, K, ids, teacher, ldk, tau, 1. / tau, teacherLse, weight, loss, stats, nullptr, dZ, lddz, 1, 0};
   const int32_t rc = check_distill(fn, handle, Ztype, a);
   if (rc) return rc < 0 ? rc : 0;
   if (!loss && !stats && !dZ) return 0;
@@ -568,7 +571,7 @@ extern "C" int32_t hyacinB200DistillGrad(const hyacinHandle_t* handle, hyacinPre
                                          const float* teacherLse, const float* weight, const float* stats, void* dZ, int32_t lddz) {
   using namespace hyb;
   const char* fn = "hyacinB200DistillGrad";
-  DistillArgs a{Z, ldz, N, T, K, ids, teacher, ldk, tau, teacherLse, weight, nullptr, nullptr, stats, dZ, lddz, 1, 0};
+  DistillArgs a{Z, ldz, N, T, K, ids, teacher, ldk, tau, 1. / tau, teacherLse, weight, nullptr, nullptr, stats, dZ, lddz, 1, 0};
   const int32_t rc = check_distill(fn, handle, Ztype, a);
   if (rc) return rc < 0 ? rc : 0;
   if (!stats || !dZ) return w4_refuse(fn, "null pointer");
