@@ -56,23 +56,68 @@ template <class T> __global__ void __launch_bounds__(256) product_t_plain_kernel
   }
 }
 
-// op 'N', plain: one thread per row of a block of 128, running over the columns.
-template <class T> __global__ void __launch_bounds__(kW4Block) product_n_plain_kernel(PlainArgs a) {
-  const int row = blockIdx.x * kW4Block + threadIdx.x;
-  if (row >= a.m) return;
-  const int in = threadIdx.x, word = 4 * ((in & 31) >> 3) + (in >> 5), shift = 4 * w4_row_nibble(in & 7), seg = row / a.seg;
-  const uint8_t* codes = a.codes + int64_t(blockIdx.x) * 64 + word * 4;
+// op 'N' in single precision (and for 16-bit types when there is nothing to sum): a block of 256 threads takes 128 rows, thread (word,
+// lane) the eight rows of a word in every 16th column, for four vectors at a time; x times the scale is formed once per word.
+// A cluster of up to eight such blocks splits the columns; sums meet in shared memory, in a fixed order.
+// Bound: the floating-point pipe, 8 conversions and 32 multiply-adds per word and four vectors.
+constexpr int kSingleLanes = 16, kSingleThreads = 16 * kSingleLanes;
+__device__ __forceinline__ float ld_cluster(const float* at, uint32_t rank) {
+  uint32_t remote; float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(uint32_t(__cvta_generic_to_shared(at))), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote) : "memory");
+  return v;
+}
+__device__ __forceinline__ void cluster_sync_all() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+template <class T> __global__ void __launch_bounds__(kSingleThreads) product_n_single_kernel(PlainArgs a, int splits) {
+  __shared__ float red[kPlainTokens][8][16][kSingleLanes + 1], sum[kPlainTokens][kW4Block];
+  const int word = threadIdx.x & 15, lane = threadIdx.x >> 4, split = blockIdx.x % splits, block = blockIdx.x / splits;
+  const int row = block * kW4Block + w4_word_row(word), seg = min(row, a.m - 1) / a.seg;
+  const int j0 = int(int64_t(a.n) * split / splits), j1 = int(int64_t(a.n) * (split + 1) / splits);
   const T* x = static_cast<const T*>(a.x);
   const T* scales = static_cast<const T*>(a.scales) + seg;
+  const uint8_t* zeros = a.zeros ? a.zeros + seg : nullptr;
+  const uint8_t* codes = a.codes + int64_t(block) * 64 + word * 4;
   for (int64_t t0 = int64_t(blockIdx.y) * kPlainTokens; t0 < a.t; t0 += int64_t(gridDim.y) * kPlainTokens) {
-    float acc[kPlainTokens] = {};
-    for (int j = 0; j < a.n; ++j) {
-      const uint32_t q = (*reinterpret_cast<const uint32_t*>(codes + j * a.ldq) >> shift) & 15u;
-      const float v = to_f32(scales[j * a.lds]) * float(int(q) - (a.zeros ? int(a.zeros[j * a.lds + seg]) : 8));
-      for (int t = 0; t < kPlainTokens; ++t) if (t0 + t < a.t) acc[t] += v * to_f32(x[(t0 + t) * a.ldx + j]);
+    float acc[kPlainTokens][8] = {};
+#pragma unroll 4
+    for (int j = j0 + lane; j < j1; j += kSingleLanes) {
+      const uint32_t q = __ldg(reinterpret_cast<const uint32_t*>(codes + j * a.ldq));
+      const float s = to_f32(scales[j * a.lds]), offset = 8388608.f + float(zeros ? int(zeros[j * a.lds]) : 8);
+      float xs[kPlainTokens], w[8];
+#pragma unroll
+      for (int t = 0; t < kPlainTokens; ++t) xs[t] = t0 + t < a.t ? s * to_f32(x[(t0 + t) * a.ldx + j]) : 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w[e] = __uint_as_float(((q >> (4 * w4_row_nibble(e))) & 15u) | 0x4b000000u) - offset;      // 2^23 + q, exact
+#pragma unroll
+      for (int t = 0; t < kPlainTokens; ++t)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc[t][e] += w[e] * xs[t];
     }
+#pragma unroll
     for (int t = 0; t < kPlainTokens; ++t)
-      if (t0 + t < a.t) static_cast<T*>(a.y)[(t0 + t) * a.ldy + row] = from_f32<T>(add_correction<T>(a, acc[t], row, int(t0 + t)));
+#pragma unroll
+      for (int e = 0; e < 8; ++e) red[t][e][word][lane] = acc[t][e];
+    __syncthreads();
+    for (int i = threadIdx.x; i < kPlainTokens * kW4Block; i += kSingleThreads) {
+      const int t = i / kW4Block, r = i % kW4Block, e = r & 7, w = r >> 3;
+      float v = 0.f;
+#pragma unroll
+      for (int l = 0; l < kSingleLanes; ++l) v += red[t][e][w][l];
+      sum[t][w4_word_row(w) + e] = v;
+    }
+    if (splits > 1) cluster_sync_all(); else __syncthreads();
+    const int share = kW4Block / splits;
+    for (int i = threadIdx.x; i < kPlainTokens * share; i += kSingleThreads) {
+      const int t = i / share, local = split * share + i % share, out = block * kW4Block + local;
+      if (out >= a.m || t0 + t >= a.t) continue;
+      float v = 0.f;
+      for (int c = 0; c < splits; ++c) v += splits > 1 ? ld_cluster(&sum[t][local], c) : sum[t][local];
+      static_cast<T*>(a.y)[(t0 + t) * a.ldy + out] = from_f32<T>(add_correction<T>(a, v, out, int(t0 + t)));
+    }
+    if (splits > 1) cluster_sync_all(); else __syncthreads();
   }
 }
 
@@ -130,7 +175,18 @@ extern "C" int32_t hyacinB200ProductW4(const hyacinHandle_t* handle, char opW, i
     const unsigned ty = unsigned(min((T + kPlainTokens - 1) / kPlainTokens, 65535));
     count_launch();
     if (trans) product_t_plain_kernel<E><<<dim3((N + 7) / 8, ty), 256, 0, stream>>>(a);
-    else product_n_plain_kernel<E><<<dim3((M + kW4Block - 1) / kW4Block, ty), kW4Block, 0, stream>>>(a);
+    else {
+      const int blocks = (M + kW4Block - 1) / kW4Block;
+      int splits = 1;
+      while (splits < 8 && int64_t(blocks) * ty * splits < 4 * int64_t(handle->DeviceSMs) && splits * 2 * kSingleLanes <= N) splits *= 2;
+      cudaLaunchConfig_t cfg{};
+      cfg.gridDim = dim3(unsigned(blocks) * splits, ty); cfg.blockDim = dim3(kSingleThreads); cfg.stream = stream;
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension; attr[0].val.clusterDim.x = splits; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+      cfg.attrs = attr; cfg.numAttrs = splits > 1 ? 1 : 0;
+      const cudaError_t e = cudaLaunchKernelEx(&cfg, product_n_single_kernel<E>, a, splits);
+      if (e != cudaSuccess) { report_cuda_error(e, fn, __FILE__, __LINE__); rc = -3; return; }
+    }
     rc = w4_launched(fn);
   });
   if (mid) HYB_CUDA(cudaFreeAsync(mid, stream));

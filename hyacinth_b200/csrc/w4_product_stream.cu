@@ -45,7 +45,7 @@ struct StreamParams {
   int rank; const void* second; int64_t ld2; const float* mid;
   void* y; int64_t ldy;
   int segs, seg_sub, seg_shift;                   // 32-row subsets per segment, its logarithm or -1
-  int blocks, cols, ring, pitch, x_aligned;       // pitch: of x in shared memory, elements
+  int blocks, cols, tiles, ring, pitch, x_aligned;       // pitch: of x in shared memory, elements
   int sums_at, ring_at, pairs_at, red_at, bars_at;
   uint32_t* status;
 };
@@ -458,28 +458,34 @@ template <class X, int TILES, int GRAIN> cudaError_t start(const hyacinHandle_t*
 }
 
 template <class X, int GRAIN> cudaError_t dispatch(const hyacinHandle_t* handle, const CUtensorMap& map, const StreamParams& p, int smem) {
-  return p.cols <= 8 ? start<X, 1, GRAIN>(handle, map, p, smem) : start<X, 2, GRAIN>(handle, map, p, smem);
+  return p.tiles == 1 ? start<X, 1, GRAIN>(handle, map, p, smem) : start<X, 2, GRAIN>(handle, map, p, smem);
 }
 
 constexpr int kMaxColumns = 16;
 int parts(hyacinPrecision_t type) { return type == HYACIN_F32 ? 3 : 1; }
 
-// Geometry for `vectors` vectors; returns the shared memory, or 0 when they do not fit beside a ring of four stages.
-int place(StreamParams& p, hyacinPrecision_t type, const ProductArgs& a, int vectors) {
-  p.t = vectors; p.cols = vectors * parts(type); p.rank = a.rank; p.m = a.m; p.n = a.n;
-  p.segs = (a.m + a.seg - 1) / a.seg; p.seg_sub = a.seg / 32; p.seg_shift = -1;
-  for (int s = 0; s < 27; ++s) if (p.seg_sub == 1 << s) p.seg_shift = s;
-  p.blocks = (a.m + kW4Block - 1) / kW4Block;
-  const int per_block = p.seg_sub % 4 == 0 ? 1 : p.seg_sub % 2 == 0 ? 2 : 4;
-  const int64_t tiles = p.cols > 8 ? 2 : 1, stage_blocks = kWarps * blocks_per_warp(int(tiles)), pitch = int64_t(p.blocks) * kW4Block + 32;      // 64 bytes over a multiple of 256: lanes g, g + 1 in different halves of the banks
+// Shared memory of the form with `tiles` eights of operand columns, 0 when it leaves no ring of four stages.
+int layout(StreamParams& p, hyacinPrecision_t type, int tiles) {
+  const int per_block = p.seg_sub % 4 == 0 ? 1 : p.seg_sub % 2 == 0 ? 2 : 4, stage_blocks = kWarps * blocks_per_warp(tiles);
+  const int64_t pitch = int64_t(p.blocks) * kW4Block + 32;          // 64 bytes over a multiple of 256: lanes g, g + 1 in different halves of the banks
   const int64_t x_bytes = (p.cols * pitch * 2 + 127) / 128 * 128, sums = type == HYACIN_F32 ? 0 : (int64_t(p.blocks) * per_block * 8 * tiles * 4 + 127) / 128 * 128;
   const int64_t red = kJoints * kWarps * kTile * (8 * tiles + 1) * 4, pair_stage = int64_t(kTile) * (per_block * stage_blocks + 1) * (type == HYACIN_F32 ? 8 : 4);
   const int64_t fixed = x_bytes + sums + red + int64_t(sizeof(StreamBars)), stage_codes = kTile * stage_blocks * 64, stage = stage_codes + pair_stage;
   const int64_t ring = std::min<int64_t>(kMaxRing, (kSmemLimit - fixed) / stage);
   if (fixed > kSmemLimit || ring < 4) return 0;
-  p.ring = int(ring); p.pitch = int(pitch); p.sums_at = int(x_bytes); p.ring_at = int(x_bytes + sums); p.pairs_at = int(p.ring_at + ring * stage_codes);
-  p.red_at = int(p.pairs_at + ring * pair_stage); p.bars_at = int(p.red_at + red);
+  p.tiles = tiles; p.ring = int(ring); p.pitch = int(pitch); p.sums_at = int(x_bytes); p.ring_at = int(x_bytes + sums);
+  p.pairs_at = int(p.ring_at + ring * stage_codes); p.red_at = int(p.pairs_at + ring * pair_stage); p.bars_at = int(p.red_at + red);
   return int(fixed + ring * stage);
+}
+// Geometry for `vectors` vectors; returns the shared memory, or 0 when they do not fit.  A long x may need the form with smaller stages.
+int place(StreamParams& p, hyacinPrecision_t type, const ProductArgs& a, int vectors) {
+  p.t = vectors; p.cols = vectors * parts(type); p.rank = a.rank; p.m = a.m; p.n = a.n;
+  p.segs = (a.m + a.seg - 1) / a.seg; p.seg_sub = a.seg / 32; p.seg_shift = -1;
+  for (int s = 0; s < 27; ++s) if (p.seg_sub == 1 << s) p.seg_shift = s;
+  p.blocks = (a.m + kW4Block - 1) / kW4Block;
+  int bytes = p.cols <= 8 ? layout(p, type, 1) : 0;
+  if (!bytes) bytes = layout(p, type, 2);
+  return bytes;
 }
 
 }  // namespace
@@ -509,7 +515,7 @@ int32_t launch_product_stream(const hyacinHandle_t* handle, const char* fn, hyac
       EncodeTiledFn encode = encode_tiled();
       CUtensorMap map{};
       const cuuint64_t dims[2] = {cuuint64_t(p.blocks) * 8, cuuint64_t(a.n)}, strides[1] = {cuuint64_t(a.ldq)};
-      const cuuint32_t box[2] = {cuuint32_t(kWarps * blocks_per_warp(p.cols > 8 ? 2 : 1) * 8), kTile}, elem[2] = {1, 1};
+      const cuuint32_t box[2] = {cuuint32_t(kWarps * blocks_per_warp(p.tiles) * 8), kTile}, elem[2] = {1, 1};
       if (!encode || encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT64, 2, const_cast<uint8_t*>(a.codes), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
                             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS) {
         std::fprintf(stderr, "hyacin-b200: %s: cuTensorMapEncodeTiled failed\n", fn);

@@ -153,6 +153,14 @@ PCASES = [  # op, m, n, t, seg, kind, zeros, rank, pads (scales, X/U, Y/V)
     ("N", 1000, 513, 16, 32, "bf16", True, 0, (0, 5, 3)), ("N", 512, 2048, 64, 64, "f16", True, 32, (0, 0, 0)), ("N", 640, 777, 65, 128, "bf16", False, 0, (0, 7, 0)),
     ("N", 384, 520, 256, 96, "bf16", True, 8, (0, 0, 0)), ("N", 200, 300, 280, 256, "f16", False, 0, (0, 4, 8)), ("N", 257, 400, 1, 32, "f32", True, 0, (0, 0, 0)),
     ("N", 1024, 350, 7, 128, "f32", False, 5, (1, 1, 1)),
+    # long x: the streaming kernel's smaller stages, the tensor-core kernel, and what neither takes
+    ("T", 16384, 40, 1, 128, "f32", False, 0, (0, 0, 0)), ("T", 30001, 24, 2, 64, "f32", True, 3, (0, 0, 0)), ("T", 16390, 40, 8, 32, "bf16", True, 0, (1, 0, 0)),
+    ("T", 20000, 20, 4, 128, "f16", False, 17, (0, 0, 0)), ("T", 16384, 33, 1, 96, "bf16", True, 0, (0, 0, 0)), ("T", 2600, 150, 13, 32, "f16", True, 6, (1, 1, 0)),
+    # every shape of the correction: ranks of 16, 32, 64 and others, one and two parts per step
+    ("T", 512, 200, 40, 128, "bf16", False, 16, (0, 0, 0)), ("T", 512, 200, 40, 128, "f16", False, 33, (0, 0, 0)), ("T", 512, 200, 129, 128, "bf16", False, 64, (0, 0, 0)),
+    ("T", 512, 200, 250, 64, "bf16", True, 70, (0, 1, 1)), ("T", 512, 200, 40, 128, "bf16", False, 150, (0, 0, 0)), ("N", 300, 512, 40, 32, "bf16", False, 90, (0, 0, 0)),
+    ("N", 300, 512, 200, 64, "f16", True, 16, (0, 2, 2)), ("N", 5000, 700, 5, 64, "f32", True, 3, (0, 0, 0)), ("N", 200, 16, 1, 64, "f32", False, 0, (0, 0, 0)),
+    ("N", 128, 20000, 33, 128, "f32", False, 2, (0, 0, 0)), ("T", 384, 19000, 20, 128, "f16", False, 0, (0, 0, 0)), ("N", 19000, 200, 20, 128, "f16", False, 0, (0, 0, 0)),
 ]
 
 
