@@ -16,6 +16,8 @@ struct ProductArgs {
 // Fifth-generation tensor cores, 16-bit types, both directions.  Returns 0 or -3.
 int32_t launch_product_umma(const hyacinHandle_t* handle, const char* fn, bool trans, hyacinPrecision_t type, const ProductArgs& a);
 
+// mid(k, t) = sum_r first(r, k) x(r, t) in single precision, [t][k], for the 16-bit types.
+cudaError_t launch_mid_float(const hyacinHandle_t* handle, hyacinPrecision_t type, const void* first, int64_t ld1, int rows, int rank, const void* x, int64_t ldx, int t, float* mid, bool aligned);
 // Few vectors, opW 'T', all types, any number of passes over W; product_stream_vectors: vectors per pass (0: not even one fits).
 int product_stream_vectors(hyacinPrecision_t type, const ProductArgs& a);
 int32_t launch_product_stream(const hyacinHandle_t* handle, const char* fn, hyacinPrecision_t type, const ProductArgs& a);

@@ -528,13 +528,18 @@ int32_t launch_product_stream(const hyacinHandle_t* handle, const char* fn, hyac
       const bool wide = reinterpret_cast<uintptr_t>(p.x) % 16 == 0 && (p.ldx * sizeof(X) % 16 == 0 || p.t == 1);
       p.x_aligned = sizeof(X) == 2 && wide;
       if (a.rank) {
-        // the product's blocks move in beside this kernel's only if the SM is already split between cache and shared memory their way
-        static std::atomic<uint64_t> carved{0};
-        const uint64_t mine = uint64_t(1) << (handle->DeviceID & 63);
-        if (!(carved.load() & mine)) { HYB_CUDA(cudaFuncSetAttribute(mid_kernel<X>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared)); carved.fetch_or(mine); }
-        count_launch();
-        mid_kernel<X><<<dim3(a.rank, (p.t + 7) / 8), p.t == 1 ? 64 : 256, 0, stream>>>(static_cast<const X*>(a.first), a.ld1, a.m, a.rank, static_cast<const X*>(p.x), a.ldx, p.t, mid + t0 * a.rank,
-                                                                      wide && reinterpret_cast<uintptr_t>(a.first) % 16 == 0 && a.ld1 * sizeof(X) % 16 == 0);
+        const bool both = wide && reinterpret_cast<uintptr_t>(a.first) % 16 == 0 && a.ld1 * sizeof(X) % 16 == 0;
+        if (sizeof(X) == 2 && (p.t > 2 || !both)) {                  // a cluster per 16 x 16 entries
+          const cudaError_t e = launch_mid_float(handle, type, a.first, a.ld1, a.m, a.rank, p.x, a.ldx, p.t, mid + t0 * a.rank, both);
+          if (e != cudaSuccess) { report_cuda_error(e, fn, __FILE__, __LINE__); rc = -3; return; }
+        } else {
+          // the product's blocks move in beside this kernel's only if the SM is already split between cache and shared memory their way
+          static std::atomic<uint64_t> carved{0};
+          const uint64_t mine = uint64_t(1) << (handle->DeviceID & 63);
+          if (!(carved.load() & mine)) { HYB_CUDA(cudaFuncSetAttribute(mid_kernel<X>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared)); carved.fetch_or(mine); }
+          count_launch();
+          mid_kernel<X><<<dim3(a.rank, (p.t + 7) / 8), p.t == 1 ? 64 : 256, 0, stream>>>(static_cast<const X*>(a.first), a.ld1, a.m, a.rank, static_cast<const X*>(p.x), a.ldx, p.t, mid + t0 * a.rank, both);
+        }
       }
       const cudaError_t e = p.seg_sub % 4 == 0 ? dispatch<X, 4>(handle, map, p, smem) : p.seg_sub % 2 == 0 ? dispatch<X, 2>(handle, map, p, smem) : dispatch<X, 1>(handle, map, p, smem);
       if (e != cudaSuccess) { report_cuda_error(e, fn, __FILE__, __LINE__); rc = -3; }

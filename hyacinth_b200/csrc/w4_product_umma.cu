@@ -37,8 +37,8 @@ constexpr int kThreads = 32 * (2 + kLoaders + kGroups * kGroupWarps);
 // More than half of the shared memory, always: one CTA per SM, so tensor memory is not contended for, which clusters whose CTAs
 // wait for one another could not afford.
 constexpr uint32_t kSmemLimit = 232448, kSmemFloor = 120 * 1024;
-template <bool TRANS> struct Geometry {
-  static constexpr int step = TRANS ? 128 : 64;                          // K per step
+template <bool TRANS, int STEP> struct Geometry {
+  static constexpr int step = STEP;                                      // K per step: 128; 64 for 'N' with more than 128 tokens, whose tiles leave less room
   static constexpr int cols = TRANS ? kOut : step;                       // columns of W per step
   static constexpr uint32_t code_bytes = cols * 64;
   static constexpr uint32_t scale_bytes = cols * 12;                     // four 16-bit scales and four zero points per column
@@ -187,15 +187,16 @@ template <> struct Scale<__nv_bfloat16> {
   }
 };
 
-template <class T, bool TRANS>
+template <class T, bool TRANS, int STEP>
 __global__ void __launch_bounds__(kThreads, 1)
 product_umma_kernel(const __grid_constant__ CUtensorMap code_map, const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap mid_map,
                     const __grid_constant__ UmmaParams p) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* aligned = smem_raw + (base - smem_u32(smem_raw));
-  using G = Geometry<TRANS>;
+  using G = Geometry<TRANS, STEP>;
   constexpr int kStep = G::step;
+  constexpr bool kFull = STEP == 128;
   const uint32_t x_bytes = uint32_t(p.nt) * kStep * 2;
   const uint32_t operand = base + p.ring * G::code_bytes, x_ring = operand + p.bufs * G::operand_bytes, scale_ring = x_ring + p.ring * x_bytes;
   UmmaBars* bars = reinterpret_cast<UmmaBars*>(aligned + (scale_ring - base) + p.ring * G::scale_bytes);
@@ -214,12 +215,12 @@ product_umma_kernel(const __grid_constant__ CUtensorMap code_map, const __grid_c
       if (TRANS) tma_load_2d(base + stage * G::code_bytes, &code_map, bar, k * 64, tile * kOut);
       else tma_load_2d(base + stage * G::code_bytes, &code_map, bar, tile * 64, k * kStep);
       tma_load_2d(sx, &x_map, bar, k * kStep, t0);
-      if (TRANS) tma_load_2d(sx + x_bytes / 2, &x_map, bar, k * kStep + 64, t0);
+      if (kFull) tma_load_2d(sx + x_bytes / 2, &x_map, bar, k * kStep + 64, t0);
     } else {
       mbar_expect_tx(bar, x_bytes);
       const int c = (k - p.code_steps) * kStep;
       tma_load_2d(sx, &mid_map, bar, c, t0);
-      if (TRANS) tma_load_2d(sx + x_bytes / 2, &mid_map, bar, c + 64, t0);
+      if (kFull) tma_load_2d(sx + x_bytes / 2, &mid_map, bar, c + 64, t0);
     }
   };
   if (threadIdx.x == 0) {
@@ -370,7 +371,7 @@ product_umma_kernel(const __grid_constant__ CUtensorMap code_map, const __grid_c
   } else {
     const int id = threadIdx.x - 32 * (2 + kLoaders), group = id >> 7;
     // column of W within the step; for 'T' that is the output, which has to be this thread's lane of tensor memory
-    const int row = TRANS ? 32 * (warp & 3) + lane : id & 63, half = (id >> 6) & 1;
+    const int row = TRANS ? 32 * (warp & 3) + lane : kFull ? id & 127 : id & 63, half = kFull ? 0 : (id >> 6) & 1;
     const uint32_t swz = (row & 7) << 4;
     // An operand buffer is free when the step before on it, k - bufs, was multiplied: the barrier that also frees that step's ring
     // stage.  A group waits for its own steps only and a barrier cannot overtake it: step k + ring is not loaded, and step
@@ -398,29 +399,36 @@ product_umma_kernel(const __grid_constant__ CUtensorMap code_map, const __grid_c
       if (TRANS) tc_fence_after();
       if (k < p.code_steps) {
         const uint32_t at = scale_ring + stage * G::scale_bytes, codes = base + stage * G::code_bytes + row * 64, chunk = (row >> 1) & 3;
-        constexpr int kQuarters = TRANS ? 4 : 2;
+        constexpr int kQuarters = kFull ? 4 : 2;
         uint32_t s[2], z; uint4 q[kQuarters];
         asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(s[0]), "=r"(s[1]) : "r"(at + row * 8));
         asm volatile("ld.shared.u32 %0, [%1];" : "=r"(z) : "r"(at + G::cols * 8 + row * 4));
 #pragma unroll
-        for (int c = 0; c < kQuarters; ++c) q[c] = lds128(codes + (((TRANS ? c : 2 * half + c) ^ chunk) << 4));
+        for (int c = 0; c < kQuarters; ++c) q[c] = lds128(codes + (((2 * half + c) ^ chunk) << 4));
 #pragma unroll
         for (int pair = 0; pair < 2; ++pair) {
-          uint32_t o[2][kQuarters][4];
+          typename Scale<T>::Ready r[2];
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             Scale<T> sc; sc.bits = uint16_t(s[pair] >> (16 * i)); sc.zero = (z >> (16 * pair + 8 * i)) & 0xff;
-            const typename Scale<T>::Ready r = sc.ready();
-#pragma unroll
-            for (int c = 0; c < kQuarters; ++c) Scale<T>::word(pair == 0 ? (i == 0 ? q[c].x : q[c].y) : (i == 0 ? q[c].z : q[c].w), r, o[i][c]);
+            r[i] = sc.ready();
           }
-          if constexpr (TRANS) tmem_st32(tdst + pair * 32, reinterpret_cast<const uint32_t (&)[32]>(o));
-          else {
+          auto word = [&](int i, int c) { return pair == 0 ? (i == 0 ? q[c].x : q[c].y) : (i == 0 ? q[c].z : q[c].w); };
+          if constexpr (TRANS) {
+            uint32_t o[32];
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
-              for (int c = 0; c < kQuarters; ++c)
-                sts128(dst + pair * (G::operand_bytes / 2) + (((4 * i + 2 * half + c) << 4) ^ swz), o[i][c][0], o[i][c][1], o[i][c][2], o[i][c][3]);
+              for (int c = 0; c < kQuarters; ++c) Scale<T>::word(word(i, c), r[i], o + 16 * i + 4 * c);
+            tmem_st32(tdst + pair * 32, o);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+              for (int c = 0; c < kQuarters; ++c) {
+                uint32_t o[4]; Scale<T>::word(word(i, c), r[i], o);
+                sts128(dst + pair * (G::operand_bytes / 2) + (((4 * i + 2 * half + c) << 4) ^ swz), o[0], o[1], o[2], o[3]);
+              }
           }
         }
       } else {
@@ -476,9 +484,9 @@ product_umma_kernel(const __grid_constant__ CUtensorMap code_map, const __grid_c
           const uint16_t* from = second + int64_t(of) * p.ld2 + tile * kOut + 64 * half;
           const int valid = c < 2 * p.rank16 && of < p.rank ? p.out - tile * kOut - 64 * half : 0;
 #pragma unroll 4
-          for (int j = 0; j < 8; ++j) {
+          for (int j = 0; j < (kFull ? 16 : 8); ++j) {
             const uint4 v = load8(reinterpret_cast<const T*>(from) + 8 * j, valid - 8 * j, p.second_aligned != 0);
-            sts128(dst + half * (G::operand_bytes / 2) + ((j << 4) ^ swz), v.x, v.y, v.z, v.w);
+            sts128(dst + (half + (j >> 3)) * (G::operand_bytes / 2) + (((j & 7) << 4) ^ swz), v.x, v.y, v.z, v.w);
           }
         }
       }
@@ -551,7 +559,7 @@ constexpr int kMidWarps = 8, kMidSplits = 8;
 // order of K inside an instruction is free as long as both operands agree.  The product waits for this kernel, so what counts is
 // its latency: 4096 rows, rank 64, 256 tokens took 9 us with one block per tile.
 template <class T> __global__ void __launch_bounds__(kMidWarps * 32)
-mid_split_kernel(const T* first, int64_t ld1, int rows, int rank, const T* x, int64_t ldx, int t, T* mid, int64_t ldm, int aligned) {
+mid_split_kernel(const T* first, int64_t ld1, int rows, int rank, const T* x, int64_t ldx, int t, T* mid, int64_t ldm, int aligned, float* mid32) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   __shared__ float red[kMidWarps][16][17];
   __shared__ __align__(16) float part[256];
@@ -599,7 +607,8 @@ mid_split_kernel(const T* first, int64_t ld1, int rows, int rank, const T* x, in
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int k = k0 + (e & 15) + i;
-      if (t0 + tok < t) {                            // zeros behind the rank
+      if (mid32) { if (t0 + tok < t && k < rank) mid32[(t0 + tok) * rank + k] = v[i]; }      // for the streaming kernel, in one part
+      else if (t0 + tok < t) {                       // zeros behind the rank
         T* m = mid + (t0 + tok) * ldm + k;
         const T value = from_f32<T>(v[i]);
         m[0] = value; m[ldm / 2] = from_f32<T>(v[i] - to_f32(value));
@@ -607,6 +616,23 @@ mid_split_kernel(const T* first, int64_t ld1, int rows, int rank, const T* x, in
     }
   }
   cluster_sync_all();
+}
+
+template <class T> cudaError_t start_mid(const hyacinHandle_t* handle, const T* first, int64_t ld1, int rows, int rank, const T* x, int64_t ldx, int t, T* mid, int64_t ldm, int aligned, float* mid32) {
+  cudaLaunchConfig_t mc{};
+  mc.gridDim = dim3(unsigned((rank + 15) / 16) * kMidSplits, unsigned((int64_t(t) + 15) / 16)); mc.blockDim = dim3(kMidWarps * 32); mc.stream = handle->cudaStream;
+  cudaLaunchAttribute ma[1];
+  ma[0].id = cudaLaunchAttributeClusterDimension; ma[0].val.clusterDim.x = kMidSplits; ma[0].val.clusterDim.y = 1; ma[0].val.clusterDim.z = 1;
+  mc.attrs = ma; mc.numAttrs = 1;
+  // the product's blocks move in beside this kernel's only if the SM is already split between cache and shared memory their way
+  static std::atomic<uint64_t> carved{0};
+  const uint64_t bit = uint64_t(1) << (handle->DeviceID & 63);
+  if (!(carved.load() & bit)) {
+    HYB_CUDA(cudaFuncSetAttribute(mid_split_kernel<T>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
+    carved.fetch_or(bit);
+  }
+  count_launch();
+  return cudaLaunchKernelEx(&mc, mid_split_kernel<T>, first, ld1, rows, rank, x, ldx, t, mid, ldm, aligned, mid32);
 }
 
 // X with rows that TMA can address (16-byte pitch and start).
@@ -637,7 +663,7 @@ int choose_splits(int64_t tiles, int steps, int slots, int overhead) {
   return best;
 }
 
-template <class T, bool TRANS> int32_t launch(const hyacinHandle_t* handle, const char* fn, hyacinPrecision_t type, const ProductArgs& a) {
+template <class T, bool TRANS, int STEP> int32_t launch(const hyacinHandle_t* handle, const char* fn, hyacinPrecision_t type, const ProductArgs& a) {
   cudaStream_t stream = handle->cudaStream;
   const int in = TRANS ? a.m : a.n, out = TRANS ? a.n : a.m;
   void *x_copy = nullptr, *mid = nullptr;
@@ -667,7 +693,7 @@ template <class T, bool TRANS> int32_t launch(const hyacinHandle_t* handle, cons
   const int per_block = p.seg_sub == 1 ? 4 : p.seg_sub == 2 ? 2 : 1;
   p.wide = per_block > 1 && a.lds % per_block == 0 && reinterpret_cast<uintptr_t>(a.scales) % (2 * per_block) == 0 &&
            reinterpret_cast<uintptr_t>(a.zeros) % per_block == 0 ? per_block : 1;
-  using G = Geometry<TRANS>;
+  using G = Geometry<TRANS, STEP>;
   constexpr int kStep = G::step;
   p.code_steps = (in + kStep - 1) / kStep;
   p.rank = a.rank; p.rank16 = (a.rank + 15) / 16 * 16; p.second = a.second; p.ld2 = a.ld2; p.y = a.y; p.ldy = a.ldy;
@@ -690,7 +716,7 @@ template <class T, bool TRANS> int32_t launch(const hyacinHandle_t* handle, cons
   const uint32_t smem = std::max(fixed + p.bufs * G::operand_bytes + p.ring * stage_bytes, kSmemFloor);
   p.second_aligned = reinterpret_cast<uintptr_t>(a.second) % 16 == 0 && a.ld2 % 8 == 0;
   const int tiles = (out + kOut - 1) / kOut;
-  p.splits = choose_splits(int64_t(tiles) * token_tiles, p.steps, handle->DeviceSMs, TRANS ? 6 : 12);
+  p.splits = choose_splits(int64_t(tiles) * token_tiles, p.steps, handle->DeviceSMs, kStep == 128 ? 6 : 12);
   const uint32_t fmt = type == HYACIN_F16 ? 0u : 1u;
   p.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((TRANS ? 0u : 1u) << 15) | (uint32_t(p.nt >> 3) << 17) | (uint32_t(kOut >> 4) << 24);
   p.status = status_word_device(handle->DeviceID);
@@ -704,24 +730,11 @@ template <class T, bool TRANS> int32_t launch(const hyacinHandle_t* handle, cons
     if (!allocate(&mid, size_t(ldm) * a.t * 2)) { cleanup(); return -3; }
     fine = encode_2d(&mid_map, dt, mid, uint64_t(ldm), a.t, uint64_t(ldm) * 2, 64, p.nt, CU_TENSOR_MAP_SWIZZLE_128B);
     const int aligned = reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx % 8 == 0 && reinterpret_cast<uintptr_t>(a.first) % 16 == 0 && a.ld1 % 8 == 0;
-    cudaLaunchConfig_t mc{};
-    mc.gridDim = dim3(unsigned((a.rank + 15) / 16) * kMidSplits, unsigned((int64_t(a.t) + 15) / 16)); mc.blockDim = dim3(kMidWarps * 32); mc.stream = stream;
-    cudaLaunchAttribute ma[1];
-    ma[0].id = cudaLaunchAttributeClusterDimension; ma[0].val.clusterDim.x = kMidSplits; ma[0].val.clusterDim.y = 1; ma[0].val.clusterDim.z = 1;
-    mc.attrs = ma; mc.numAttrs = 1;
-    // the product's blocks move in beside this kernel's only if the SM is already split between cache and shared memory their way
-    static std::atomic<uint64_t> carved{0};
-    const uint64_t mine = uint64_t(1) << (handle->DeviceID & 63);
-    if (!(carved.load() & mine)) {
-      HYB_CUDA(cudaFuncSetAttribute(mid_split_kernel<T>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
-      carved.fetch_or(mine);
-    }
-    count_launch();
-    const cudaError_t e = cudaLaunchKernelEx(&mc, mid_split_kernel<T>, static_cast<const T*>(a.first), a.ld1, in, a.rank, static_cast<const T*>(x), ldx, a.t, static_cast<T*>(mid), ldm, aligned);
+    const cudaError_t e = start_mid<T>(handle, static_cast<const T*>(a.first), a.ld1, in, a.rank, static_cast<const T*>(x), ldx, a.t, static_cast<T*>(mid), ldm, aligned, nullptr);
     if (e != cudaSuccess) { report_cuda_error(e, fn, __FILE__, __LINE__); fine = false; }
   }
   if (!fine) { cleanup(); return -3; }
-  auto* kernel = product_umma_kernel<T, TRANS>;
+  auto* kernel = product_umma_kernel<T, TRANS, STEP>;
   static std::atomic<uint64_t> ready{0};                         // per device: shared memory limit raised
   const uint64_t bit = uint64_t(1) << (handle->DeviceID & 63);
   if (!(ready.load() & bit)) {
@@ -744,9 +757,15 @@ template <class T, bool TRANS> int32_t launch(const hyacinHandle_t* handle, cons
 
 }  // namespace
 
+cudaError_t launch_mid_float(const hyacinHandle_t* handle, hyacinPrecision_t type, const void* first, int64_t ld1, int rows, int rank, const void* x, int64_t ldx, int t, float* mid, bool aligned) {
+  if (type == HYACIN_F16) return start_mid<__half>(handle, static_cast<const __half*>(first), ld1, rows, rank, static_cast<const __half*>(x), ldx, t, nullptr, 0, aligned, mid);
+  return start_mid<__nv_bfloat16>(handle, static_cast<const __nv_bfloat16*>(first), ld1, rows, rank, static_cast<const __nv_bfloat16*>(x), ldx, t, nullptr, 0, aligned, mid);
+}
+
 int32_t launch_product_umma(const hyacinHandle_t* handle, const char* fn, bool trans, hyacinPrecision_t type, const ProductArgs& a) {
-  if (type == HYACIN_F16) return trans ? launch<__half, true>(handle, fn, type, a) : launch<__half, false>(handle, fn, type, a);
-  return trans ? launch<__nv_bfloat16, true>(handle, fn, type, a) : launch<__nv_bfloat16, false>(handle, fn, type, a);
+  const bool small = a.t <= 128;
+  if (type == HYACIN_F16) return trans ? launch<__half, true, 128>(handle, fn, type, a) : small ? launch<__half, false, 128>(handle, fn, type, a) : launch<__half, false, 64>(handle, fn, type, a);
+  return trans ? launch<__nv_bfloat16, true, 128>(handle, fn, type, a) : small ? launch<__nv_bfloat16, false, 128>(handle, fn, type, a) : launch<__nv_bfloat16, false, 64>(handle, fn, type, a);
 }
 
 }  // namespace hyb
