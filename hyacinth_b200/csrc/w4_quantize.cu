@@ -62,40 +62,51 @@ template <class S> __device__ __forceinline__ SegmentCode segment_code(float lo,
   return c;
 }
 
+// kRound + rint(v / s), the form that the codes are read from.  For a 16-bit scale the quotient itself is cheaper than the remainder above:
+// one correction step (Markstein, IBM J. Res. Dev. 34, 1990) leaves it within 2^-22 of a last place of its rounding to 32 bits, and that
+// rounding hits a half only where the quotient is one: half * s is a 32-bit number then, so v is at least a last place away from
+// it, the quotient at least (1 + 2^-11) half places from the half.
+template <class S> __device__ __forceinline__ float quotient_bits(float v, float s, float inverse) {
+  if (sizeof(S) == 4) return rounded_quotient(v, s, inverse) + kRound;
+  const float q = __fmul_rn(v, inverse);
+  return __fadd_rn(__fmaf_rn(__fmaf_rn(-q, s, v), inverse, q), kRound);
+}
+__device__ __forceinline__ float larger(float a, float b) { float d; asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b)); return d; }
+
 // Segments of 32, 64, 128 or 256 rows: a lane owns eight consecutive rows, one word of codes, a warp 256 rows of a column; a
 // segment's lanes are neighbours and find its extremes with shuffles, so W is read once and everything stays in registers.
 // Rows that are not 16-byte aligned pass through shared memory, so that DRAM sees whole lines all the same.
-// Bound: DRAM (read W, write half a byte per weight, and 4 bytes of residual where asked for).
-// A warp walks down the columns of its row group with the next column's load in flight.
-template <class T, class S> __global__ void __launch_bounds__(256, 4) quantize_w4_warp_kernel(QuantizeArgs a, int w_aligned, int r_aligned) {
-  __shared__ float turns[8][256];
-  constexpr int kWords = int(sizeof(T)) * 8 / 16;
+// A warp walks down the columns of its row group with the next columns' loads in flight.
+// Bound: instruction issue beside DRAM (read W, write half a byte per weight, and 4 bytes of residual where asked for).
+template <class T, class S, bool WIDE> __device__ __forceinline__ void quantize_columns(const QuantizeArgs& a, int r_aligned, float* turn) {
+  constexpr int kWords = int(sizeof(T)) * 8 / 16, kDepth = WIDE && sizeof(T) == 2 ? 2 : 1;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  float* turn = turns[warp];
-  const int row0 = blockIdx.x * 256, row = row0 + lane * 8, valid = a.m - row, all = a.m - row0;
-  const bool wide = w_aligned && all >= 256, symmetric = a.zeros == nullptr;
-  const int step = gridDim.y * 8, lanes = a.seg / 8, r8 = row / 8;
+  const int row0 = blockIdx.x * 256, row = row0 + lane * 8, valid = WIDE ? 8 : a.m - row, all = WIDE ? 256 : a.m - row0;
+  const bool symmetric = a.zeros == nullptr;
+  const int step = gridDim.y * 8, lanes = a.seg / 8, r8 = row / 8, col0 = blockIdx.y * 8 + warp;
   const bool writes = r8 < (a.m + kW4Block - 1) / kW4Block * 16, leads = lane % lanes == 0 && valid > 0;
-  const int64_t code_at = int64_t(r8 / 16) * 64 + (4 * (r8 & 3) + ((r8 >> 2) & 3)) * 4;
-  const T* w = static_cast<const T*>(a.w) + row0;
-  uint4 raw[kWords]; T part[8];
-  auto fetch = [&](int col) {
-    if (col >= a.n) return;
-    const T* from = w + col * a.ldw;
-    if (wide) {
+  uint8_t* codes = a.codes + col0 * a.ldq + int64_t(r8 / 16) * 64 + (4 * (r8 & 3) + ((r8 >> 2) & 3)) * 4;
+  const T* from = static_cast<const T*>(a.w) + col0 * a.ldw + row0;
+  int64_t table = col0 * a.lds + row / a.seg;
+  float* to = a.r ? a.r + col0 * a.ldr + row0 : nullptr;
+  const int64_t w_step = step * a.ldw, q_step = step * a.ldq, s_step = step * a.lds, r_step = step * a.ldr;
+  uint4 raw[kDepth][kWords]; T part[8];
+  auto fetch = [&](int64_t col, int buf) {
+    if (col < a.n) {
+      if (WIDE) {
 #pragma unroll
-      for (int i = 0; i < kWords; ++i) raw[i] = __ldcs(reinterpret_cast<const uint4*>(from + lane * 8) + i);
-    } else {
+        for (int i = 0; i < kWords; ++i) raw[buf][i] = __ldcs(reinterpret_cast<const uint4*>(from + lane * 8) + i);
+      } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) if (i * 32 + lane < all) part[i] = from[i * 32 + lane];
+        for (int i = 0; i < 8; ++i) if (i * 32 + lane < all) part[i] = from[i * 32 + lane];
+      }
     }
+    from += w_step;
   };
-  int col = blockIdx.y * 8 + warp;
-  fetch(col);
-  for (; col < a.n; col += step) {
+  auto column = [&](int64_t col, int buf) {
     float v[8];
-    if (wide) {
-      const T* e = reinterpret_cast<const T*>(raw);
+    if (WIDE) {
+      const T* e = reinterpret_cast<const T*>(raw[buf]);
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] = to_f32(e[i]);
     } else {
@@ -107,11 +118,12 @@ template <class T, class S> __global__ void __launch_bounds__(256, 4) quantize_w
       for (int i = 0; i < 8; ++i) v[i] = turn[lane * 8 + i];
       __syncwarp();
     }
-    fetch(col + step);
-    // the largest magnitude as an integer finds infinities and NaNs as well
-    int size = 0;
+    fetch(col + kDepth * step, buf);
+    // the largest magnitude, infinities and NaNs among them; as an integer a NaN is the largest
+    float most = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) size = max(size, __float_as_int(v[i]) & 0x7fffffff);
+    for (int i = 0; i < 8; ++i) most = larger(most, fabsf(v[i]));
+    int size = __float_as_int(most) & 0x7fffffff;
     float lo = 0.f, hi = 0.f;
     if (symmetric) {
       for (int d = 1; d < lanes; d *= 2) size = max(size, __shfl_xor_sync(~0u, size, d));
@@ -125,51 +137,61 @@ template <class T, class S> __global__ void __launch_bounds__(256, 4) quantize_w
     }
     S scale; const SegmentCode c = segment_code<S>(lo, hi, size >= 0x7f800000, symmetric, &scale);
     if (leads) {
-      const int64_t at = col * a.lds + row / a.seg;
-      static_cast<S*>(a.scales)[at] = scale;
-      if (!symmetric) a.zeros[at] = uint8_t(c.zero);
+      static_cast<S*>(a.scales)[table] = scale;
+      if (!symmetric) a.zeros[table] = uint8_t(c.zero);
     }
+    table += s_step;
     const float s = to_f32(scale), inverse = reciprocal(s);
-    const bool slow = c.live && !ordinary(s, inverse, __int_as_float(size));
     // codes minus their zero point lie in [low, high]: 0 for a segment without a scale (also where the quotient is a NaN)
-    const float zero = float(c.zero), low = !c.live ? 0.f : symmetric ? -7.f : -zero, high = !c.live ? 0.f : symmetric ? 7.f : 15.f - zero;
-    uint32_t word = 0;
-    float r[8];
+    const float zero = float(c.zero), low = kRound + (!c.live ? 0.f : symmetric ? -7.f : -zero), high = kRound + (!c.live ? 0.f : symmetric ? 7.f : 15.f - zero);
+    float whole[8];                                  // kRound + the code minus its zero point
+    if (c.live && !ordinary(s, inverse, __int_as_float(size))) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float whole = fminf(fmaxf(rounded_quotient(v[i], s, inverse), low), high);
-      const uint32_t q = __float_as_uint(whole + (kRound + zero)) & 15u;
-      word |= q << (4 * w4_row_nibble(i));
-      r[i] = fmaf(-s, whole, v[i]);
-    }
-    if (slow) {                                      // the same with quotients in 64 bits
-      word = 0;
+      for (int i = 0; i < 8; ++i) whole[i] = fminf(fmaxf(quotient_in_64_bits(v[i], s) + kRound, low), high);
+    } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float whole = fminf(fmaxf(quotient_in_64_bits(v[i], s), low), high);
-        word |= (__float_as_uint(whole + (kRound + zero)) & 15u) << (4 * w4_row_nibble(i));
-        r[i] = fmaf(-s, whole, v[i]);
-      }
+      for (int i = 0; i < 8; ++i) whole[i] = fminf(fmaxf(quotient_bits<S>(v[i], s, inverse), low), high);
     }
-    if (valid < 8) {                                 // rows behind the last one are stored as 0
+    // the last places of kRound + k are 0x4b400000 + k: summed with shifts, the codes come out where they belong
+    uint32_t word = uint32_t(c.zero) * 0x11111111u - 0x4b400000u * 0x11111111u;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) word += __float_as_uint(whole[i]) << (4 * w4_row_nibble(i));
+    if (!WIDE && valid < 8) {                        // rows behind the last one are stored as 0
 #pragma unroll
       for (int i = 0; i < 8; ++i) if (i >= valid) word &= ~(15u << (4 * w4_row_nibble(i)));
     }
-    if (writes) *reinterpret_cast<uint32_t*>(a.codes + col * a.ldq + code_at) = word;
-    if (a.r) {
-      float* to = a.r + col * a.ldr + row0;
+    if (writes) *reinterpret_cast<uint32_t*>(codes) = word;
+    codes += q_step;
+    if (to) {
+      float r[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) r[i] = fmaf(-s, whole[i] - kRound, v[i]);
       if (r_aligned && all >= 256) {
         __stcs(reinterpret_cast<float4*>(to + lane * 8), make_float4(r[0], r[1], r[2], r[3]));
         __stcs(reinterpret_cast<float4*>(to + lane * 8) + 1, make_float4(r[4], r[5], r[6], r[7]));
       } else {
+        __syncwarp();
 #pragma unroll
         for (int i = 0; i < 8; ++i) turn[lane * 8 + i] = r[i];
         __syncwarp();
 #pragma unroll
         for (int i = 0; i < 8; ++i) if (i * 32 + lane < all) __stcs(to + i * 32 + lane, turn[i * 32 + lane]);
       }
+      to += r_step;
     }
+  };
+#pragma unroll
+  for (int d = 0; d < kDepth; ++d) fetch(col0 + d * step, d);
+  for (int64_t col = col0; col < a.n; col += kDepth * step) {
+#pragma unroll
+    for (int d = 0; d < kDepth; ++d) if (col + d * step < a.n) column(col + d * step, d);
   }
+}
+template <class T, class S> __global__ void __launch_bounds__(256, 4) quantize_w4_warp_kernel(QuantizeArgs a, int w_aligned, int r_aligned) {
+  __shared__ __align__(16) float turns[8][256];
+  float* turn = turns[threadIdx.x >> 5];
+  if (w_aligned && a.m - int(blockIdx.x) * 256 >= 256) quantize_columns<T, S, true>(a, r_aligned, turn);
+  else quantize_columns<T, S, false>(a, r_aligned, turn);
 }
 
 // Any other segment length: one warp per (column, segment), a pass for the extremes, a pass for the codes.
