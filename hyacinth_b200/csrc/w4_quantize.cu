@@ -39,17 +39,27 @@ __device__ __forceinline__ bool ordinary(float s, float inverse, float largest) 
 __device__ __noinline__ float quotient_in_64_bits(float v, float s) { return float(fmin(fmax(rint(double(v) / double(s)), -64.), 64.)); }
 __device__ __forceinline__ float reciprocal(float s) { float r; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s)); return r; }
 
+// x / by for 7 and 15.  A product with the rounded reciprocal is within a last place, and one step corrects it (Markstein, IBM J. Res. Dev.
+// 34, 1990; all 2^23 fractions compared with the division on the CPU); the range keeps the remainder's last place above the smallest number.
+__device__ __forceinline__ float divided(float x, float by) {
+  if (!(x > 1e-28f && x < 1e30f)) return __fdiv_rn(x, by);
+  const float inverse = by == 7.f ? 1.f / 7.f : 1.f / 15.f, q = __fmul_rn(x, inverse);
+  return __fmaf_rn(__fmaf_rn(-by, q, x), inverse, q);
+}
 // lo, hi: extremes of the segment together with 0; bad: it holds a NaN or an infinity.  float(double / 7) is the 32-bit quotient;
 // so is float(double / 15) of a difference that 32 bits hold.
+template <class S> __device__ __forceinline__ S segment_scale(float lo, float hi, bool bad, bool symmetric) {
+  float span;
+  if (symmetric) span = divided(fmaxf(-lo, hi), 7.f);
+  else {
+    const float more = fmaxf(hi, -lo), less = fminf(hi, -lo), f = __fadd_rn(more, less);
+    span = __fsub_rn(f, more) == less ? divided(f, 15.f) : float((double(hi) - double(lo)) / 15.);   // the sum is exact or it is not
+  }
+  return from_f32<S>(bad ? __int_as_float(0x7fc00000) : span);
+}
 template <class S> __device__ __forceinline__ SegmentCode segment_code(float lo, float hi, bool bad, bool symmetric, S* scale) {
   SegmentCode c;
-  float span;
-  if (symmetric) span = __fdiv_rn(fmaxf(-lo, hi), 7.f);
-  else {
-    const double d = double(hi) - double(lo); const float f = float(d);
-    span = double(f) == d ? __fdiv_rn(f, 15.f) : float(d / 15.);
-  }
-  *scale = from_f32<S>(bad ? __int_as_float(0x7fc00000) : span);
+  *scale = segment_scale<S>(lo, hi, bad, symmetric);
   const float s = to_f32(*scale);
   c.s = double(s);
   c.live = s > 0.f;                                    // false for NaN as well
@@ -78,11 +88,10 @@ __device__ __forceinline__ float larger(float a, float b) { float d; asm("max.Na
 // Rows that are not 16-byte aligned pass through shared memory, so that DRAM sees whole lines all the same.
 // A warp walks down the columns of its row group with the next columns' loads in flight.
 // Bound: instruction issue beside DRAM (read W, write half a byte per weight, and 4 bytes of residual where asked for).
-template <class T, class S, bool WIDE> __device__ __forceinline__ void quantize_columns(const QuantizeArgs& a, int r_aligned, float* turn) {
+template <class T, class S, bool SYMMETRIC, bool WIDE> __device__ __forceinline__ void quantize_columns(const QuantizeArgs& a, int r_aligned, float* turn) {
   constexpr int kWords = int(sizeof(T)) * 8 / 16, kDepth = WIDE && sizeof(T) == 2 ? 2 : 1;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int row0 = blockIdx.x * 256, row = row0 + lane * 8, valid = WIDE ? 8 : a.m - row, all = WIDE ? 256 : a.m - row0;
-  const bool symmetric = a.zeros == nullptr;
   const int step = gridDim.y * 8, lanes = a.seg / 8, r8 = row / 8, col0 = blockIdx.y * 8 + warp;
   const bool writes = r8 < (a.m + kW4Block - 1) / kW4Block * 16, leads = lane % lanes == 0 && valid > 0;
   uint8_t* codes = a.codes + col0 * a.ldq + int64_t(r8 / 16) * 64 + (4 * (r8 & 3) + ((r8 >> 2) & 3)) * 4;
@@ -90,6 +99,9 @@ template <class T, class S, bool WIDE> __device__ __forceinline__ void quantize_
   int64_t table = col0 * a.lds + row / a.seg;
   float* to = a.r ? a.r + col0 * a.ldr + row0 : nullptr;
   const int64_t w_step = step * a.ldw, q_step = step * a.ldq, s_step = step * a.lds, r_step = step * a.ldr;
+  int partner[5];
+#pragma unroll
+  for (int i = 0; i < 5; ++i) partner[i] = (1 << i) < lanes ? 1 << i : 0;
   uint4 raw[kDepth][kWords]; T part[8];
   auto fetch = [&](int64_t col, int buf) {
     if (col < a.n) {
@@ -125,35 +137,41 @@ template <class T, class S, bool WIDE> __device__ __forceinline__ void quantize_
     for (int i = 0; i < 8; ++i) most = larger(most, fabsf(v[i]));
     int size = __float_as_int(most) & 0x7fffffff;
     float lo = 0.f, hi = 0.f;
-    if (symmetric) {
-      for (int d = 1; d < lanes; d *= 2) size = max(size, __shfl_xor_sync(~0u, size, d));
-      hi = __int_as_float(size);
-    } else {
+    if (!SYMMETRIC) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) { lo = fminf(lo, v[i]); hi = fmaxf(hi, v[i]); }
-      for (int d = 1; d < lanes; d *= 2) {
-        size = max(size, __shfl_xor_sync(~0u, size, d)); lo = fminf(lo, __shfl_xor_sync(~0u, lo, d)); hi = fmaxf(hi, __shfl_xor_sync(~0u, hi, d));
-      }
     }
-    S scale; const SegmentCode c = segment_code<S>(lo, hi, size >= 0x7f800000, symmetric, &scale);
-    if (leads) {
-      static_cast<S*>(a.scales)[table] = scale;
-      if (!symmetric) a.zeros[table] = uint8_t(c.zero);
-    }
-    table += s_step;
-    const float s = to_f32(scale), inverse = reciprocal(s);
-    // codes minus their zero point lie in [low, high]: 0 for a segment without a scale (also where the quotient is a NaN)
-    const float zero = float(c.zero), low = kRound + (!c.live ? 0.f : symmetric ? -7.f : -zero), high = kRound + (!c.live ? 0.f : symmetric ? 7.f : 15.f - zero);
-    float whole[8];                                  // kRound + the code minus its zero point
-    if (c.live && !ordinary(s, inverse, __int_as_float(size))) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) whole[i] = fminf(fmaxf(quotient_in_64_bits(v[i], s) + kRound, low), high);
-    } else {
+    for (int i = 0; i < 5; ++i) {                    // a lane beyond the segment's is taken for itself
+      size = max(size, __shfl_xor_sync(~0u, size, partner[i]));
+      if (!SYMMETRIC) { lo = fminf(lo, __shfl_xor_sync(~0u, lo, partner[i])); hi = fmaxf(hi, __shfl_xor_sync(~0u, hi, partner[i])); }
+    }
+    const float largest = __int_as_float(size);
+    if (SYMMETRIC) hi = largest;
+    const S scale = segment_scale<S>(lo, hi, size >= 0x7f800000, SYMMETRIC);
+    const float s = to_f32(scale), inverse = reciprocal(s);
+    float zero = SYMMETRIC ? 8.f : 0.f, whole[8];    // whole: kRound + the code minus its zero point
+    if (ordinary(s, inverse, largest)) {
+      if (!SYMMETRIC) zero = fminf(quotient_bits<S>(-lo, s, inverse) - kRound, 15.f);
+      const float low = kRound - (SYMMETRIC ? 7.f : zero), high = kRound + (SYMMETRIC ? 7.f : 15.f - zero);
 #pragma unroll
       for (int i = 0; i < 8; ++i) whole[i] = fminf(fmaxf(quotient_bits<S>(v[i], s, inverse), low), high);
+    } else if (s > 0.f) {                            // the same with quotients in 64 bits
+      if (!SYMMETRIC) zero = fminf(fmaxf(quotient_in_64_bits(-lo, s), 0.f), 15.f);
+      const float low = SYMMETRIC ? -7.f : -zero, high = SYMMETRIC ? 7.f : 15.f - zero;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) whole[i] = kRound + fminf(fmaxf(quotient_in_64_bits(v[i], s), low), high);
+    } else {                                         // no scale: nothing but zeros, or a NaN
+#pragma unroll
+      for (int i = 0; i < 8; ++i) whole[i] = kRound;
     }
+    if (leads) {
+      static_cast<S*>(a.scales)[table] = scale;
+      if (!SYMMETRIC) a.zeros[table] = uint8_t(int(zero));
+    }
+    table += s_step;
     // the last places of kRound + k are 0x4b400000 + k: summed with shifts, the codes come out where they belong
-    uint32_t word = uint32_t(c.zero) * 0x11111111u - 0x4b400000u * 0x11111111u;
+    uint32_t word = (__float_as_uint(kRound + zero) - 0x4b400000u) * 0x11111111u - 0x4b400000u * 0x11111111u;
 #pragma unroll
     for (int i = 0; i < 8; ++i) word += __float_as_uint(whole[i]) << (4 * w4_row_nibble(i));
     if (!WIDE && valid < 8) {                        // rows behind the last one are stored as 0
@@ -187,11 +205,11 @@ template <class T, class S, bool WIDE> __device__ __forceinline__ void quantize_
     for (int d = 0; d < kDepth; ++d) if (col + d * step < a.n) column(col + d * step, d);
   }
 }
-template <class T, class S> __global__ void __launch_bounds__(256, 4) quantize_w4_warp_kernel(QuantizeArgs a, int w_aligned, int r_aligned) {
+template <class T, class S, bool SYMMETRIC> __global__ void __launch_bounds__(256, 4) quantize_w4_warp_kernel(QuantizeArgs a, int w_aligned, int r_aligned) {
   __shared__ __align__(16) float turns[8][256];
   float* turn = turns[threadIdx.x >> 5];
-  if (w_aligned && a.m - int(blockIdx.x) * 256 >= 256) quantize_columns<T, S, true>(a, r_aligned, turn);
-  else quantize_columns<T, S, false>(a, r_aligned, turn);
+  if (w_aligned && a.m - int(blockIdx.x) * 256 >= 256) quantize_columns<T, S, SYMMETRIC, true>(a, r_aligned, turn);
+  else quantize_columns<T, S, SYMMETRIC, false>(a, r_aligned, turn);
 }
 
 // Any other segment length: one warp per (column, segment), a pass for the extremes, a pass for the codes.
@@ -260,7 +278,8 @@ extern "C" int32_t hyacinB200QuantizeW4(const hyacinHandle_t* handle, hyacinPrec
     // about six blocks per SM, so that a warp sees several columns
     const int64_t chunks = std::max<int64_t>(1, std::min<int64_t>({(int64_t(N) + 7) / 8, 6 * int64_t(handle->DeviceSMs) / groups, 65535}));
     with_w4_type(Wtype, [&](auto t) { with_w4_type(Stype, [&](auto s) {
-      quantize_w4_warp_kernel<decltype(t), decltype(s)><<<dim3(unsigned(groups), unsigned(chunks)), 256, 0, handle->cudaStream>>>(a, w_aligned, r_aligned);
+      auto* kernel = zeros ? quantize_w4_warp_kernel<decltype(t), decltype(s), false> : quantize_w4_warp_kernel<decltype(t), decltype(s), true>;
+      kernel<<<dim3(unsigned(groups), unsigned(chunks)), 256, 0, handle->cudaStream>>>(a, w_aligned, r_aligned);
     }); });
     return w4_launched("quantize_w4_warp_kernel");
   }
