@@ -81,7 +81,7 @@ template <class S> __device__ __forceinline__ float quotient_bits(float v, float
   const float q = __fmul_rn(v, inverse);
   return __fadd_rn(__fmaf_rn(__fmaf_rn(-q, s, v), inverse, q), kRound);
 }
-__device__ __forceinline__ float larger(float a, float b) { float d; asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b)); return d; }
+__device__ __forceinline__ float largest_of(float a, float b, float c) { float d; asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c)); return d; }
 
 // Segments of 32, 64, 128 or 256 rows: a lane owns eight consecutive rows, one word of codes, a warp 256 rows of a column; a
 // segment's lanes are neighbours and find its extremes with shuffles, so W is read once and everything stays in registers.
@@ -132,9 +132,7 @@ template <class T, class S, bool SYMMETRIC, bool WIDE> __device__ __forceinline_
     }
     fetch(col + kDepth * step, buf);
     // the largest magnitude, infinities and NaNs among them; as an integer a NaN is the largest
-    float most = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) most = larger(most, fabsf(v[i]));
+    const float most = largest_of(largest_of(v[0], v[1], v[2]), largest_of(v[3], v[4], v[5]), largest_of(v[6], v[7], 0.f));
     int size = __float_as_int(most) & 0x7fffffff;
     float lo = 0.f, hi = 0.f;
     if (!SYMMETRIC) {
@@ -151,11 +149,15 @@ template <class T, class S, bool SYMMETRIC, bool WIDE> __device__ __forceinline_
     const S scale = segment_scale<S>(lo, hi, size >= 0x7f800000, SYMMETRIC);
     const float s = to_f32(scale), inverse = reciprocal(s);
     float zero = SYMMETRIC ? 8.f : 0.f, whole[8];    // whole: kRound + the code minus its zero point
-    if (ordinary(s, inverse, largest)) {
-      if (!SYMMETRIC) zero = fminf(quotient_bits<S>(-lo, s, inverse) - kRound, 15.f);
-      const float low = kRound - (SYMMETRIC ? 7.f : zero), high = kRound + (SYMMETRIC ? 7.f : 15.f - zero);
+    // With the largest quotient below 7.44 (15.44) nothing has to be clamped but the upper end beside a zero point, where both ends may
+    // have been rounded up: rint is monotonic and odd, so no code falls below 1 (0).
+    if (ordinary(s, inverse, largest) && largest * inverse < (SYMMETRIC ? 7.4375f : 15.4375f)) {
+      if (!SYMMETRIC) zero = quotient_bits<S>(-lo, s, inverse) - kRound;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) whole[i] = fminf(fmaxf(quotient_bits<S>(v[i], s, inverse), low), high);
+      for (int i = 0; i < 8; ++i) {
+        whole[i] = quotient_bits<S>(v[i], s, inverse);
+        if (!SYMMETRIC) whole[i] = fminf(whole[i], kRound + 15.f - zero);
+      }
     } else if (s > 0.f) {                            // the same with quotients in 64 bits
       if (!SYMMETRIC) zero = fminf(fmaxf(quotient_in_64_bits(-lo, s), 0.f), 15.f);
       const float low = SYMMETRIC ? -7.f : -zero, high = SYMMETRIC ? 7.f : 15.f - zero;
@@ -275,8 +277,8 @@ extern "C" int32_t hyacinB200QuantizeW4(const hyacinHandle_t* handle, hyacinPrec
     const int64_t groups = (int64_t(M) + 255) / 256;
     const int w_aligned = reinterpret_cast<uintptr_t>(W) % 16 == 0 && int64_t(ldw) * int64_t(w4_type_bytes(Wtype)) % 16 == 0;
     const int r_aligned = reinterpret_cast<uintptr_t>(R) % 16 == 0 && ldr % 4 == 0;
-    // about six blocks per SM, so that a warp sees several columns
-    const int64_t chunks = std::max<int64_t>(1, std::min<int64_t>({(int64_t(N) + 7) / 8, 6 * int64_t(handle->DeviceSMs) / groups, 65535}));
+    // about eight blocks per SM, so that a warp sees several columns
+    const int64_t chunks = std::max<int64_t>(1, std::min<int64_t>({(int64_t(N) + 7) / 8, 8 * int64_t(handle->DeviceSMs) / groups, 65535}));
     with_w4_type(Wtype, [&](auto t) { with_w4_type(Stype, [&](auto s) {
       auto* kernel = zeros ? quantize_w4_warp_kernel<decltype(t), decltype(s), false> : quantize_w4_warp_kernel<decltype(t), decltype(s), true>;
       kernel<<<dim3(unsigned(groups), unsigned(chunks)), 256, 0, handle->cudaStream>>>(a, w_aligned, r_aligned);
