@@ -380,7 +380,8 @@ template <class T> __global__ void __launch_bounds__(kClusterThreads, 3) distill
       edge[threadIdx.x] = mine ? to_f32(z[j]) : -INFINITY;
     }
     main_sync();
-    ptx::mbar_wait(&bar, 0u, &abort_flag, status, 41u);      // expired: the status word says so, the values are then undefined
+    // expired: the status word says so, the values are then undefined, and the copies get a second term before shared memory goes
+    if (!ptx::mbar_wait(&bar, 0u, &abort_flag, status, 41u)) { uint32_t ignore = 0; ptx::mbar_wait(&bar, 0u, &ignore, status, 42u); }
     asm volatile("bar.sync 2, %0;" ::"n"(kClusterThreads) : "memory");        // every thread has seen the copy land, and the classes
     for (int i = threadIdx.x; i < a.k; i += kMainThreads) {  // listed classes leave the row (equal values for a class listed twice)
       const int id = s.id[i];
@@ -546,6 +547,8 @@ int32_t check_distill(const char* fn, const hyacinHandle_t* handle, hyacinPrecis
   if (a.k > 0 && (!a.ids || !a.teacher || a.ldk < a.k)) return w4_refuse(fn, "ids, teacher: null or leading dimension too small");
   if (a.dz && a.lddz < a.n) return w4_refuse(fn, "dZ: leading dimension too small");
   if (a.dz == a.z && a.lddz != a.ldz) return w4_refuse(fn, "dZ in place of Z needs the same leading dimension");
+  if (!w4_on_boundary(w4_type_bytes(type), a.z, a.dz) || !w4_on_boundary(4, a.ids, a.teacher, a.teacher_lse, a.weight, a.loss, a.stats_out, a.stats_in))
+    return w4_refuse(fn, "a pointer that is not on a boundary of its type");
   if (!w4_device_ok(handle)) return w4_refuse(fn, "the handle belongs to another device than the current one");
   return 0;
 }

@@ -40,6 +40,9 @@ inline int32_t w4_refuse(const char* fn, const char* why) {
   std::fprintf(stderr, "hyacin-b200: %s: %s\n", fn, why);
   return -1;
 }
+// Pointers lie on a boundary of their type's size: the kernels' loads would fault otherwise.
+inline bool w4_on_boundary(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+template <class... P> bool w4_on_boundary(size_t bytes, P... p) { return (w4_on_boundary(static_cast<const void*>(p), bytes) && ...); }
 // The handle's device must be the current one: launches would otherwise go to the wrong GPU.
 inline bool w4_device_ok(const hyacinHandle_t* handle) {
   int device = -1;

@@ -136,6 +136,7 @@ extern "C" int32_t hyacinB200ProductW4(const hyacinHandle_t* handle, char opW, i
   if (!is_w4_type(Xtype)) return w4_refuse(fn, "type not supported");
   if (M < 0 || N < 0 || T < 0 || rank < 0 || segM <= 0 || segM % 32) return w4_refuse(fn, "sizes: M, N, T, rank >= 0 and segM a positive multiple of 32");
   if (M > 0x7fffff00 || N > 0x7fffff00 || T > 0x7fffff00) return w4_refuse(fn, "sizes: M, N, T at most 2^31 - 256");
+  if (rank > 1 << 20) return w4_refuse(fn, "rank: at most 2^20");
   const int in = trans ? M : N, out = trans ? N : M;
   if (T == 0 || out == 0) return 0;
   if (!Y || ldy < out) return w4_refuse(fn, "Y: null or leading dimension too small");
@@ -146,6 +147,8 @@ extern "C" int32_t hyacinB200ProductW4(const hyacinHandle_t* handle, char opW, i
     if (ldq % 16 || ldq < (int64_t(M) + 127) / 128 * 64 || reinterpret_cast<uintptr_t>(codes) % 16) return w4_refuse(fn, "codes: 16-byte aligned, ldq a multiple of 16 and at least 64 ceil(M / 128)");
     if (rank > 0 && (!U || !V || ldu < M || ldv < N)) return w4_refuse(fn, "U, V: null or leading dimension too small");
   }
+  if (!w4_on_boundary(w4_type_bytes(Xtype), Y) || (in > 0 && !w4_on_boundary(w4_type_bytes(Xtype), X, scales)) || (in > 0 && rank > 0 && !w4_on_boundary(w4_type_bytes(Xtype), U, V)))
+    return w4_refuse(fn, "a pointer that is not on a boundary of its type");
   if (!w4_device_ok(handle)) return w4_refuse(fn, "the handle belongs to another device than the current one");
   cudaStream_t stream = handle->cudaStream;
   PlainArgs a;

@@ -38,7 +38,7 @@ constexpr int kThreads = 32 * (2 + kLoaders + kGroups * kGroupWarps);
 // wait for one another could not afford.
 constexpr uint32_t kSmemLimit = 232448, kSmemFloor = 120 * 1024;
 template <bool TRANS, int STEP> struct Geometry {
-  static constexpr int step = STEP;                                      // K per step: 128; 64 for 'N' with more than 128 tokens, whose tiles leave less room
+  static constexpr int step = STEP;                                      // K per step
   static constexpr int cols = TRANS ? kOut : step;                       // columns of W per step
   static constexpr uint32_t code_bytes = cols * 64;
   static constexpr uint32_t scale_bytes = cols * 12;                     // four 16-bit scales and four zero points per column
@@ -637,7 +637,8 @@ template <class T> cudaError_t start_mid(const hyacinHandle_t* handle, const T* 
 
 // X with rows that TMA can address (16-byte pitch and start).
 __global__ void __launch_bounds__(256) align_rows_kernel(const uint16_t* x, int64_t ldx, int rows, uint16_t* out, int64_t ldo) {
-  for (int r = blockIdx.x * 256 + threadIdx.x; r < rows; r += gridDim.x * 256) out[int64_t(blockIdx.y) * ldo + r] = x[int64_t(blockIdx.y) * ldx + r];
+  const int64_t r = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  if (r < rows) out[int64_t(blockIdx.y) * ldo + r] = x[int64_t(blockIdx.y) * ldx + r];
 }
 
 bool encode_2d(CUtensorMap* map, CUtensorMapDataType type, const void* ptr, uint64_t inner, uint64_t outer, uint64_t pitch, uint32_t box_inner, uint32_t box_outer,
@@ -763,6 +764,19 @@ cudaError_t launch_mid_float(const hyacinHandle_t* handle, hyacinPrecision_t typ
 }
 
 int32_t launch_product_umma(const hyacinHandle_t* handle, const char* fn, bool trans, hyacinPrecision_t type, const ProductArgs& a) {
+  constexpr int kMostTokens = 1 << 19;                           // of one launch: the grids' second dimensions end at 65535
+  if (a.t > kMostTokens) {
+    int32_t rc = 0;
+    for (int64_t t0 = 0; t0 < a.t && rc == 0; t0 += kMostTokens) {
+      ProductArgs b = a;
+      b.t = int(std::min<int64_t>(kMostTokens, a.t - t0));
+      b.x = static_cast<const uint16_t*>(a.x) + t0 * a.ldx; b.y = static_cast<uint16_t*>(a.y) + t0 * a.ldy;
+      rc = launch_product_umma(handle, fn, trans, type, b);
+    }
+    return rc;
+  }
+  // opW 'N' keeps its operand in shared memory.  Steps of 128 columns halve the hand-overs between the warps' roles (4096 x 16384 times 64
+  // tokens 28 against 36 us), but beside tiles of more than 128 tokens only two of them fit (times 256: 47 against 42 us).
   const bool small = a.t <= 128;
   if (type == HYACIN_F16) return trans ? launch<__half, true, 128>(handle, fn, type, a) : small ? launch<__half, false, 128>(handle, fn, type, a) : launch<__half, false, 64>(handle, fn, type, a);
   return trans ? launch<__nv_bfloat16, true, 128>(handle, fn, type, a) : small ? launch<__nv_bfloat16, false, 128>(handle, fn, type, a) : launch<__nv_bfloat16, false, 64>(handle, fn, type, a);

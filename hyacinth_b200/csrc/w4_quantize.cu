@@ -221,7 +221,7 @@ template <class T, class S> __global__ void __launch_bounds__(256) quantize_w4_k
   if (task >= int64_t(a.n) * a.segs) return;
   const int col = int(task / a.segs), seg = int(task % a.segs);
   const T* w = static_cast<const T*>(a.w) + col * a.ldw;
-  const int row0 = seg * a.seg, row1 = min(row0 + a.seg, a.m);
+  const int row0 = seg * a.seg, row1 = int(min(int64_t(row0) + a.seg, int64_t(a.m)));
   float lo = 0.f, hi = 0.f; bool bad = false;
   for (int r = row0 + lane; r < row1; r += 32) {
     const float v = to_f32(w[r]);
@@ -236,7 +236,7 @@ template <class T, class S> __global__ void __launch_bounds__(256) quantize_w4_k
     if (!symmetric) a.zeros[col * a.lds + seg] = uint8_t(c.zero);
   }
   // words of the segment's 32-row subsets; the last segment also fills its block up
-  const int sub0 = row0 / 32, sub1 = (row0 + a.seg >= a.m) ? (a.m + kW4Block - 1) / kW4Block * 4 : (row0 + a.seg) / 32;
+  const int sub0 = row0 / 32, sub1 = seg + 1 == a.segs ? (a.m + kW4Block - 1) / kW4Block * 4 : row1 / 32;
   for (int k = lane; k < (sub1 - sub0) * 4; k += 32) {
     const int sub = sub0 + k / 4, quarter = k & 3, row = 32 * sub + 8 * quarter;
     uint32_t word = 0;
@@ -262,11 +262,13 @@ extern "C" int32_t hyacinB200QuantizeW4(const hyacinHandle_t* handle, hyacinPrec
   if (!handle) return w4_refuse(fn, "no handle");
   if (!is_w4_type(Wtype) || !is_w4_type(Stype)) return w4_refuse(fn, "type not supported");
   if (M < 0 || N < 0 || segM <= 0 || segM % 32) return w4_refuse(fn, "sizes: M, N >= 0 and segM a positive multiple of 32");
+  if (M > 0x7fffff00 || N > 0x7fffff00) return w4_refuse(fn, "sizes: M, N at most 2^31 - 256");
   if (M == 0 || N == 0) return 0;
   const int segs = (int64_t(M) + segM - 1) / segM;
   if (!W || !codes || !scales) return w4_refuse(fn, "null pointer");
   if (ldw < M || lds < segs || (R && ldr < M)) return w4_refuse(fn, "leading dimension too small");
   if (ldq % 16 || ldq < (int64_t(M) + 127) / 128 * 64 || reinterpret_cast<uintptr_t>(codes) % 16) return w4_refuse(fn, "codes: 16-byte aligned, ldq a multiple of 16 and at least 64 ceil(M / 128)");
+  if (!w4_on_boundary(w4_type_bytes(Wtype), W) || !w4_on_boundary(w4_type_bytes(Stype), scales) || !w4_on_boundary(4, R)) return w4_refuse(fn, "a pointer that is not on a boundary of its type");
   if (!w4_device_ok(handle)) return w4_refuse(fn, "the handle belongs to another device than the current one");
   QuantizeArgs a{W, ldw, M, N, segM, segs, codes, ldq, scales, zeros, lds, R, ldr};
   const int64_t blocks = (int64_t(N) * segs + 7) / 8;

@@ -15,8 +15,8 @@
 extern "C" {
 #endif
 
-/* Non-zero if a bounded wait inside the Gram kernel expired on the current device since the word was last
- * cleared (the integer Gram of that call is then invalid).  Call after synchronising the stream.
+/* Non-zero if a bounded wait inside a kernel (Gram, product of 4-bit weights, distillation loss) expired on the current device since the
+ * word was last cleared (the results of that call are then invalid).  Call after synchronising the stream.
  * No counterpart in the reference (its kernels have no waits). */
 uint32_t hyacinB200Status(int32_t clear);
 
@@ -159,7 +159,7 @@ int32_t hyacinB200PivotedCholesky(const hyacinHandle_t* handle, double eps, int3
  * All calls are asynchronous on handle->cudaStream, may be captured into a CUDA graph, and return 0, -1 for arguments
  * they do not take (message on stderr, nothing launched), or -3 when CUDA refused a launch or an allocation.  The handle
  * has to belong to the current device.  Scratch comes from handle->mempool in stream order.  Outputs do not overlap inputs
- * unless stated.  Results do not depend on timing: there are no atomic sums. */
+ * unless stated.  M, N and T of the products are at most 2^31 - 256, and pointers lie on a boundary of their type.  Results do not depend on timing: there are no atomic sums. */
 #define HYACIN_B200_BF16 ((hyacinPrecision_t)32)
 
 /* 4-bit form of W (type Wtype, leading dimension ldw).  scales has type Stype.  zeros == NULL: symmetric,
@@ -174,7 +174,8 @@ int32_t hyacinB200QuantizeW4(const hyacinHandle_t* handle, hyacinPrecision_t Wty
 /* opW 'T': Y (N x T) = Wq^T X + V (U^T X), X (M x T).   opW 'N': Y (M x T) = Wq X + U (V^T X), X (N x T), the gradient of
  * the former to its input.  U is M x rank, V is N x rank; rank 0 leaves the correction out.  scales, X, Y, U and V have type
  * Xtype.  Any T >= 0; made for few vectors.  Sums are held in 32 bits and Y is rounded once.  The 16-bit types round the
- * scaled weights to 16 bits before the product for opW 'N' and for T > 16. */
+ * scaled weights to 16 bits before the product for opW 'N' and, but for some scale tables, for T > 8; single precision is made for up to
+ * five vectors a pass.  rank <= 2^20. */
 int32_t hyacinB200ProductW4(const hyacinHandle_t* handle, char opW, int32_t M, int32_t N, int32_t T, hyacinPrecision_t Xtype,
                             const uint8_t* codes, int64_t ldq, int32_t segM, const void* scales, const uint8_t* zeros, int32_t lds,
                             const void* X, int32_t ldx, int32_t rank, const void* U, int32_t ldu, const void* V, int32_t ldv,
@@ -191,8 +192,9 @@ int32_t hyacinB200ProductW4(const hyacinHandle_t* handle, char opW, int32_t M, i
  * weight[t] * dKL_t / dz; weight == NULL means 1; a token with weight 0 is not read and gets loss 0 and a zero gradient.
  * loss, dZ and stats may each be NULL; stats (2 floats per token) is what hyacinB200DistillGrad needs to give the same
  * gradient later, with the weights known by then (NaN for a token that had weight 0).  1e-30 <= tau <= 1e30, 0 <= K <= 1024,
- * 1 <= N <= 2^20.  A student probability of zero under a
- * positive teacher probability gives an infinite loss and a finite gradient. */
+ * 1 <= N <= 2^20; finite
+ * logits stay below 2^127 tau in magnitude.  A student probability of zero under a positive teacher probability gives an infinite loss and a
+ * finite gradient. */
 int32_t hyacinB200DistillLoss(const hyacinHandle_t* handle, hyacinPrecision_t Ztype, int32_t N, int32_t T, const void* Z, int32_t ldz,
                               int32_t K, const int32_t* ids, const float* teacher, int32_t ldk, double tau, const float* teacherLse,
                               const float* weight, float* loss, float* stats, void* dZ, int32_t lddz);

@@ -71,7 +71,7 @@ def _check(r, z, ids, teacher, tau, lse, weight, d=None):
     tol = P.HALF_STEP["f32"] * np.abs(want_loss) + 2 * TERM * w * 2
     fin = np.isfinite(want_loss)
     assert np.array_equal(got[~fin], want_loss[~fin])
-    assert (np.abs(got - want_loss)[fin] <= tol[fin]).all(), (np.abs(got - want_loss)[fin] / tol[fin]).max()
+    assert (np.abs(got[fin] - want_loss[fin]) <= tol[fin]).all(), (np.abs(got[fin] - want_loss[fin]) / tol[fin]).max()
     if d is None:
         return
     g = d[:, :r.n].double().cpu().numpy()

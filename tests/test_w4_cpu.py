@@ -123,3 +123,14 @@ def test_plain_distillation_gradient_against_differences(tail):
         d[0, j] = step
         diff = (P.distill(z + d, ids, teacher, tau, lse, weight)[0] - P.distill(z - d, ids, teacher, tau, lse, weight)[0]) / (2 * step)
         assert abs(diff[0] - grad[0, j]) < 2e-9
+
+
+def test_pointers_off_their_boundary_and_sizes_beyond_the_largest_are_refused():
+    for bad in (dict(W=FAKE + 2), dict(wtype=api.F16, W=FAKE + 1), dict(scales=FAKE + 2), dict(R=FAKE + 2, ldr=200), dict(m=0x7fffff80, ldw=0x7fffff80, seg=1 << 20, lds=4096, ldq=1 << 30)):
+        assert _quantize(**bad) == -1
+    factors = dict(rank=2, U=FAKE, ldu=200, V=FAKE, ldv=3)
+    for bad in (dict(X=FAKE + 1), dict(Y=FAKE + 1), dict(scales=FAKE + 1), dict(factors, U=FAKE + 1), dict(factors, V=FAKE + 1), dict(factors, rank=(1 << 20) + 1), dict(t=0x7fffff80)):
+        assert _product(**bad) == -1
+    for bad in (dict(Z=FAKE + 1), dict(ids=FAKE + 2), dict(teacher=FAKE + 2), dict(lse=FAKE + 1), dict(weight=FAKE + 2), dict(stats=FAKE + 2), dict(dZ=FAKE + 4097, lddz=100)):
+        assert _loss(**bad) == -1 and _grad(**bad) == -1
+    assert _loss(loss=FAKE + 2) == -1

@@ -351,3 +351,115 @@ def test_quantise_fit_product_and_distil_together(hy):
         d = np.zeros_like(xd); d[a, b] = step
         diff = (P.distill((xd + d) @ weff.T, *args)[0][a] - P.distill((xd - d) @ weff.T, *args)[0][a]) / (2 * step)
         assert abs(diff - want_dx[a, b]) < 1e-6
+
+
+# ---- the ends of the ranges ------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("wkind,skind", [("f32", "f32"), ("f32", "f16"), ("f32", "bf16"), ("f16", "f16"), ("bf16", "bf16"), ("bf16", "f32"), ("f16", "f32")])
+@pytest.mark.parametrize("zeros", [False, True])
+def test_codes_beside_halves_and_at_the_ends_of_the_range(hy, wkind, skind, zeros):
+    """Weights on every half-way point of their scale and on the numbers next to it, for scales of every size: those that lose bits as
+    a subnormal number, vanish or overflow among them."""
+    torch = _torch()
+    rng = np.random.default_rng(5)
+    dt, code = P.kinds()[wkind]
+    low, high = {"f32": (-149, 125), "f16": (-24, 12), "bf16": (-133, 125)}[wkind]
+    seg, n = 64, 4 * (high - low)
+    m = 2 * seg + 32
+    exponent = low + (np.arange(n) % (high - low))
+    s = P.round_to((1 + rng.random(n)), skind) * 2.0 ** exponent                      # a scale with all its bits
+    steps = rng.integers(-15, 15, (n, m)) / 2 if not zeros else rng.integers(-10, 20, (n, m)) / 2
+    w = P.round_to(steps * s[:, None], wkind)
+    t = torch.from_numpy(w).to(dt)
+    bits = t.view(torch.int32 if dt == torch.float32 else torch.int16)
+    moved = bits + torch.from_numpy(rng.integers(-1, 2, (n, m))).to(bits.dtype)       # up or down a place
+    w = torch.where((t != 0) & torch.isfinite(moved.view(dt)), moved.view(dt), t).double().numpy()
+    w[:, 0::seg], w[:, 1::seg] = (7 * s)[:, None], (0 * s)[:, None]                    # where these are the extremes the scale is s
+    if zeros:
+        w[:, 0::seg], w[:, 1::seg] = (10 * s)[:, None], (-5 * s)[:, None]
+    w = P.round_to(w, wkind)
+    w[~np.isfinite(w)] = 0
+    segs = -(-m // seg)
+    ldq = -(-m // 128) * 64
+    W = _dev(w, wkind)
+    codes = torch.zeros((n, ldq), dtype=torch.uint8, device="cuda")
+    scales = torch.zeros((n, segs), dtype=P.kinds()[skind][0], device="cuda")
+    zp = torch.zeros((n, segs), dtype=torch.uint8, device="cuda") if zeros else None
+    assert hy.quantize_w4(code, m, n, W, m, seg, P.kinds()[skind][1], codes, ldq, scales, zp, segs, None, 0) == 0
+    torch.cuda.synchronize()
+    with np.errstate(over="ignore"):
+        want_codes, want_scales, want_zp = P.quantize(w, seg, skind, zeros)
+    assert np.array_equal(_back(scales, segs), want_scales, equal_nan=True)
+    if zeros:
+        assert np.array_equal(zp.cpu().numpy(), want_zp)
+    assert np.array_equal(P.unpack(codes.cpu().numpy(), m), want_codes)
+
+
+@pytest.mark.parametrize("op,rank", [("T", 2), ("N", 0), ("N", 2)])
+def test_product_of_more_vectors_than_one_launch_takes(hy, op, rank):
+    rng = np.random.default_rng(12)
+    m, n, t, kind = (32, 8, (1 << 19) + 300, "bf16") if op == "T" else (8, 32, (1 << 19) + 300, "bf16")
+    codes, scales, zp = _problem(rng, m, n, 32, kind, False)
+    x = P.round_to(rng.standard_normal((t, m if op == "T" else n)), kind)
+    u = P.round_to(0.1 * rng.standard_normal((rank, m)), kind) if rank else None
+    v = P.round_to(rng.standard_normal((rank, n)) / np.sqrt(n), kind) if rank else None
+    got = _run_product(hy, op, m, n, t, kind, 32, codes, scales, zp, x, u, v)
+    _check_product(got, op, m, n, kind, 32, codes, scales, zp, x, u, v)
+
+
+def test_two_threads_on_two_streams(hy):
+    """Two handles used at the same time from two threads give what each gives alone."""
+    import threading
+    torch = _torch()
+    from hyacinth_b200 import api
+    rng = np.random.default_rng(14)
+    m, n, seg, rank, vocab, k = 1024, 512, 64, 8, 9001, 8
+    problems = []
+    for kind in ("bf16", "f16"):
+        dt, code = P.kinds()[kind]
+        W = torch.from_numpy(rng.standard_normal((n, m))).to(dt).cuda()
+        U, V = torch.from_numpy(rng.standard_normal((rank, m)) * 0.1).to(dt).cuda(), torch.from_numpy(rng.standard_normal((rank, n))).to(dt).cuda()
+        xs = [(op, t, torch.from_numpy(rng.standard_normal((t, m if op == "T" else n))).to(dt).cuda()) for op, t in (("T", 1), ("T", 4), ("T", 40), ("N", 3))]
+        Z = torch.from_numpy(3 * rng.standard_normal((6, vocab))).to(dt).cuda()
+        ids = torch.from_numpy(rng.integers(0, vocab, (6, k)).astype(np.int32)).cuda()
+        teacher = torch.from_numpy(rng.standard_normal((6, k))).float().cuda()
+        problems.append((dt, code, W, U, V, xs, Z, ids, teacher))
+    torch.cuda.synchronize()
+
+    def run(problem, repeats, out):
+        dt, code, W, U, V, xs, Z, ids, teacher = problem
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream), api.Hyacin(stream=stream.cuda_stream) as h:
+            for _ in range(repeats):
+                Q = torch.zeros((n, m // 2), dtype=torch.uint8, device="cuda")
+                S = torch.zeros((n, m // seg), dtype=dt, device="cuda")
+                loss = torch.zeros(6, device="cuda")
+                dZ = torch.zeros_like(Z)
+                results = [Q, S, loss, dZ]
+                rc = h.quantize_w4(code, m, n, W, m, seg, code, Q, m // 2, S, None, m // seg, None, 0)
+                for op, t, x in xs:
+                    inn, wide = (m, n) if op == "T" else (n, m)
+                    Y = torch.zeros((t, wide), dtype=dt, device="cuda")
+                    rc |= h.product_w4(op, m, n, t, code, Q, m // 2, seg, S, None, m // seg, x, inn, rank, U, m, V, n, Y, wide)
+                    results.append(Y)
+                rc |= h.distill_loss(code, vocab, 6, Z, vocab, k, ids, teacher, k, 1.5, None, None, loss, None, dZ, vocab)
+                stream.synchronize()
+                out.append((rc, [r.clone() for r in results]))
+            stream.synchronize()
+
+    alone = []
+    for problem in problems:
+        run(problem, 1, alone)
+    together = [[], []]
+    threads = [threading.Thread(target=run, args=(problems[i], 15, together[i])) for i in range(2)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    torch.cuda.synchronize()
+    assert hy.status() == 0
+    for i in range(2):
+        assert alone[i][0] == 0 and len(together[i]) == 15
+        for rc, results in together[i]:
+            assert rc == 0
+            for a, b in zip(alone[i][1], results):
+                assert torch.equal(a, b)
