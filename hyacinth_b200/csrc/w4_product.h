@@ -1,6 +1,7 @@
-// Interfaces between the kernels of hyacinB200ProductW4 (host side).
+// Interfaces between the kernels of hyacinB200ProductW4.
 #pragma once
 #include "w4.cuh"
+#include <cuda.h>
 
 namespace hyb {
 
@@ -12,6 +13,9 @@ struct ProductArgs {
   int rank; const void* first; int64_t ld1; const void* second; int64_t ld2;
   void* y; int64_t ldy;
 };
+
+// The descriptor of a tensor map, a kernel's argument, on its way before the first copy needs it.
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory"); }
 
 // Fifth-generation tensor cores, 16-bit types, both directions.  Returns 0 or -3.
 int32_t launch_product_umma(const hyacinHandle_t* handle, const char* fn, bool trans, hyacinPrecision_t type, const ProductArgs& a);

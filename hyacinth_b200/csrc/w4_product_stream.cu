@@ -144,6 +144,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_stream_kernel(const __gri
     tma_load_2d(smem_u32(ring) + stage * kTile * kColumnPitch, &code_map, &bars->full[stage], chunk * (kColumnPitch / 8), tile * kTile);
   };
   if (threadIdx.x == 0) {
+    prefetch_map(&code_map);
     for (int s = 0; s < p.ring; ++s) { mbar_init(&bars->full[s], 2); mbar_init(&bars->empty[s], kWarps); }
     for (int j = 0; j < kJoints; ++j) { mbar_init(&bars->joint_full[j], kWarps); mbar_init(&bars->joint_empty[j], 1); }
     bars->abort_flag = 0;

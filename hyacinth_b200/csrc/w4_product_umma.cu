@@ -88,18 +88,18 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&v)[32]
 // hardware, and many warps that poll slow the multiplying warp down (a satisfied wait took it 800 cycles with 20 single-lane
 // pollers).  So few warps poll at a time, the ones that run ahead with pauses in between.
 template <bool PAUSE> __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_flag, uint32_t* status, uint32_t code) {
-  bool ok = false;
 #pragma unroll 1
   for (uint32_t it = 0; it < (1u << 20); ++it) {
     uint32_t done;
     asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
                  : "=r"(done) : "r"(smem_u32(bar)), "r"(parity), "r"(20000u) : "memory");
-    if (__all_sync(~0u, done)) { ok = true; break; }
+    if (__all_sync(~0u, done)) return true;
     if (__any_sync(~0u, *abort_flag)) break;
     if (PAUSE) __nanosleep(64);
   }
-  if (!ok && (threadIdx.x & 31) == 0 && !*abort_flag) { *abort_flag = 1u; *reinterpret_cast<volatile uint32_t*>(status) = code; }
-  return __all_sync(~0u, ok);
+  if ((threadIdx.x & 31) == 0 && !*abort_flag) { *abort_flag = 1u; *reinterpret_cast<volatile uint32_t*>(status) = code; }
+  __syncwarp();
+  return false;
 }
 __device__ __forceinline__ bool elect_one() {
   uint32_t r;
@@ -224,6 +224,7 @@ product_umma_kernel(const __grid_constant__ CUtensorMap code_map, const __grid_c
     }
   };
   if (threadIdx.x == 0) {
+    prefetch_map(&code_map); prefetch_map(&x_map);
     for (int s = 0; s < p.ring; ++s) { mbar_init(&bars->full[s], 2); mbar_init(&bars->empty[s], 1); }
     for (int a = 0; a < p.bufs; ++a) mbar_init(&bars->a_full[a], kGroupWarps);
     mbar_init(&bars->done, 1);
