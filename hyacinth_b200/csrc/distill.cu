@@ -14,6 +14,8 @@
 // from DRAM once, with bulk copies, and the gradient is written from there; one exchange of (maximum, sum) per CTA is all the
 // communication.  Slices of at most 72 KiB leave three CTAs per SM, whose loads, arithmetic and stores overlap.
 // distill_plain_kernel (one block per token, passes over global memory) takes rows that do not fit a cluster.
+// Bound: DRAM, less what the phases of a token (copy, maximum, sum, exchange, gradient) leave idle with three CTAs per SM.  512 tokens of
+// 128000 bfloat16 logits, a fifth masked, loss and gradient: 69 us with the launch, 3.4 TB/s; the plain kernel took 590.
 // exp is taken as 2^(z scale - c), scale = log2(e) / tau and c = float(top scale), one fused multiply-add and one ex2 per entry;
 // what rounding c loses, kappa = top scale - c, is known in 64 bits and put back into the sum, so the loss does not see it.
 #include "w4.cuh"

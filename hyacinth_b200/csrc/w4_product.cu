@@ -29,7 +29,8 @@ template <class T> __global__ void __launch_bounds__(256) correction_mid_kernel(
 
 constexpr int kPlainTokens = 4;
 
-// op 'T', plain: one warp per column, the lanes share its words.
+// op 'T', plain: one warp per column, the lanes share its words.  For single-precision x too long for the streaming kernel's shared memory
+// (more than about 20 000 rows) and for sums over nothing.
 template <class T> __global__ void __launch_bounds__(256) product_t_plain_kernel(PlainArgs a) {
   const int lane = threadIdx.x & 31, col = blockIdx.x * 8 + (threadIdx.x >> 5);
   if (col >= a.n) return;
@@ -59,7 +60,7 @@ template <class T> __global__ void __launch_bounds__(256) product_t_plain_kernel
 // op 'N' in single precision (and for 16-bit types when there is nothing to sum): a block of 256 threads takes 128 rows, thread (word,
 // lane) the eight rows of a word in every 16th column, for four vectors at a time; x times the scale is formed once per word.
 // A cluster of up to eight such blocks splits the columns; sums meet in shared memory, in a fixed order.
-// Bound: the floating-point pipe, 8 conversions and 32 multiply-adds per word and four vectors.
+// Bound: the floating-point pipe, 8 conversions and 32 multiply-adds per word and four vectors; 4096 x 4096, four vectors: 24 us.
 constexpr int kSingleLanes = 16, kSingleThreads = 16 * kSingleLanes;
 __device__ __forceinline__ float ld_cluster(const float* at, uint32_t rank) {
   uint32_t remote; float v;

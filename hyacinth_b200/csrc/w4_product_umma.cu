@@ -10,14 +10,19 @@
 //              to six operand buffers: from the dequantised tile to the freed buffer takes some 1700 cycles, several steps' worth.
 // opW 'T': a step is 128 rows of W, a thread owns one output and writes its K values to tensor memory, the A operand of the
 // instruction (an instruction with A in shared memory takes 40 cycles for its 4 KiB however small NT is, from tensor memory
-// 10 to 33).  opW 'N': a step is 64 columns of W; a word of codes is eight consecutive outputs at one K, a 16-byte chunk of an
-// MN-major operand in shared memory.
+// 10 to 33).  opW 'N': a step is 128 columns of W (64 beside tiles of more than 128 tokens); a word of codes is eight consecutive outputs
+// at one K, a 16-byte chunk of an MN-major operand in shared memory.
 // The correction V (U^T X) is two more operands of the same product: K steps whose A tile is V and whose X tile is
 // mid = U^T X, kept as two 16-bit parts (value and remainder), so that it adds no rounding of its own.
 // Few tiles: a cluster of up to 8 CTAs splits the K steps of one tile and adds the partial sums through distributed shared memory
 // in a fixed order.
 // Rounding: s (q - zero) has up to 15 significant bits (8 of s, 5 of q for bfloat16) and is rounded to the operand type, which
 // is what the matrix instruction takes; one half step, independent per weight, of the size of the rounding of Y itself.
+// Bound: the hand-overs between the roles.  A step takes 750 cycles with 32 tokens, of which the dequantising warps fill 250 and the tensor
+// pipe 260, and 1140 with 256, of which the pipe fills 1030; the first step's operand is there after 5700 cycles (copies, scales,
+// dequantising, each behind the other).  Measured, matrices cycled through more than the L2: 4096 x 16384 bfloat16 times 32 tokens 21.3 us
+// (1.7 TB/s), 128 tokens 24.3 us (707 TFLOP/s), 256 tokens 32.7 us (1050 TFLOP/s, 0.66 of measured); half with segments of 64 rows
+// and zero points, opW 'N', 64 tokens 27.0 us.  Without the code stream the first of these takes 1.6 us less, without dequantising 2 us.
 #include "w4_product.h"
 #include "ptx_sm100.cuh"
 #include <algorithm>

