@@ -26,4 +26,7 @@ cudaError_t launch_mid_float(const hyacinHandle_t* handle, hyacinPrecision_t typ
 int product_stream_vectors(hyacinPrecision_t type, const ProductArgs& a);
 int32_t launch_product_stream(const hyacinHandle_t* handle, const char* fn, hyacinPrecision_t type, const ProductArgs& a);
 
+// Single precision, both directions, any size.
+int32_t launch_product_single(const hyacinHandle_t* handle, const char* fn, bool trans, const ProductArgs& a);
+
 }  // namespace hyb
