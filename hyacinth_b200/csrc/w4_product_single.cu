@@ -1,18 +1,21 @@
 // Products with a 4-bit weight matrix in single precision where the streaming kernel does not serve: opW 'N', many vectors, very long x.
 //
-// Y (out x T) = A X, A = Wq^T or Wq, in 32 bits throughout.  A block of 256 threads computes 128 outputs x TOK vectors: steps of 32 along the sum
-// bring the dequantised weights and x to shared memory as floats, a thread holds 8 x TOK / 16 sums.  A step's sums start from
+// Y (out x T) = A X, A = Wq^T or Wq, in 32 bits throughout.  A block of 128 threads computes 128 outputs x TOK vectors: steps of 32 along the sum
+// bring the dequantised weights and x to shared memory as floats, a thread holds 8 x TOK / 8 sums.  A step's sums start from
 // zero and are then added to the total, so no term passes through more than 32 + K / 32 additions.  The next step's words are on their way
 // in registers meanwhile.  The correction V (U^T X) is more steps of the same sum with mid = U^T X as x, and mid itself the same
 // kernel over a plain matrix.  Few tiles: a cluster of up to 8 blocks splits the steps, sums joined in a fixed order.
-// Bound: the floating-point pipe, 128 multiply-adds per clock and SM (72 TFLOP/s at 1.9 GHz).
+// Bound: the floating-point pipe, 128 multiply-adds per clock and SM (72 TFLOP/s at 1.9 GHz), and shared memory beside it: four 16-byte loads, sixteen
+// wavefronts, per 64 multiply-adds of a warp.  8 x 8 sums per thread need half the loads of 8 x 4 (276 -> 236 us below); two blocks per SM
+// leave eight warps to cover what remains.  Measured, 4096 x 4096 with segments of 64 rows: opW 'N', 16 vectors 37 us, 64 64 us, 256 236 us
+// (36 TFLOP/s); opW 'T', 256 vectors 252 us.  Five vectors with the kernel for four, in two passes, would take 42 us.
 #include "w4_product.h"
 #include <algorithm>
 
 namespace hyb {
 namespace {
 
-constexpr int kOut = 128, kStep = 32, kThreads = 256, kPitch = kOut + 4;
+constexpr int kOut = 128, kStep = 32, kThreads = 128, kPitch = kOut + 4;
 enum Mode { kCodesT, kCodesN, kDense };           // weights: Wq^T, Wq, or the transpose of a plain matrix
 
 struct SingleArgs {
@@ -51,44 +54,34 @@ __device__ __forceinline__ Two add2(Two a, Two b) { Two r; asm("add.rn.f32x2 %0,
 __device__ __forceinline__ Two mul2(Two a, Two b) { Two r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v)); return r; }
 
 template <Mode MODE, int TOK> __global__ void __launch_bounds__(kThreads, 2) product_single_kernel(const __grid_constant__ SingleArgs a) {
-  constexpr int kTok = TOK / 16, kXPitch = TOK + 4, kXPer = kStep * TOK / kThreads;       // sums of a thread along the vectors; values of x it brings
+  constexpr int kTok = TOK / 8, kXPitch = TOK + 4, kXPer = kStep * TOK / kThreads;       // sums of a thread along the vectors; values of x it brings
   constexpr int kTiles = kStep * kPitch + kStep * kXPitch, kSums = TOK * kOut;
   __shared__ __align__(16) float smem[kTiles > kSums ? kTiles : kSums];
   float* ws = smem;                                // [k][output]
   float* xs = smem + kStep * kPitch;               // [k][vector]
   const int tid = threadIdx.x, split = blockIdx.x % a.splits, out0 = blockIdx.x / a.splits * kOut;
   const int step0 = int(int64_t(a.steps) * split / a.splits), step1 = int(int64_t(a.steps) * (split + 1) / a.splits);
-  const int o = tid & 127, half = tid >> 7;        // output and half of a step that this thread brings ('T', plain, correction)
-  const int word = tid & 15, lane = tid >> 4;      // 'N': word of the block, column modulo 16
+  const int o = tid;                               // output that this thread brings ('T', plain, correction)
+  const int word = tid & 15, lane = tid >> 4;      // 'N': word of the block, column modulo 8
   const int xt = tid % TOK, xk = tid / TOK * kXPer;
   for (int64_t t0 = int64_t(blockIdx.y) * TOK; t0 < a.t; t0 += int64_t(gridDim.y) * TOK) {
     Two total[4][kTok] = {};
-    uint32_t q[2] = {}; float s[2] = {}; int zero[2] = {}; float dense[16], xv[kXPer];
+    uint32_t q[4] = {}; float s[4] = {}; int zero[4] = {}; float xv[kXPer];
     auto fetch = [&](int k) {
       const bool more = k >= a.code_steps;         // a step of the correction
       const int k0 = (more ? k - a.code_steps : k) * kStep, length = more ? a.rank : a.in;
-      if (more) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int r = k0 + 2 * i + half;
-          dense[i] = r < length && out0 + o < a.out ? now(a.second + r * a.ld2 + out0 + o) : 0.f;
-        }
-      } else if (MODE == kDense) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int r = k0 + 16 * half + i;
-          dense[i] = r < length && out0 + o < a.out ? now(a.second + (out0 + o) * a.ld2 + r) : 0.f;
-        }
+      if (more || MODE == kDense) {                // few of these: read when they are stored
       } else if (MODE == kCodesT) {
         const int col = min(out0 + o, a.n - 1), sub = k, seg = k0 / a.seg;
-        const uint8_t* from = a.codes + col * a.ldq + int64_t(sub >> 2) * 64 + (sub & 3) * 4 + 32 * half;
-        q[0] = now(reinterpret_cast<const uint32_t*>(from)); q[1] = now(reinterpret_cast<const uint32_t*>(from + 16));
+        const uint8_t* from = a.codes + col * a.ldq + int64_t(sub >> 2) * 64 + (sub & 3) * 4;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) q[u] = now(reinterpret_cast<const uint32_t*>(from + 16 * u));
         s[0] = now(a.scales + col * a.lds + seg); zero[0] = a.zeros ? now(a.zeros + col * a.lds + seg) : 8;
       } else {
         const int seg = min(out0 + w4_word_row(word), a.m - 1) / a.seg;
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const int col = min(k0 + lane + 16 * u, a.n - 1);                  // behind the last column x is zero and the weights are not used
+        for (int u = 0; u < 4; ++u) {
+          const int col = min(k0 + lane + 8 * u, a.n - 1);                  // behind the last column x is zero and the weights are not used
           q[u] = now(reinterpret_cast<const uint32_t*>(a.codes + col * a.ldq + int64_t(out0 / kOut) * 64 + word * 4));
           s[u] = now(a.scales + col * a.lds + seg); zero[u] = a.zeros ? now(a.zeros + col * a.lds + seg) : 8;
         }
@@ -106,30 +99,31 @@ template <Mode MODE, int TOK> __global__ void __launch_bounds__(kThreads, 2) pro
     };
     auto store = [&](int k) {
       const bool more = k >= a.code_steps;
-      const int k0 = k * kStep;
-      const float offset[2] = {8388608.f + float(zero[0]), 8388608.f + float(zero[1])};
-      if (more) {
+      const int k0 = (more ? k - a.code_steps : k) * kStep, length = more ? a.rank : a.in;
+      float offset[4];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) ws[(2 * i + half) * kPitch + o] = dense[i];
-      } else if (MODE == kDense) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) ws[(16 * half + i) * kPitch + o] = dense[i];
+      for (int u = 0; u < 4; ++u) offset[u] = 8388608.f + float(zero[MODE == kCodesT ? 0 : u]);
+      if (more || MODE == kDense) {
+        const float* from = more ? a.second + k0 * a.ld2 + out0 + o : a.second + (out0 + o) * a.ld2 + k0;
+        const int64_t pitch = more ? a.ld2 : 1;
+#pragma unroll 16
+        for (int r = 0; r < kStep; ++r) ws[r * kPitch + o] = k0 + r < length && out0 + o < a.out ? __ldg(from + r * pitch) : 0.f;
       } else if (MODE == kCodesT) {
         // rows behind the last one: whatever scale and codes say there, it is not multiplied
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int u = 0; u < 4; ++u)
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            const int r = 16 * half + 8 * u + e;
+            const int r = 8 * u + e;
             ws[r * kPitch + o] = k0 + r < a.in ? s[0] * code(q[u], e, offset[0]) : 0.f;
           }
       } else {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
+        for (int u = 0; u < 4; ++u) {
           float w[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) w[e] = k0 + lane + 16 * u < a.in ? s[u] * code(q[u], e, offset[u]) : 0.f;
-          float4* to = reinterpret_cast<float4*>(ws + (lane + 16 * u) * kPitch + w4_word_row(word));
+          for (int e = 0; e < 8; ++e) w[e] = k0 + lane + 8 * u < a.in ? s[u] * code(q[u], e, offset[u]) : 0.f;
+          float4* to = reinterpret_cast<float4*>(ws + (lane + 8 * u) * kPitch + w4_word_row(word));
           to[0] = make_float4(w[0], w[1], w[2], w[3]); to[1] = make_float4(w[4], w[5], w[6], w[7]);
         }
       }
@@ -150,12 +144,15 @@ template <Mode MODE, int TOK> __global__ void __launch_bounds__(kThreads, 2) pro
         const ulonglong2 w0 = *reinterpret_cast<const ulonglong2*>(ws + r * kPitch + 4 * ox), w1 = *reinterpret_cast<const ulonglong2*>(ws + r * kPitch + 64 + 4 * ox);
         const Two w[4] = {{w0.x}, {w0.y}, {w1.x}, {w1.y}};
         Two x[kTok];
-        if constexpr (kTok == 4) {
-          const float4 v = *reinterpret_cast<const float4*>(xs + r * kXPitch + 4 * og);
-          x[0] = two(v.x, v.x); x[1] = two(v.y, v.y); x[2] = two(v.z, v.z); x[3] = two(v.w, v.w);
-        } else {
+        if constexpr (kTok % 4 == 0) {
 #pragma unroll
-          for (int j = 0; j < kTok; ++j) { const float v = xs[r * kXPitch + kTok * og + j]; x[j] = two(v, v); }
+          for (int j = 0; j < kTok; j += 4) {
+            const float4 v = *reinterpret_cast<const float4*>(xs + r * kXPitch + kTok * og + j);
+            x[j] = two(v.x, v.x); x[j + 1] = two(v.y, v.y); x[j + 2] = two(v.z, v.z); x[j + 3] = two(v.w, v.w);
+          }
+        } else {
+          const float2 v = *reinterpret_cast<const float2*>(xs + r * kXPitch + kTok * og);
+          x[0] = two(v.x, v.x); x[1] = two(v.y, v.y);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -200,8 +197,8 @@ template <Mode MODE, int TOK> __global__ void __launch_bounds__(kThreads, 2) pro
   }
 }
 
-// Few vectors, opW 'N': a block of 256 threads takes 128 rows, thread (word, lane) the eight rows of a word in every 16th column, for four
-// vectors at a time; x times the scale is formed once per word.  A cluster of up to eight such blocks splits the columns; sums meet
+// Few vectors, opW 'N': a block of 256 threads takes 128 rows, thread (word, lane) the eight rows of a word in every 16th column, for up to
+// four vectors; x times the scale is formed once per word.  A cluster of up to eight such blocks splits the columns; sums meet
 // in shared memory, in a fixed order.
 // Bound: the floating-point pipe, 8 conversions and 32 multiply-adds per word and four vectors; 4096 x 4096, four vectors: 24 us.
 constexpr int kFew = 4, kFewLanes = 16, kFewThreads = 16 * kFewLanes;
@@ -220,52 +217,50 @@ __global__ void __launch_bounds__(kFewThreads) product_few_kernel(const __grid_c
   const float* scales = a.scales + seg;
   const uint8_t* zeros = a.zeros ? a.zeros + seg : nullptr;
   const uint8_t* codes = a.codes + int64_t(block) * 64 + word * 4;
-  for (int64_t t0 = int64_t(blockIdx.y) * kFew; t0 < a.t; t0 += int64_t(gridDim.y) * kFew) {
-    float acc[kFew][8] = {};
+  float acc[kFew][8] = {};
 #pragma unroll 4
-    for (int j = j0 + lane; j < j1; j += kFewLanes) {
-      const uint32_t q = __ldg(reinterpret_cast<const uint32_t*>(codes + j * a.ldq));
-      const float s = scales[j * a.lds], offset = 8388608.f + float(zeros ? int(zeros[j * a.lds]) : 8);
-      float xs[kFew], w[8];
+  for (int j = j0 + lane; j < j1; j += kFewLanes) {
+    const uint32_t q = __ldg(reinterpret_cast<const uint32_t*>(codes + j * a.ldq));
+    const float s = scales[j * a.lds], offset = 8388608.f + float(zeros ? int(zeros[j * a.lds]) : 8);
+    float xs[kFew], w[8];
 #pragma unroll
-      for (int t = 0; t < kFew; ++t) xs[t] = t0 + t < a.t ? s * x[(t0 + t) * a.ldx + j] : 0.f;
+    for (int t = 0; t < kFew; ++t) xs[t] = t < a.t ? s * x[t * a.ldx + j] : 0.f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) w[e] = __uint_as_float(((q >> (4 * w4_row_nibble(e))) & 15u) | 0x4b000000u) - offset;      // 2^23 + q, exact
-#pragma unroll
-      for (int t = 0; t < kFew; ++t)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) acc[t][e] += w[e] * xs[t];
-    }
+    for (int e = 0; e < 8; ++e) w[e] = __uint_as_float(((q >> (4 * w4_row_nibble(e))) & 15u) | 0x4b000000u) - offset;      // 2^23 + q, exact
 #pragma unroll
     for (int t = 0; t < kFew; ++t)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) red[t][e][word][lane] = acc[t][e];
-    __syncthreads();
-    for (int i = threadIdx.x; i < kFew * kW4Block; i += kFewThreads) {
-      const int t = i / kW4Block, r = i % kW4Block, e = r & 7, w = r >> 3;
-      float v = 0.f;
-#pragma unroll
-      for (int l = 0; l < kFewLanes; ++l) v += red[t][e][w][l];
-      sum[t][w4_word_row(w) + e] = v;
-    }
-    if (a.splits > 1) cluster_sync_all(); else __syncthreads();
-    const int share = kW4Block / a.splits;
-    for (int i = threadIdx.x; i < kFew * share; i += kFewThreads) {
-      const int t = i / share, local = split * share + i % share, out = block * kW4Block + local;
-      if (out >= a.m || t0 + t >= a.t) continue;
-      float v = 0.f;
-      for (int c = 0; c < a.splits; ++c) v += a.splits > 1 ? ld_cluster(&sum[t][local], c) : sum[t][local];
-      for (int k = 0; k < a.rank; ++k) v += a.second[k * a.ld2 + out] * a.mid[(t0 + t) * a.rank + k];
-      a.y[(t0 + t) * a.ldy + out] = v;
-    }
-    if (a.splits > 1) cluster_sync_all(); else __syncthreads();
+      for (int e = 0; e < 8; ++e) acc[t][e] += w[e] * xs[t];
   }
+#pragma unroll
+  for (int t = 0; t < kFew; ++t)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) red[t][e][word][lane] = acc[t][e];
+  __syncthreads();
+  for (int i = threadIdx.x; i < kFew * kW4Block; i += kFewThreads) {
+    const int t = i / kW4Block, r = i % kW4Block, e = r & 7, w = r >> 3;
+    float v = 0.f;
+#pragma unroll
+    for (int l = 0; l < kFewLanes; ++l) v += red[t][e][w][l];
+    sum[t][w4_word_row(w) + e] = v;
+  }
+  if (a.splits > 1) cluster_sync_all(); else __syncthreads();
+  const int share = kW4Block / a.splits;
+  for (int i = threadIdx.x; i < kFew * share; i += kFewThreads) {
+    const int t = i / share, local = split * share + i % share, out = block * kW4Block + local;
+    if (out >= a.m || t >= a.t) continue;
+    float v = 0.f;
+    for (int c = 0; c < a.splits; ++c) v += a.splits > 1 ? ld_cluster(&sum[t][local], c) : sum[t][local];
+    for (int k = 0; k < a.rank; ++k) v += a.second[k * a.ld2 + out] * a.mid[t * a.rank + k];
+    a.y[t * a.ldy + out] = v;
+  }
+  if (a.splits > 1) cluster_sync_all();            // shared memory stays until every peer has read it
 }
 
 template <Mode MODE, int TOK> cudaError_t start(const hyacinHandle_t* handle, SingleArgs a) {
   a.code_steps = int((int64_t(a.in) + kStep - 1) / kStep); a.steps = a.code_steps + (a.rank + kStep - 1) / kStep;
   const int64_t tiles = (int64_t(a.out) + kOut - 1) / kOut, groups = std::min<int64_t>((int64_t(a.t) + TOK - 1) / TOK, 65535);
-  a.splits = 1;                                    // two blocks fit an SM; at least four steps for each
+  a.splits = 1;                                    // two blocks fit an SM; at least four steps for each block
   while (a.splits < 8 && tiles * groups * a.splits * 2 <= 2 * int64_t(handle->DeviceSMs) && a.steps >= 8 * a.splits) a.splits *= 2;
   a.x_aligned = reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && a.ldx % 4 == 0;
   cudaLaunchConfig_t cfg{};
@@ -277,11 +272,11 @@ template <Mode MODE, int TOK> cudaError_t start(const hyacinHandle_t* handle, Si
   return cudaLaunchKernelEx(&cfg, product_single_kernel<MODE, TOK>, a);
 }
 cudaError_t start_few(const hyacinHandle_t* handle, SingleArgs a) {
-  const int64_t blocks = (int64_t(a.m) + kOut - 1) / kOut, groups = (a.t + kFew - 1) / kFew;
+  const int64_t blocks = (int64_t(a.m) + kOut - 1) / kOut;
   a.splits = 1;
-  while (a.splits < 8 && blocks * groups * a.splits < 4 * int64_t(handle->DeviceSMs) && a.splits * 2 * kFewLanes <= a.n) a.splits *= 2;
+  while (a.splits < 8 && blocks * a.splits < 4 * int64_t(handle->DeviceSMs) && a.splits * 2 * kFewLanes <= a.n) a.splits *= 2;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(unsigned(blocks * a.splits), unsigned(groups)); cfg.blockDim = dim3(kFewThreads); cfg.stream = handle->cudaStream;
+  cfg.gridDim = dim3(unsigned(blocks * a.splits)); cfg.blockDim = dim3(kFewThreads); cfg.stream = handle->cudaStream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension; attr[0].val.clusterDim.x = a.splits; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr; cfg.numAttrs = a.splits > 1 ? 1 : 0;
@@ -310,7 +305,7 @@ int32_t launch_product_single(const hyacinHandle_t* handle, const char* fn, bool
     e = start_for<kDense>(handle, b);
     a.rank = p.rank; a.second = static_cast<const float*>(p.second); a.ld2 = p.ld2; a.mid = mid;
   }
-  if (e == cudaSuccess) e = trans ? start_for<kCodesT>(handle, a) : p.t <= 2 * kFew ? start_few(handle, a) : start_for<kCodesN>(handle, a);
+  if (e == cudaSuccess) e = trans ? start_for<kCodesT>(handle, a) : p.t <= kFew ? start_few(handle, a) : start_for<kCodesN>(handle, a);
   if (mid) HYB_CUDA(cudaFreeAsync(mid, stream));
   if (e != cudaSuccess) { report_cuda_error(e, fn, __FILE__, __LINE__); return -3; }
   return w4_launched(fn);

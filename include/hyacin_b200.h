@@ -173,9 +173,9 @@ int32_t hyacinB200QuantizeW4(const hyacinHandle_t* handle, hyacinPrecision_t Wty
 
 /* opW 'T': Y (N x T) = Wq^T X + V (U^T X), X (M x T).   opW 'N': Y (M x T) = Wq X + U (V^T X), X (N x T), the gradient of
  * the former to its input.  U is M x rank, V is N x rank; rank 0 leaves the correction out.  scales, X, Y, U and V have type
- * Xtype.  Any T >= 0; made for few vectors.  Sums are held in 32 bits and Y is rounded once.  The 16-bit types round the
- * scaled weights to 16 bits before the product for opW 'N' and, but for some scale tables, for T > 8; single precision is made for up to
- * five vectors a pass.  rank <= 2^20. */
+ * Xtype.  Any T >= 0.  Sums are held in 32 bits and Y is rounded once.  The 16-bit types round the
+ * scaled weights to 16 bits before the product for opW 'N' and, but for some scale tables, for T > 8; single precision rounds
+ * nothing but its sums.  rank <= 2^20. */
 int32_t hyacinB200ProductW4(const hyacinHandle_t* handle, char opW, int32_t M, int32_t N, int32_t T, hyacinPrecision_t Xtype,
                             const uint8_t* codes, int64_t ldq, int32_t segM, const void* scales, const uint8_t* zeros, int32_t lds,
                             const void* X, int32_t ldx, int32_t rank, const void* U, int32_t ldu, const void* V, int32_t ldv,

@@ -463,3 +463,19 @@ def test_two_threads_on_two_streams(hy):
             assert rc == 0
             for a, b in zip(alone[i][1], results):
                 assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("op,m,n,t,seg,zeros,rank,pads", [
+    ("T", 33, 1, 25, 32, True, 0, (0, 1, 0)), ("T", 513, 200, 21, 96, False, 33, (1, 3, 1)), ("T", 4096, 300, 64, 128, True, 16, (0, 0, 0)), ("T", 300, 129, 200, 32, False, 0, (0, 0, 0)),
+    ("T", 2000, 127, 70, 64, True, 40, (1, 1, 0)), ("N", 1, 40, 5, 32, False, 1, (0, 0, 0)), ("N", 129, 33, 16, 64, True, 0, (1, 1, 0)), ("N", 300, 2000, 65, 32, True, 50, (0, 2, 2)),
+    ("N", 1000, 31, 130, 256, False, 7, (0, 1, 3)), ("N", 128, 4100, 17, 128, True, 0, (0, 0, 0)), ("N", 5000, 64, 4, 64, True, 2, (0, 0, 1)), ("T", 40000, 20, 3, 128, False, 5, (0, 0, 0)),
+])
+def test_single_precision_of_many_vectors(hy, op, m, n, t, seg, zeros, rank, pads):
+    """The tiled kernel: sizes beside its tiles and steps, odd pitches, corrections that end inside a step."""
+    rng = np.random.default_rng(m + n + t)
+    codes, scales, zp = _problem(rng, m, n, seg, "f32", zeros)
+    x = P.round_to(rng.standard_normal((t, m if op == "T" else n)), "f32")
+    u = P.round_to(0.1 * rng.standard_normal((rank, m)), "f32") if rank else None
+    v = P.round_to(rng.standard_normal((rank, n)) / np.sqrt(n), "f32") if rank else None
+    got = _run_product(hy, op, m, n, t, "f32", seg, codes, scales, zp, x, u, v, pads)
+    _check_product(got, op, m, n, "f32", seg, codes, scales, zp, x, u, v)
