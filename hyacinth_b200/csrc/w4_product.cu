@@ -51,8 +51,10 @@ extern "C" int32_t hyacinB200ProductW4(const hyacinHandle_t* handle, char opW, i
   }
   const int per = trans ? product_stream_vectors(Xtype, a) : 0;
   if (Xtype == HYACIN_F32) {
-    // A pass of the streaming kernel over 4096 x 4096 takes 10 us (four vectors), the tiled kernel 37 us for up to 16 vectors, 63 for up to 64.
-    if (per > 0 && T <= 5 * per) return launch_product_stream(handle, fn, Xtype, a);
+    // A pass of the streaming kernel over 4096 x 4096 takes 10 us (four vectors), the tiled kernel 37 us for up to 16 vectors, 49 for up to 32; with
+    // few columns the streaming kernel leaves SMs idle and the tiled one splits the rows (16384 x 200 times 4: 49 against 16 us).
+    const bool filled = N >= (T <= per ? 2 : 8) * handle->DeviceSMs;
+    if (per > 0 && T <= 5 * per && filled) return launch_product_stream(handle, fn, Xtype, a);
     return launch_product_single(handle, fn, trans, a);
   }
   // Up to eight vectors stream (17 against 23 us, 4096 x 16384); up to sixteen where the tensor-core kernel cannot fetch a block's

@@ -7,8 +7,9 @@
 // kernel over a plain matrix.  Few tiles: a cluster of up to 8 blocks splits the steps, sums joined in a fixed order.
 // Bound: the floating-point pipe, 128 multiply-adds per clock and SM (72 TFLOP/s at 1.9 GHz), and shared memory beside it: four 16-byte loads, sixteen
 // wavefronts, per 64 multiply-adds of a warp.  8 x 8 sums per thread need half the loads of 8 x 4 (276 -> 236 us below); two blocks per SM
-// leave eight warps to cover what remains.  Measured, 4096 x 4096 with segments of 64 rows: opW 'N', 16 vectors 37 us, 64 64 us, 256 236 us
-// (36 TFLOP/s); opW 'T', 256 vectors 252 us.  Five vectors with the kernel for four, in two passes, would take 42 us.
+// leave eight warps to cover what remains.  Measured, 4096 x 4096 with segments of 64 rows: opW 'N', 16 vectors 37 us, 32 43 us, 64 64 us,
+// 256 236 us (36 TFLOP/s); opW 'T', 256 vectors 252 us; 200 x 32768 times 32, opW 'N' (two tiles, 1024 steps) 42 us, 263 without the second split.
+// The kernel for few vectors takes 42 us for eight, two passes of it, where this one takes 37.
 #include "w4_product.h"
 #include <algorithm>
 
@@ -24,7 +25,8 @@ struct SingleArgs {
   const float* x; int64_t ldx;
   int rank; const float* second; int64_t ld2; const float* mid;          // second: also the plain matrix
   float* y; int64_t ldy;
-  int code_steps, steps, splits, x_aligned;
+  int code_steps, steps, splits, parts, x_aligned;      // splits: blocks of a cluster, parts: clusters that share a tile's steps
+  float* scratch;                                 // a part's share of Y, [part][vector][output]
 };
 
 __device__ __forceinline__ float4 ld_cluster4(const float* at, uint32_t rank) {
@@ -60,7 +62,10 @@ template <Mode MODE, int TOK> __global__ void __launch_bounds__(kThreads, 2) pro
   float* ws = smem;                                // [k][output]
   float* xs = smem + kStep * kPitch;               // [k][vector]
   const int tid = threadIdx.x, split = blockIdx.x % a.splits, out0 = blockIdx.x / a.splits * kOut;
-  const int step0 = int(int64_t(a.steps) * split / a.splits), step1 = int(int64_t(a.steps) * (split + 1) / a.splits);
+  const int piece = int(blockIdx.z) * a.splits + split, pieces = a.parts * a.splits;
+  const int step0 = int(int64_t(a.steps) * piece / pieces), step1 = int(int64_t(a.steps) * (piece + 1) / pieces);
+  float* y = a.parts > 1 ? a.scratch + int64_t(blockIdx.z) * a.t * a.out : a.y;
+  const int64_t ldy = a.parts > 1 ? a.out : a.ldy;
   const int o = tid;                               // output that this thread brings ('T', plain, correction)
   const int word = tid & 15, lane = tid >> 4;      // 'N': word of the block, column modulo 8
   const int xt = tid % TOK, xk = tid / TOK * kXPer;
@@ -171,8 +176,8 @@ template <Mode MODE, int TOK> __global__ void __launch_bounds__(kThreads, 2) pro
         for (int i = 0; i < 4; ++i) {
           const int out = out0 + 64 * (i >> 1) + 4 * ox + 2 * (i & 1); const int64_t t = t0 + kTok * og + j;
           const float2 v = unpack(total[i][j]);
-          if (out < a.out && t < a.t) a.y[t * a.ldy + out] = v.x;
-          if (out + 1 < a.out && t < a.t) a.y[t * a.ldy + out + 1] = v.y;
+          if (out < a.out && t < a.t) y[t * ldy + out] = v.x;
+          if (out + 1 < a.out && t < a.t) y[t * ldy + out + 1] = v.y;
         }
       continue;
     }
@@ -191,7 +196,7 @@ template <Mode MODE, int TOK> __global__ void __launch_bounds__(kThreads, 2) pro
       if (t >= a.t) continue;
       const float p[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) if (out + i < a.out) a.y[t * a.ldy + out + i] = p[i];
+      for (int i = 0; i < 4; ++i) if (out + i < a.out) y[t * ldy + out + i] = p[i];
     }
     cluster_sync_all();                            // shared memory stays until every peer has read it
   }
@@ -257,19 +262,44 @@ __global__ void __launch_bounds__(kFewThreads) product_few_kernel(const __grid_c
   if (a.splits > 1) cluster_sync_all();            // shared memory stays until every peer has read it
 }
 
+// Y = the sum of the parts, in their order.
+__global__ void __launch_bounds__(256) join_kernel(const float* scratch, int parts, int out, int t, float* y, int64_t ldy) {
+  const int64_t size = int64_t(out) * t, e = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  if (e >= size) return;
+  float v = 0.f;
+#pragma unroll 8
+  for (int p = 0; p < parts; ++p) v += scratch[p * size + e];
+  y[e / out * ldy + e % out] = v;
+}
+
 template <Mode MODE, int TOK> cudaError_t start(const hyacinHandle_t* handle, SingleArgs a) {
   a.code_steps = int((int64_t(a.in) + kStep - 1) / kStep); a.steps = a.code_steps + (a.rank + kStep - 1) / kStep;
   const int64_t tiles = (int64_t(a.out) + kOut - 1) / kOut, groups = std::min<int64_t>((int64_t(a.t) + TOK - 1) / TOK, 65535);
-  a.splits = 1;                                    // two blocks fit an SM; at least four steps for each block
+  // two blocks fit an SM; at least four steps for each block.  Where a cluster of eight leaves most of the GPU idle several share a tile
+  // and a second kernel adds their shares (200 x 32768 times 32, opW 'N': 263 us without).
+  a.splits = a.parts = 1;
   while (a.splits < 8 && tiles * groups * a.splits * 2 <= 2 * int64_t(handle->DeviceSMs) && a.steps >= 8 * a.splits) a.splits *= 2;
+  if (a.splits == 8) a.parts = int(std::max<int64_t>(1, std::min<int64_t>({2 * int64_t(handle->DeviceSMs) / (tiles * groups * 8), a.steps / 32, 64})));
   a.x_aligned = reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && a.ldx % 4 == 0;
+  if (a.parts > 1) {
+    const cudaError_t e = cudaMallocFromPoolAsync(reinterpret_cast<void**>(&a.scratch), size_t(a.parts) * a.t * a.out * sizeof(float), handle->mempool, handle->cudaStream);
+    if (e != cudaSuccess) return e;
+  }
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(unsigned(tiles * a.splits), unsigned(groups)); cfg.blockDim = dim3(kThreads); cfg.stream = handle->cudaStream;
+  cfg.gridDim = dim3(unsigned(tiles * a.splits), unsigned(groups), unsigned(a.parts)); cfg.blockDim = dim3(kThreads); cfg.stream = handle->cudaStream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension; attr[0].val.clusterDim.x = a.splits; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr; cfg.numAttrs = a.splits > 1 ? 1 : 0;
   count_launch();
-  return cudaLaunchKernelEx(&cfg, product_single_kernel<MODE, TOK>, a);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, product_single_kernel<MODE, TOK>, a);
+  if (a.parts > 1) {
+    if (e == cudaSuccess) {
+      count_launch();
+      join_kernel<<<unsigned((int64_t(a.out) * a.t + 255) / 256), 256, 0, handle->cudaStream>>>(a.scratch, a.parts, a.out, a.t, a.y, a.ldy);
+    }
+    HYB_CUDA(cudaFreeAsync(a.scratch, handle->cudaStream));
+  }
+  return e;
 }
 cudaError_t start_few(const hyacinHandle_t* handle, SingleArgs a) {
   const int64_t blocks = (int64_t(a.m) + kOut - 1) / kOut;
@@ -284,7 +314,7 @@ cudaError_t start_few(const hyacinHandle_t* handle, SingleArgs a) {
   return cudaLaunchKernelEx(&cfg, product_few_kernel, a);
 }
 template <Mode MODE> cudaError_t start_for(const hyacinHandle_t* handle, const SingleArgs& a) {
-  return a.t <= 16 ? start<MODE, 16>(handle, a) : start<MODE, 64>(handle, a);
+  return a.t <= 16 ? start<MODE, 16>(handle, a) : a.t <= 32 ? start<MODE, 32>(handle, a) : start<MODE, 64>(handle, a);
 }
 
 }  // namespace
@@ -305,7 +335,7 @@ int32_t launch_product_single(const hyacinHandle_t* handle, const char* fn, bool
     e = start_for<kDense>(handle, b);
     a.rank = p.rank; a.second = static_cast<const float*>(p.second); a.ld2 = p.ld2; a.mid = mid;
   }
-  if (e == cudaSuccess) e = trans ? start_for<kCodesT>(handle, a) : p.t <= kFew ? start_few(handle, a) : start_for<kCodesN>(handle, a);
+  if (e == cudaSuccess) e = trans ? start_for<kCodesT>(handle, a) : p.t <= kFew && p.m >= 8 * kOut ? start_few(handle, a) : start_for<kCodesN>(handle, a);
   if (mid) HYB_CUDA(cudaFreeAsync(mid, stream));
   if (e != cudaSuccess) { report_cuda_error(e, fn, __FILE__, __LINE__); return -3; }
   return w4_launched(fn);

@@ -468,6 +468,8 @@ def test_two_threads_on_two_streams(hy):
 @pytest.mark.parametrize("op,m,n,t,seg,zeros,rank,pads", [
     ("T", 33, 1, 25, 32, True, 0, (0, 1, 0)), ("T", 513, 200, 21, 96, False, 33, (1, 3, 1)), ("T", 4096, 300, 64, 128, True, 16, (0, 0, 0)), ("T", 300, 129, 200, 32, False, 0, (0, 0, 0)),
     ("T", 2000, 127, 70, 64, True, 40, (1, 1, 0)), ("N", 1, 40, 5, 32, False, 1, (0, 0, 0)), ("N", 129, 33, 16, 64, True, 0, (1, 1, 0)), ("N", 300, 2000, 65, 32, True, 50, (0, 2, 2)),
+    # few outputs and long sums, which several clusters share
+    ("N", 200, 20000, 31, 32, True, 9, (0, 1, 1)), ("N", 130, 9001, 3, 64, False, 0, (0, 0, 0)), ("T", 20001, 70, 2, 64, True, 12, (1, 1, 1)), ("T", 16384, 129, 40, 128, False, 0, (0, 0, 0)),
     ("N", 1000, 31, 130, 256, False, 7, (0, 1, 3)), ("N", 128, 4100, 17, 128, True, 0, (0, 0, 0)), ("N", 5000, 64, 4, 64, True, 2, (0, 0, 1)), ("T", 40000, 20, 3, 128, False, 5, (0, 0, 0)),
 ])
 def test_single_precision_of_many_vectors(hy, op, m, n, t, seg, zeros, rank, pads):
