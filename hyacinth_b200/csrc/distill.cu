@@ -159,7 +159,7 @@ __device__ __forceinline__ float listed_gradient(const DistillArgs& a, const Lis
 }
 
 template <class T> __global__ void __launch_bounds__(512) distill_plain_kernel(DistillArgs a) {
-  extern __shared__ __align__(16) uint8_t smem[];
+  extern __shared__ __align__(128) uint8_t smem[];
   uint32_t* listed = reinterpret_cast<uint32_t*>(smem + (list_bytes(a.k) + 15) / 16 * 16);
   List s(smem, a.k);
   const T* z_all = static_cast<const T*>(a.z);

@@ -42,7 +42,7 @@ constexpr int kMaxRing = 8;
 constexpr int kSmemLimit = 232448;
 
 struct StreamParams {
-  const uint8_t* codes; int64_t ldq; int m, n, t;
+  int m, n, t;
   const void* scales; const uint8_t* zeros; int64_t lds;
   const void* x; int64_t ldx;
   int rank; const void* second; int64_t ld2; const float* mid;
@@ -525,7 +525,7 @@ int32_t launch_product_stream(const hyacinHandle_t* handle, const char* fn, hyac
         std::fprintf(stderr, "hyacin-b200: %s: cuTensorMapEncodeTiled failed\n", fn);
         rc = -3; return;
       }
-      p.codes = a.codes; p.ldq = a.ldq; p.scales = a.scales; p.zeros = a.zeros; p.lds = a.lds;
+      p.scales = a.scales; p.zeros = a.zeros; p.lds = a.lds;
       p.x = static_cast<const X*>(a.x) + t0 * a.ldx; p.ldx = a.ldx; p.y = static_cast<X*>(a.y) + t0 * a.ldy; p.ldy = a.ldy;
       p.second = a.second; p.ld2 = a.ld2; p.mid = mid ? mid + t0 * a.rank : nullptr;
       p.status = status_word_device(handle->DeviceID);

@@ -134,3 +134,24 @@ def test_pointers_off_their_boundary_and_sizes_beyond_the_largest_are_refused():
     for bad in (dict(Z=FAKE + 1), dict(ids=FAKE + 2), dict(teacher=FAKE + 2), dict(lse=FAKE + 1), dict(weight=FAKE + 2), dict(stats=FAKE + 2), dict(dZ=FAKE + 4097, lddz=100)):
         assert _loss(**bad) == -1 and _grad(**bad) == -1
     assert _loss(loss=FAKE + 2) == -1
+
+
+def test_refusals_name_their_reason(capfd):
+    """Each refusal comes from the check of that argument, not from the last one (the handle's device), which stops every call here."""
+    def message(call, bad):
+        capfd.readouterr()
+        assert call(**bad) == -1
+        return capfd.readouterr().err
+
+    marks = {f: [m for m in f.pytestmark if m.name == "parametrize"][0].args[1] for f in (test_quantize_refuses, test_product_refuses)}
+    calls = [(_quantize, bad) for bad in marks[test_quantize_refuses]] + [(_product, bad) for bad in marks[test_product_refuses]]
+    calls += [(call, bad) for bad in DISTILL_BAD for call in (_loss, _grad)] + [(_grad, dict(stats=None)), (_quantize, dict(W=FAKE + 2)), (_product, dict(rank=(1 << 20) + 1))]
+    for call, bad in calls:
+        err = message(call, bad)
+        if bad in (dict(stats=None),):               # found after the device
+            continue
+        assert "hyacinB200" in err and "another device" not in err, (call.__name__, bad, err)
+    import os
+    if not os.path.exists("/dev/nvidiactl"):         # no GPU: the calls that are in order get as far as the device
+        for call in (_quantize, _product, _loss, _grad):
+            assert "another device" in message(call, {})

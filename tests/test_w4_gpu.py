@@ -481,3 +481,67 @@ def test_single_precision_of_many_vectors(hy, op, m, n, t, seg, zeros, rank, pad
     v = P.round_to(rng.standard_normal((rank, n)) / np.sqrt(n), "f32") if rank else None
     got = _run_product(hy, op, m, n, t, "f32", seg, codes, scales, zp, x, u, v, pads)
     _check_product(got, op, m, n, "f32", seg, codes, scales, zp, x, u, v)
+
+
+def test_a_handle_of_another_device_is_refused(hy):
+    torch = _torch()
+    from hyacinth_b200 import api
+    W = torch.ones((4, 128), device="cuda")
+    Q, S = torch.zeros((4, 64), dtype=torch.uint8, device="cuda"), torch.zeros((4, 1), device="cuda")
+    Y, loss = torch.zeros((1, 4), device="cuda"), torch.zeros(1, device="cuda")
+    with api.Hyacin(stream=torch.cuda.current_stream().cuda_stream) as h:
+        own = h.h.DeviceID
+        h.h.DeviceID = own + 1
+        try:
+            assert h.quantize_w4(api.F32, 128, 4, W, 128, 128, api.F32, Q, 64, S, None, 1, None, 0) == -1
+            assert h.product_w4("T", 128, 4, 1, api.F32, Q, 64, 128, S, None, 1, W, 128, 0, None, 0, None, 0, Y, 4) == -1
+            assert h.distill_loss(api.F32, 4, 1, Y, 4, 0, None, None, 0, 1.0, None, None, loss, None, None, 0) == -1
+        finally:
+            h.h.DeviceID = own
+        assert h.quantize_w4(api.F32, 128, 4, W, 128, 128, api.F32, Q, 64, S, None, 1, None, 0) == 0
+    torch.cuda.synchronize()
+    assert torch.equal(S, torch.full_like(S, float(np.float32(1) / np.float32(7))))
+
+
+@pytest.mark.parametrize("op,m,n,t", [("N", 130, 9001, 3), ("N", 130, 9001, 40), ("T", 9001, 130, 5), ("N", 2000, 300, 2)])
+def test_single_precision_captured_and_replayed(op, m, n, t):
+    """Its scratch (mid, the shares of several clusters) in two graphs that are replayed on two streams at once."""
+    torch = _torch()
+    from hyacinth_b200 import api
+    rng = np.random.default_rng(t)
+    rank = 4
+    codes, scales, _ = _problem(rng, m, n, 64, "f32", False)
+    inn, out = (m, n) if op == "T" else (n, m)
+    ldq = -(-m // 128) * 64
+    Q, S = torch.from_numpy(P.pack(codes, ldq)).cuda(), _dev(scales, "f32")
+    u, v = P.round_to(0.1 * rng.standard_normal((rank, m)), "f32"), P.round_to(0.1 * rng.standard_normal((rank, n)), "f32")
+    U, V = _dev(u, "f32"), _dev(v, "f32")
+    xs = [P.round_to(rng.standard_normal((t, inn)), "f32") for _ in range(2)]
+    X, Y = [_dev(x, "f32") for x in xs], [torch.zeros((t, out), device="cuda") for _ in range(2)]
+    torch.cuda.synchronize()
+    streams, handles, graphs = [torch.cuda.Stream() for _ in range(2)], [], []
+    for i in range(2):
+        h = api.Hyacin(stream=streams[i].cuda_stream)
+        handles.append(h)
+
+        def call():
+            assert h.product_w4(op, m, n, t, api.F32, Q, ldq, 64, S, None, S.shape[1], X[i], inn, rank, U, m, V, n, Y[i], out) == 0
+        with torch.cuda.stream(streams[i]):
+            call()
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=streams[i]):
+                call()
+            graphs.append(g)
+    for _ in range(5):
+        for y in Y:
+            y.zero_()
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for i in range(2):
+            _check_product(_back(Y[i], out), op, m, n, "f32", 64, codes, scales, None, xs[i], u, v)
+    del graphs, g
+    for h in handles:
+        h.destroy()
