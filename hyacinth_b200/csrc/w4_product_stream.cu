@@ -19,7 +19,8 @@
 // Bound.  DRAM, at 23 bytes per clock and SM: 710 cycles for a stage of 16 KiB, for which the extraction takes 450 cycles of the
 // integer pipe (7 instructions per eight codes at half rate) and the matrix pipe 256 per eight vectors.  Measured, matrices cycled
 // through more than the L2: bfloat16 4096 x 16384, one vector 14.7 us (2.4 TB/s), eight 17.1 us; half 8192 x 16384 with zero points for
-// every 64 rows 25.6 us (2.9 TB/s; the integer pipe is the busiest, 54 % of the issue slots used); 4096 x 4096 6.4 us, of which a start
+// every 64 rows 25.6 us (2.9 TB/s; 54 % of the issue slots used; two instructions less per word, with the nibbles of the second and
+// fourth pair left in place, made it 26.5); 4096 x 4096 6.4 us, of which a start
 // from nothing (launch, x and its sums, the first copies) takes four.
 #include "w4_product.h"
 #include "ptx_sm100.cuh"
