@@ -35,6 +35,9 @@ __host__ __device__ inline int w4_word_row(int word) { return 32 * (word & 3) + 
 __host__ __device__ inline int w4_nibble_row(int nibble) { return 2 * (nibble & 3) + (nibble >> 2); }  // within the word
 __host__ __device__ inline int w4_row_nibble(int row8) { return (row8 >> 1) + 4 * (row8 & 1); }
 
+// Segments of a column of m rows.  The sum before the division passes 2^31 when seg is near its upper end ("one scale per column").
+__host__ __device__ inline int w4_segments(int m, int seg) { return int((int64_t(m) + seg - 1) / seg); }
+
 // ---- argument checks -----------------------------------------------------------------------------------------
 inline int32_t w4_refuse(const char* fn, const char* why) {
   std::fprintf(stderr, "hyacin-b200: %s: %s\n", fn, why);

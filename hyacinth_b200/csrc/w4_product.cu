@@ -34,7 +34,7 @@ extern "C" int32_t hyacinB200ProductW4(const hyacinHandle_t* handle, char opW, i
   if (in > 0) {
     if (!X || ldx < in) return w4_refuse(fn, "X: null or leading dimension too small");
     if (!codes || !scales) return w4_refuse(fn, "null pointer");
-    if (lds < (int64_t(M) + segM - 1) / segM) return w4_refuse(fn, "lds too small");
+    if (lds < w4_segments(M, segM)) return w4_refuse(fn, "lds too small");
     if (ldq % 16 || ldq < (int64_t(M) + 127) / 128 * 64 || reinterpret_cast<uintptr_t>(codes) % 16) return w4_refuse(fn, "codes: 16-byte aligned, ldq a multiple of 16 and at least 64 ceil(M / 128)");
     if (rank > 0 && (!U || !V || ldu < M || ldv < N)) return w4_refuse(fn, "U, V: null or leading dimension too small");
   }

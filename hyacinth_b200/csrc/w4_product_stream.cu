@@ -485,7 +485,7 @@ int layout(StreamParams& p, hyacinPrecision_t type, int tiles) {
 // Geometry for `vectors` vectors; returns the shared memory, or 0 when they do not fit.  A long x may need the form with smaller stages.
 int place(StreamParams& p, hyacinPrecision_t type, const ProductArgs& a, int vectors) {
   p.t = vectors; p.cols = vectors * parts(type); p.rank = a.rank; p.m = a.m; p.n = a.n;
-  p.segs = (a.m + a.seg - 1) / a.seg; p.seg_sub = a.seg / 32; p.seg_shift = -1;
+  p.segs = w4_segments(a.m, a.seg); p.seg_sub = a.seg / 32; p.seg_shift = -1;
   for (int s = 0; s < 27; ++s) if (p.seg_sub == 1 << s) p.seg_shift = s;
   p.blocks = (a.m + kW4Block - 1) / kW4Block;
   int bytes = p.cols <= 8 ? layout(p, type, 1) : 0;

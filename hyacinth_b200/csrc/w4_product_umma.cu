@@ -694,7 +694,7 @@ template <class T, bool TRANS, int STEP> int32_t launch(const hyacinHandle_t* ha
   }
   UmmaParams p{};
   p.scales = a.scales; p.zeros = a.zeros; p.lds = a.lds; p.m = a.m; p.n = a.n; p.t = a.t; p.out = out;
-  p.segs = (a.m + a.seg - 1) / a.seg; p.seg_sub = a.seg / 32; p.seg_shift = -1;
+  p.segs = w4_segments(a.m, a.seg); p.seg_sub = a.seg / 32; p.seg_shift = -1;
   for (int s = 0; s < 27; ++s) if (p.seg_sub == 1 << s) p.seg_shift = s;
   // two or four segments per block of 128 rows, fetched at once where the table's rows allow it
   const int per_block = p.seg_sub == 1 ? 4 : p.seg_sub == 2 ? 2 : 1;

@@ -266,7 +266,7 @@ extern "C" int32_t hyacinB200QuantizeW4(const hyacinHandle_t* handle, hyacinPrec
   if (M < 0 || N < 0 || segM <= 0 || segM % 32) return w4_refuse(fn, "sizes: M, N >= 0 and segM a positive multiple of 32");
   if (M > 0x7fffff00 || N > 0x7fffff00) return w4_refuse(fn, "sizes: M, N at most 2^31 - 256");
   if (M == 0 || N == 0) return 0;
-  const int segs = (int64_t(M) + segM - 1) / segM;
+  const int segs = w4_segments(M, segM);
   if (!W || !codes || !scales) return w4_refuse(fn, "null pointer");
   if (ldw < M || lds < segs || (R && ldr < M)) return w4_refuse(fn, "leading dimension too small");
   if (ldq % 16 || ldq < (int64_t(M) + 127) / 128 * 64 || reinterpret_cast<uintptr_t>(codes) % 16) return w4_refuse(fn, "codes: 16-byte aligned, ldq a multiple of 16 and at least 64 ceil(M / 128)");
