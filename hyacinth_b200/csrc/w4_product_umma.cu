@@ -12,8 +12,10 @@
 // instruction (an instruction with A in shared memory takes 40 cycles for its 4 KiB however small NT is, from tensor memory
 // 10 to 33).  opW 'N': a step is 128 columns of W (64 beside tiles of more than 128 tokens); a word of codes is eight consecutive outputs
 // at one K, a 16-byte chunk of an MN-major operand in shared memory.
-// The correction V (U^T X) is two more operands of the same product: K steps whose A tile is V and whose X tile is
-// mid = U^T X, kept as two 16-bit parts (value and remainder), so that it adds no rounding of its own.
+// The correction V (U^T X) is two more operands of the same product: K steps whose A tile is V and whose X tile is mid = U^T X, both in
+// bfloat16 parts, whose exponents hold every 32-bit mid (a half ends at 65504 and loses small remainders).  bfloat16: mid in two
+// parts, value and remainder, 16 bits, 2^-8 of the rounding of Y.  Half: V in two parts, exact, mid in three, all of its 24 bits; of
+// their six products the last, 2^-24, is left out.
 // Few tiles: a cluster of up to 8 CTAs splits the K steps of one tile and adds the partial sums through distributed shared memory
 // in a fixed order.
 // Rounding: s (q - zero) has up to 15 significant bits (8 of s, 5 of q for bfloat16) and is rounded to the operand type, which
@@ -27,6 +29,7 @@
 #include "ptx_sm100.cuh"
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 namespace hyb {
 namespace {
@@ -57,9 +60,9 @@ struct UmmaParams {
   int segs, seg_sub, seg_shift;                   // 32-row subsets per segment; shift when that is a power of two, else -1
   int wide;                                       // segments of a block that one aligned load fetches (1, 2, 4)
   int code_steps, steps;                          // K steps of codes, and with those of the correction
-  int rank, rank16; const void* second; int64_t ld2;      // rank16: rank rounded up to 16, the width of either part of mid
+  int rank, rank16; const void* second; int64_t ld2;      // rank16: rank rounded up to 16, the width of a part of mid
   void* y; int64_t ldy;
-  int nt, ring, bufs, groups, splits, second_aligned; uint32_t nt_cols, tmem_cols, idesc;
+  int nt, ring, bufs, groups, splits, second_aligned; uint32_t nt_cols, tmem_cols, idesc, idesc_more;      // idesc_more: of the correction
   uint32_t* status;
 };
 
@@ -192,6 +195,22 @@ template <> struct Scale<__nv_bfloat16> {
   }
 };
 
+// Parts of the correction's operands, the same K range after another: with mid part i (i < mid) V, or what of it is left beyond
+// bfloat16 with part i - mid.
+template <class T> struct Parts { static constexpr bool split = std::is_same<T, __half>::value; static constexpr int mid = split ? 3 : 2, all = split ? 5 : 2; };
+// Eight halves as bfloat16: the nearest, or what it leaves (3 bits, exact).
+__device__ __forceinline__ uint4 factor_part(const uint4& v, bool rest) {
+  uint32_t o[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&o[i]));
+    __nv_bfloat162 b = __floats2bfloat162_rn(f.x, f.y);
+    if (rest) b = __floats2bfloat162_rn(fabsf(f.x) <= 65504.f ? f.x - __low2float(b) : 0.f, fabsf(f.y) <= 65504.f ? f.y - __high2float(b) : 0.f);
+    o[i] = *reinterpret_cast<const uint32_t*>(&b);
+  }
+  return make_uint4(o[0], o[1], o[2], o[3]);
+}
+
 template <class T, bool TRANS, int STEP>
 __global__ void __launch_bounds__(kThreads, 1)
 product_umma_kernel(const __grid_constant__ CUtensorMap code_map, const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap mid_map,
@@ -275,13 +294,13 @@ product_umma_kernel(const __grid_constant__ CUtensorMap code_map, const __grid_c
       tc_fence_after();
       const uint32_t sx = x_ring + stage * x_bytes, ta = tmem + p.nt_cols + buf * G::operand_cols;
       const uint64_t a0 = operand_desc(operand + buf * G::operand_bytes, G::operand_bytes / 2), b0 = operand_desc(sx, 16);
-      const uint32_t b_half = x_bytes / 32;
+      const uint32_t b_half = x_bytes / 32, idesc = Parts<T>::split && k >= p.code_steps ? p.idesc_more : p.idesc;
       if (elect_one()) {
 #pragma unroll
         for (int q = 0; q < kStep / 16; ++q) {
           const uint64_t bd = b0 + ((q >> 2) * b_half + (q & 3) * 2);
-          if (TRANS) umma_f16_ts(tmem, ta + q * 8, bd, p.idesc, (k > step0 || q > 0) ? 1u : 0u);
-          else umma_f16(tmem, a0 + q * 128, bd, p.idesc, (k > step0 || q > 0) ? 1u : 0u);
+          if (TRANS) umma_f16_ts(tmem, ta + q * 8, bd, idesc, (k > step0 || q > 0) ? 1u : 0u);
+          else umma_f16(tmem, a0 + q * 128, bd, idesc, (k > step0 || q > 0) ? 1u : 0u);
         }
         umma_commit(&bars->empty[stage]);
       }
@@ -438,7 +457,7 @@ product_umma_kernel(const __grid_constant__ CUtensorMap code_map, const __grid_c
           }
         }
       } else {
-        // correction step: entry (output, c) of the operand is second(output, c mod rank16), c < 2 rank16; mid is zero behind the rank
+        // correction step: entry (output, c) of the operand is second(output, c mod rank16), c < Parts::all rank16; mid is zero behind the rank
         const uint16_t* second = static_cast<const uint16_t*>(p.second);
         const int c0 = (k - p.code_steps) * kStep;
         if constexpr (TRANS) {
@@ -452,10 +471,14 @@ product_umma_kernel(const __grid_constant__ CUtensorMap code_map, const __grid_c
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               const int e = (id & 127) + 128 * i, chunk = e & 15;
-              int a = c + (e >> 4);
-              if (a >= 2 * p.rank16) a -= 2 * p.rank16;
-              if (a >= p.rank16) a -= p.rank16;
-              v[i] = load8(reinterpret_cast<const T*>(from + int64_t(a) * p.ld2) + chunk * 8, a < p.rank ? valid - chunk * 8 : 0, p.second_aligned != 0);
+              int a = c + (e >> 4), part = 0;
+              if (Parts<T>::split) { part = a / p.rank16; a -= part * p.rank16; }
+              else {
+                if (a >= 2 * p.rank16) a -= 2 * p.rank16;
+                if (a >= p.rank16) a -= p.rank16;
+              }
+              v[i] = load8(reinterpret_cast<const T*>(from + int64_t(a) * p.ld2) + chunk * 8, a < p.rank && part < Parts<T>::all ? valid - chunk * 8 : 0, p.second_aligned != 0);
+              if (Parts<T>::split) v[i] = factor_part(v[i], part >= Parts<T>::mid);
             }
             group_sync();
 #pragma unroll
@@ -469,7 +492,7 @@ product_umma_kernel(const __grid_constant__ CUtensorMap code_map, const __grid_c
               to[e] = uint32_t(lo) | uint32_t(hi) << 16;
             }
           };
-          if (p.rank16 <= 64 && 64 % p.rank16 == 0) {                // the pattern repeats every 64 columns
+          if (!Parts<T>::split && p.rank16 <= 64 && 64 % p.rank16 == 0) {      // the pattern repeats every 64 columns
             gather(0, o);
             if (p.rank16 == 64) gather(32, o + 16);
             else {
@@ -480,18 +503,19 @@ product_umma_kernel(const __grid_constant__ CUtensorMap code_map, const __grid_c
           } else {
 #pragma unroll 1
             for (int pair = 0; pair < 2; ++pair) {
-              const int c = (c0 + pair * 64) % (2 * p.rank16);
-              gather(c, o); gather((c + 32) % (2 * p.rank16), o + 16);
+              const int c = Parts<T>::split ? c0 + pair * 64 : (c0 + pair * 64) % (2 * p.rank16);
+              gather(c, o); gather(Parts<T>::split ? c + 32 : (c + 32) % (2 * p.rank16), o + 16);
               tmem_st32(tdst + pair * 32, o);
             }
           }
         } else {
-          const int c = c0 + row, of = c < p.rank16 ? c : c - p.rank16;
+          const int c = c0 + row, of = Parts<T>::split ? c % p.rank16 : c < p.rank16 ? c : c - p.rank16;
           const uint16_t* from = second + int64_t(of) * p.ld2 + tile * kOut + 64 * half;
-          const int valid = c < 2 * p.rank16 && of < p.rank ? p.out - tile * kOut - 64 * half : 0;
+          const int valid = c < Parts<T>::all * p.rank16 && of < p.rank ? p.out - tile * kOut - 64 * half : 0;
 #pragma unroll 4
           for (int j = 0; j < (kFull ? 16 : 8); ++j) {
-            const uint4 v = load8(reinterpret_cast<const T*>(from) + 8 * j, valid - 8 * j, p.second_aligned != 0);
+            uint4 v = load8(reinterpret_cast<const T*>(from) + 8 * j, valid - 8 * j, p.second_aligned != 0);
+            if (Parts<T>::split) v = factor_part(v, c >= Parts<T>::mid * p.rank16);
             sts128(dst + (half + (j >> 3)) * (G::operand_bytes / 2) + (((j & 7) << 4) ^ swz), v.x, v.y, v.z, v.w);
           }
         }
@@ -548,7 +572,7 @@ product_umma_kernel(const __grid_constant__ CUtensorMap code_map, const __grid_c
   }
 }
 
-// ---- mid = first^T X for many tokens, as two 16-bit parts: [token][value, remainder], each padded with zeros to a multiple of 16 ----------------------
+// ---- mid = first^T X for many tokens, in bfloat16 parts: [token][Parts::all][entry of the rank], each padded with zeros to a multiple of 16 ----------
 template <class T> __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1);
 template <> __device__ __forceinline__ void mma16816<__half>(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -565,7 +589,7 @@ constexpr int kMidWarps = 8, kMidSplits = 8;
 // order of K inside an instruction is free as long as both operands agree.  The product waits for this kernel, so what counts is
 // its latency: 4096 rows, rank 64, 256 tokens took 9 us with one block per tile.
 template <class T> __global__ void __launch_bounds__(kMidWarps * 32)
-mid_split_kernel(const T* first, int64_t ld1, int rows, int rank, const T* x, int64_t ldx, int t, T* mid, int64_t ldm, int aligned, float* mid32) {
+mid_split_kernel(const T* first, int64_t ld1, int rows, int rank, const T* x, int64_t ldx, int t, __nv_bfloat16* mid, int64_t ldm, int aligned, float* mid32) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   __shared__ float red[kMidWarps][16][17];
   __shared__ __align__(16) float part[256];
@@ -615,16 +639,28 @@ mid_split_kernel(const T* first, int64_t ld1, int rows, int rank, const T* x, in
       const int k = k0 + (e & 15) + i;
       if (mid32) { if (t0 + tok < t && k < rank) mid32[(t0 + tok) * rank + k] = v[i]; }      // for the streaming kernel, in one part
       else if (t0 + tok < t) {                       // zeros behind the rank
-        T* m = mid + (t0 + tok) * ldm + k;
-        const T value = from_f32<T>(v[i]);
-        m[0] = value; m[ldm / 2] = from_f32<T>(v[i] - to_f32(value));
+        __nv_bfloat16* m = mid + (t0 + tok) * ldm + k;
+        const int64_t next = ldm / Parts<T>::all;
+        const bool finite = fabsf(v[i]) <= 3.402823466e38f;      // an infinity or a NaN is one part: what it left would be a NaN
+        if constexpr (Parts<T>::split) {
+          float rest = v[i];
+          __nv_bfloat16 p[3];
+#pragma unroll
+          for (int q = 0; q < 3; ++q) { p[q] = __float2bfloat16_rz(rest); rest = finite ? rest - __bfloat162float(p[q]) : 0.f; }
+#pragma unroll
+          for (int q = 0; q < 3; ++q) m[q * next] = p[q];
+          m[3 * next] = finite ? p[0] : __float2bfloat16_rn(0.f); m[4 * next] = p[1];
+        } else {
+          const __nv_bfloat16 value = __float2bfloat16_rn(v[i]);
+          m[0] = value; m[next] = __float2bfloat16_rn(finite ? v[i] - __bfloat162float(value) : 0.f);
+        }
       }
     }
   }
   cluster_sync_all();
 }
 
-template <class T> cudaError_t start_mid(const hyacinHandle_t* handle, const T* first, int64_t ld1, int rows, int rank, const T* x, int64_t ldx, int t, T* mid, int64_t ldm, int aligned, float* mid32) {
+template <class T> cudaError_t start_mid(const hyacinHandle_t* handle, const T* first, int64_t ld1, int rows, int rank, const T* x, int64_t ldx, int t, __nv_bfloat16* mid, int64_t ldm, int aligned, float* mid32) {
   cudaLaunchConfig_t mc{};
   mc.gridDim = dim3(unsigned((rank + 15) / 16) * kMidSplits, unsigned((int64_t(t) + 15) / 16)); mc.blockDim = dim3(kMidWarps * 32); mc.stream = handle->cudaStream;
   cudaLaunchAttribute ma[1];
@@ -704,7 +740,7 @@ template <class T, bool TRANS, int STEP> int32_t launch(const hyacinHandle_t* ha
   constexpr int kStep = G::step;
   p.code_steps = (in + kStep - 1) / kStep;
   p.rank = a.rank; p.rank16 = (a.rank + 15) / 16 * 16; p.second = a.second; p.ld2 = a.ld2; p.y = a.y; p.ldy = a.ldy;
-  p.steps = p.code_steps + (2 * p.rank16 + kStep - 1) / kStep;
+  p.steps = p.code_steps + (Parts<T>::all * p.rank16 + kStep - 1) / kStep;
   const int64_t token_tiles = (int64_t(a.t) + kMaxTokens - 1) / kMaxTokens;
   p.nt = int((int64_t(a.t) + token_tiles - 1) / token_tiles + 15) / 16 * 16;
   p.nt_cols = (p.nt + 31) / 32 * 32;
@@ -725,7 +761,8 @@ template <class T, bool TRANS, int STEP> int32_t launch(const hyacinHandle_t* ha
   const int tiles = (out + kOut - 1) / kOut;
   p.splits = choose_splits(int64_t(tiles) * token_tiles, p.steps, handle->DeviceSMs, kStep == 128 ? 6 : 12);
   const uint32_t fmt = type == HYACIN_F16 ? 0u : 1u;
-  p.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((TRANS ? 0u : 1u) << 15) | (uint32_t(p.nt >> 3) << 17) | (uint32_t(kOut >> 4) << 24);
+  p.idesc_more = (1u << 4) | (1u << 7) | (1u << 10) | ((TRANS ? 0u : 1u) << 15) | (uint32_t(p.nt >> 3) << 17) | (uint32_t(kOut >> 4) << 24);
+  p.idesc = (p.idesc_more & ~((1u << 7) | (1u << 10))) | (fmt << 7) | (fmt << 10);
   p.status = status_word_device(handle->DeviceID);
   const CUtensorMapDataType dt = type == HYACIN_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   CUtensorMap code_map{}, x_map{}, mid_map{};
@@ -733,11 +770,11 @@ template <class T, bool TRANS, int STEP> int32_t launch(const hyacinHandle_t* ha
               encode_2d(&x_map, dt, x, in, a.t, uint64_t(ldx) * 2, 64, p.nt, CU_TENSOR_MAP_SWIZZLE_128B);
   mid_map = x_map;
   if (fine && a.rank) {
-    const int64_t ldm = 2 * int64_t(p.rank16);
+    const int64_t ldm = Parts<T>::all * int64_t(p.rank16);
     if (!allocate(&mid, size_t(ldm) * a.t * 2)) { cleanup(); return -3; }
-    fine = encode_2d(&mid_map, dt, mid, uint64_t(ldm), a.t, uint64_t(ldm) * 2, 64, p.nt, CU_TENSOR_MAP_SWIZZLE_128B);
+    fine = encode_2d(&mid_map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, mid, uint64_t(ldm), a.t, uint64_t(ldm) * 2, 64, p.nt, CU_TENSOR_MAP_SWIZZLE_128B);
     const int aligned = reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx % 8 == 0 && reinterpret_cast<uintptr_t>(a.first) % 16 == 0 && a.ld1 % 8 == 0;
-    const cudaError_t e = start_mid<T>(handle, static_cast<const T*>(a.first), a.ld1, in, a.rank, static_cast<const T*>(x), ldx, a.t, static_cast<T*>(mid), ldm, aligned, nullptr);
+    const cudaError_t e = start_mid<T>(handle, static_cast<const T*>(a.first), a.ld1, in, a.rank, static_cast<const T*>(x), ldx, a.t, static_cast<__nv_bfloat16*>(mid), ldm, aligned, nullptr);
     if (e != cudaSuccess) { report_cuda_error(e, fn, __FILE__, __LINE__); fine = false; }
   }
   if (!fine) { cleanup(); return -3; }

@@ -26,3 +26,64 @@ def test_one_scale_per_column_by_the_largest_segments(hy, op, t, m, seg):
         x = P.round_to(rng.standard_normal((t, m if op == "T" else n)), kind)
         got = _run_product(hy, op, m, n, t, kind, seg, codes, scales, zp, x)
         _check_product(got, op, m, n, kind, seg, codes, scales, zp, x)
+
+
+# ---- the correction apart from the main sum ---------------------------------------------------------------------------
+def _correction_only(hy, op, kind, rank, t, exponents, m=512, n=200):
+    """All scales zero: Y = second (first^T x).  first and x hold whole numbers below 2^10 and 2^3 times powers of two, so every sum of
+    first^T x is a whole number below 2^10 2^3 512 = 2^22 times a power of two, exact in 32 bits."""
+    e_first, e_x, e_second = exponents
+    rng = np.random.default_rng(rank + t)
+    inn = m if op == "T" else n
+    codes, scales, _ = _problem(rng, m, n, 128, kind, False)
+    scales[:] = 0
+    most = 128 if kind == "bf16" else 1024
+    first = rng.integers(-most, most, (rank, inn)) * 2.0 ** e_first
+    second = rng.integers(-most, most, (rank, n if op == "T" else m)) * 2.0 ** e_second / most
+    x = rng.integers(-7, 8, (t, inn)) * 2.0 ** e_x
+    for v in (first, second, x):
+        assert np.array_equal(P.round_to(v, kind), v)
+    u, v = (first, second) if op == "T" else (second, first)
+    got = _run_product(hy, op, m, n, t, kind, 128, codes, scales, None, x, u, v)
+    mid = x @ first.T
+    assert np.abs(mid).max() < 2.0 ** (24 + e_first + e_x)
+    want, mag = mid @ second, np.abs(mid) @ np.abs(second)
+    # mid in parts of 8 bits: three for half (what is left of second times the third is 2^-24 of the magnitude), two for bfloat16; one
+    # rounding by a place of the largest term, 2^-23, for each of at most five addends per entry of the rank (padded to 16) and the
+    # joining of the shares; then the rounding of Y
+    lost = {"f16": 2.0 ** -23, "bf16": 2.0 ** -15, "f32": 0.0}[kind]
+    tol = P.HALF_STEP[kind] * np.abs(want) + (lost + (5 * (-(-rank // 16) * 16) + 32) * 2.0 ** -23) * mag + P.TINY[kind]
+    assert np.isfinite(got).all()
+    assert (np.abs(got - want) <= tol).all(), (np.abs(got - want) / tol).max()
+    return mid
+
+
+@pytest.mark.parametrize("op,t", [("T", 4), ("T", 20), ("T", 200), ("N", 3), ("N", 20), ("N", 200)])
+@pytest.mark.parametrize("rank", [1, 16, 40, 64, 100])
+@pytest.mark.parametrize("kind", ["f16", "bf16", "f32"])
+def test_correction_beyond_the_ends_of_its_type(hy, op, t, rank, kind):
+    """first^T x above the largest half (65504) and far below the smallest, with a Y that a half holds."""
+    mid = _correction_only(hy, op, kind, rank, t, (3, 1, -12))
+    assert np.abs(mid).max() > 65504
+    mid = _correction_only(hy, op, kind, rank, t, (-24, -8, 9))
+    assert np.abs(mid).max() < 2.0 ** -10 and np.median(np.abs(mid)) < 2.0 ** -14
+
+
+@pytest.mark.parametrize("op,t", [("T", 2), ("T", 20), ("N", 20)])
+def test_correction_of_an_infinite_entry_stays_infinite(hy, op, t):
+    """An infinite first^T x gives infinities of the second factor's signs where that is not zero."""
+    rng = np.random.default_rng(5)
+    m, n, rank = 256, 200, 3
+    for kind in ("bf16", "f16", "f32"):
+        codes, scales, _ = _problem(rng, m, n, 128, kind, False)
+        scales[:] = 0
+        inn, out = (m, n) if op == "T" else (n, m)
+        first, second = np.abs(rng.integers(1, 9, (rank, inn))) * 1.0, P.round_to(rng.standard_normal((rank, out)), kind)
+        second[1:] = 0
+        first[1:] = 0
+        x = np.ones((t, inn))
+        first[0, 7] = np.inf
+        u, v = (first, second) if op == "T" else (second, first)
+        got = _run_product(hy, op, m, n, t, kind, 128, codes, scales, None, x, u, v)
+        want = np.where(second[0] != 0, np.inf * np.sign(second[0]), np.nan)
+        assert np.array_equal(got, np.tile(want, (t, 1)), equal_nan=True)
