@@ -2,12 +2,12 @@
 // warp-level matrix instructions from there.
 //
 // Mathematics.  Y(j, t) = sum over segments of s(j, seg) sum_{r in seg} (q(r, j) - zero) x(r, t).  A mask turns two codes into two
-// 16-bit numbers offset + q (offset 1024 for half, 128 for bfloat16); for 16-bit x these go into the instruction as they are and
-// the segment's sum is corrected afterwards, sum (offset + q) x - (offset + zero) sum x, in 32 bits, with sum x per segment
-// prepared once per block: 7 instead of 11 instructions per eight codes.  What the difference cancels are 5 bits (8 for half)
-// of a 24-bit sum, less than a tenth of the rounding of Y.  A segment's sum is multiplied by its scale in 32 bits; the only rounding to
-// 16 bits is that of Y.  Single-precision x is split into three bfloat16 parts of 8 bits that add up to it exactly, three columns
-// of the right-hand operand, and multiplies the exact whole numbers q - zero: the result is that of 32-bit sums.
+// 16-bit numbers offset + q (offset 1024 for half, 128 for bfloat16), and one subtraction into the exact whole numbers q - zero, which
+// go into the instruction.  (Offset codes in the instruction and (offset + zero) sum x taken off afterwards would save those four of eleven
+// instructions per eight codes, but for x of one sign the sums to be cancelled are a hundred times the result for half, the
+// error a rounding of Y; and an infinite or very large x ends in infinity minus infinity.)  A segment's sum is multiplied by its scale in
+// 32 bits; the only rounding to 16 bits is that of Y.  Single-precision x is split into three bfloat16 parts of 8 bits that add up to it
+// exactly (down to 2^-110), three columns of the right-hand operand: the result is that of 32-bit sums.
 // Layout.  A CTA (one per SM) takes every 148th tile of 16 columns, the rows of the m16n8k16 instruction.  A column's codes are
 // contiguous; a stage of the ring holds 4096 rows of the tile (2048 for more than eight operand columns), one TMA box, so the copies for the next
 // stages and tiles are in flight all the time (up to 190 KiB per SM) whatever the arithmetic does.  Each of 16 warps takes two
@@ -50,7 +50,7 @@ struct StreamParams {
   void* y; int64_t ldy;
   int segs, seg_sub, seg_shift;                   // 32-row subsets per segment, its logarithm or -1
   int blocks, cols, tiles, ring, pitch, x_aligned;       // pitch: of x in shared memory, elements
-  int sums_at, ring_at, pairs_at, red_at, bars_at;
+  int ring_at, pairs_at, red_at, bars_at;
   uint32_t* status;
 };
 
@@ -82,29 +82,35 @@ template <bool HALF> __device__ __forceinline__ void code_pairs(uint32_t w, uint
 #pragma unroll
   for (int p = 0; p < 4; ++p) o[p] = and_or(w >> (4 * p), 0x000f000fu, Codes<HALF>::kBits);
 }
-// bfloat16 pairs q - zero
-__device__ __forceinline__ void subtract_zero(uint32_t (&o)[4], int zero) {
-  const uint32_t low = 0xc300c300u + uint32_t(zero) * 0x10001u;               // -(128 + zero)
+// Pairs q - zero; low: -(offset + zero) twice.
+template <bool HALF> __device__ __forceinline__ void subtract_zero(uint32_t (&o)[4], uint32_t low) {
+  using Two = std::conditional_t<HALF, __half2, __nv_bfloat162>;
 #pragma unroll
   for (int p = 0; p < 4; ++p) {
-    const __nv_bfloat162 v = __hadd2(*reinterpret_cast<__nv_bfloat162*>(&o[p]), *reinterpret_cast<const __nv_bfloat162*>(&low));
+    const Two v = __hadd2(*reinterpret_cast<Two*>(&o[p]), *reinterpret_cast<const Two*>(&low));
     o[p] = *reinterpret_cast<const uint32_t*>(&v);
   }
 }
 
-// Scale and offset + zero of one (column, segment), as kept in shared memory: two numbers of the scale's own type, which holds
-// offset + zero exactly (float: the zero point itself).
-template <class X> struct Pair { uint32_t bits; };
-template <> struct Pair<float> { float scale; int zero; };
+// Scale and -(offset + zero) of one (column, segment), as kept in shared memory: two numbers of the scale's own type, which holds
+// offset + zero exactly (float: the second as bfloat16, twice).
+template <class X> struct Pair {
+  uint32_t bits;
+  __device__ __forceinline__ float scale() const { const uint16_t s = uint16_t(bits); return to_f32(*reinterpret_cast<const X*>(&s)); }
+  __device__ __forceinline__ uint32_t low() const { return __byte_perm(bits, 0, 0x3232); }
+};
+template <> struct Pair<float> {
+  float s; uint32_t twice;
+  __device__ __forceinline__ float scale() const { return s; }
+  __device__ __forceinline__ uint32_t low() const { return twice; }
+};
 template <class X> __device__ __forceinline__ Pair<X> make_pair(X scale, int zero) {
-  if constexpr (sizeof(X) == 4) return {scale, zero};
+  if constexpr (sizeof(X) == 4) return {scale, 0xc300c300u + uint32_t(zero) * 0x10001u};
   else {
-    const X off = from_f32<X>(float(Codes<std::is_same<X, __half>::value>::kOffset + zero));
+    const X off = from_f32<X>(-float(Codes<std::is_same<X, __half>::value>::kOffset + zero));
     return {uint32_t(*reinterpret_cast<const uint16_t*>(&scale)) | uint32_t(*reinterpret_cast<const uint16_t*>(&off)) << 16};
   }
 }
-__device__ __forceinline__ float2 unpack_pair(const Pair<__half>& p) { return __half22float2(*reinterpret_cast<const __half2*>(&p.bits)); }
-__device__ __forceinline__ float2 unpack_pair(const Pair<__nv_bfloat16>& p) { return make_float2(__uint_as_float(p.bits << 16), __uint_as_float(p.bits & 0xffff0000u)); }
 
 
 __device__ __forceinline__ int segment_of(int sub, const StreamParams& p) { return p.seg_shift >= 0 ? sub >> p.seg_shift : sub / p.seg_sub; }
@@ -132,7 +138,6 @@ __global__ void __launch_bounds__(kThreads, 1) product_stream_kernel(const __gri
   constexpr int kRed = 8 * TILES + 1;
   extern __shared__ __align__(128) uint8_t smem[];
   uint16_t* xs = reinterpret_cast<uint16_t*>(smem);                // [operand column][row]
-  float* sums = reinterpret_cast<float*>(smem + p.sums_at);        // [segment of a block][operand column]: sum of x over it
   uint8_t* ring = smem + p.ring_at;
   Pair<X>* pairs = reinterpret_cast<Pair<X>*>(smem + p.pairs_at);  // [stage][column][segment of the stage]
   float* red = reinterpret_cast<float*>(smem + p.red_at);          // [joint][warp][column][operand column]
@@ -238,7 +243,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_stream_kernel(const __gri
   } else {
     // ---- products ----
     const int w = warp - 2 - kLoaders, g = lane >> 2, c = lane & 3;
-    // First x, one operand column per line, zeros behind the last row, and its sums per segment, while the first codes arrive.
+    // First x, one operand column per line, zeros behind the last row, while the first codes arrive.
     {
       const int rows = p.blocks * kW4Block, tid = threadIdx.x - 32 * (2 + kLoaders), step = kWarps * 32;
       if constexpr (kSplit) {
@@ -254,7 +259,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_stream_kernel(const __gri
             }
           }
       } else {
-        // eight rows per thread and step; the threads of a block are neighbours in one half of a warp (rows / 8 is a multiple of 16)
+        // eight rows per thread and step
         const int per = rows / 8, chunks = p.t * per;
 #pragma unroll 4
         for (int e = tid; e < chunks; e += step) {
@@ -269,17 +274,6 @@ __global__ void __launch_bounds__(kThreads, 1) product_stream_kernel(const __gri
             v = make_uint4(o[0], o[1], o[2], o[3]);
           }
           *reinterpret_cast<uint4*>(xs + t * p.pitch + r) = v;
-          const uint32_t u[4] = {v.x, v.y, v.z, v.w};
-          float s = 0.f;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint16_t lo = uint16_t(u[i]), hi = uint16_t(u[i] >> 16);
-            s += to_f32(*reinterpret_cast<const X*>(&lo)) + to_f32(*reinterpret_cast<const X*>(&hi));
-          }
-          const uint32_t mask = lane < 16 ? 0x0000ffffu : 0xffff0000u;
-#pragma unroll
-          for (int d = 1; d < 4 * GRAIN; d *= 2) s += __shfl_xor_sync(mask, s, d);
-          if ((r / 8) % (4 * GRAIN) == 0) sums[r / (32 * GRAIN) * (8 * TILES) + t] = s;
         }
       }
       asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory");
@@ -295,7 +289,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_stream_kernel(const __gri
         const uint8_t* from = ring + (stage * kTile + g) * kColumnPitch + w * 64 + c * 16;
         const Pair<X>* pa = pairs + (stage * kTile + g) * kPairs - segment_of(chunk * kStageBlocks * 4, p);
         const Pair<X>* pb = pa + 8 * kPairs;
-        // one block: (offset + q) x in the matrix pipe on top of -(offset + zero) sum x, times the scale
+        // one block: (q - zero) x in the matrix pipe, times the scale
         auto block = [&](int b, const uint4& qa, const uint4& qb) {
 #pragma unroll
           for (int i0 = 0; i0 < 4; i0 += GRAIN) {
@@ -303,23 +297,14 @@ __global__ void __launch_bounds__(kThreads, 1) product_stream_kernel(const __gri
             const int seg = GRAIN < 4 ? min(segment_of(4 * b + i0, p), p.segs - 1) : segment_of(4 * b, p);
             const Pair<X> va = pa[seg], vb = pb[seg];
             float acc[TILES][4] = {}, odd[TILES][4] = {};          // two chains of instructions that do not wait for each other
-            float sa, sb;
-            if constexpr (kSplit) { sa = va.scale; sb = vb.scale; }
-            else {
-              const float2 fa = unpack_pair(va), fb = unpack_pair(vb);
-              sa = fa.x; sb = fb.x;
-#pragma unroll
-              for (int j = 0; j < TILES; ++j) {
-                const float2 sx = *reinterpret_cast<const float2*>(sums + (4 * b + i0) / GRAIN * (8 * TILES) + 8 * j + 2 * c);
-                acc[j][0] = -fa.y * sx.x; acc[j][1] = -fa.y * sx.y; acc[j][2] = -fb.y * sx.x; acc[j][3] = -fb.y * sx.y;
-              }
-            }
+            const float sa = va.scale(), sb = vb.scale();
+            const uint32_t la = va.low(), lb = vb.low();
 #pragma unroll
             for (int i = i0; i < i0 + GRAIN; ++i) {
               uint32_t a[4], e[4];
               code_pairs<kHalf>(i == 0 ? qa.x : i == 1 ? qa.y : i == 2 ? qa.z : qa.w, a);
               code_pairs<kHalf>(i == 0 ? qb.x : i == 1 ? qb.y : i == 2 ? qb.z : qb.w, e);
-              if constexpr (kSplit) { subtract_zero(a, va.zero); subtract_zero(e, vb.zero); }
+              subtract_zero<kHalf>(a, la); subtract_zero<kHalf>(e, lb);
 #pragma unroll
               for (int j = 0; j < TILES; ++j) {
                 const uint4 x = *reinterpret_cast<const uint4*>(xl[j] + b * kW4Block + 32 * i);
@@ -473,12 +458,12 @@ int parts(hyacinPrecision_t type) { return type == HYACIN_F32 ? 3 : 1; }
 int layout(StreamParams& p, hyacinPrecision_t type, int tiles) {
   const int per_block = p.seg_sub % 4 == 0 ? 1 : p.seg_sub % 2 == 0 ? 2 : 4, stage_blocks = kWarps * blocks_per_warp(tiles);
   const int64_t pitch = int64_t(p.blocks) * kW4Block + 32;          // 64 bytes over a multiple of 256: lanes g, g + 1 in different halves of the banks
-  const int64_t x_bytes = (p.cols * pitch * 2 + 127) / 128 * 128, sums = type == HYACIN_F32 ? 0 : (int64_t(p.blocks) * per_block * 8 * tiles * 4 + 127) / 128 * 128;
+  const int64_t x_bytes = (p.cols * pitch * 2 + 127) / 128 * 128;
   const int64_t red = kJoints * kWarps * kTile * (8 * tiles + 1) * 4, pair_stage = int64_t(kTile) * (per_block * stage_blocks + 1) * (type == HYACIN_F32 ? 8 : 4);
-  const int64_t fixed = x_bytes + sums + red + int64_t(sizeof(StreamBars)), stage_codes = kTile * stage_blocks * 64, stage = stage_codes + pair_stage;
+  const int64_t fixed = x_bytes + red + int64_t(sizeof(StreamBars)), stage_codes = kTile * stage_blocks * 64, stage = stage_codes + pair_stage;
   const int64_t ring = std::min<int64_t>(kMaxRing, (kSmemLimit - fixed) / stage);
   if (fixed > kSmemLimit || ring < 4) return 0;
-  p.tiles = tiles; p.ring = int(ring); p.pitch = int(pitch); p.sums_at = int(x_bytes); p.ring_at = int(x_bytes + sums);
+  p.tiles = tiles; p.ring = int(ring); p.pitch = int(pitch); p.ring_at = int(x_bytes);
   p.pairs_at = int(p.ring_at + ring * stage_codes); p.red_at = int(p.pairs_at + ring * pair_stage); p.bars_at = int(p.red_at + red);
   return int(fixed + ring * stage);
 }

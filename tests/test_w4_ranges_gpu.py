@@ -87,3 +87,53 @@ def test_correction_of_an_infinite_entry_stays_infinite(hy, op, t):
         got = _run_product(hy, op, m, n, t, kind, 128, codes, scales, None, x, u, v)
         want = np.where(second[0] != 0, np.inf * np.sign(second[0]), np.nan)
         assert np.array_equal(got, np.tile(want, (t, 1)), equal_nan=True)
+
+
+# ---- few vectors: nothing but Y is rounded ------------------------------------------------------------------------------
+@pytest.mark.parametrize("kind,m,bits", [("f16", 512, 10), ("f16", 500, 10), ("f16", 4096, 7), ("bf16", 512, 7), ("bf16", 4000, 7)])
+@pytest.mark.parametrize("seg", [128, 64, 32, 96, 512])
+@pytest.mark.parametrize("t,zeros", [(1, False), (3, True), (8, False)])
+def test_few_vectors_of_one_sign_are_exact(hy, kind, m, bits, seg, t, zeros):
+    """x = 1 + k 2^-bits, scales of 1: every product is a multiple of 2^-bits and every sum of them, at most 15 * 2 * M, a 32-bit
+    number, so Y is the exact sum, rounded once."""
+    rng = np.random.default_rng(m + seg + t)
+    n = 150
+    codes, scales, zp = _problem(rng, m, n, seg, kind, zeros)
+    scales[:] = 1
+    x = 1 + rng.integers(0, 1 << bits, (t, m)) * 2.0 ** -bits
+    assert 30 * m * 2 ** bits <= 2 ** 24 and np.array_equal(P.round_to(x, kind), x)
+    got = _run_product(hy, "T", m, n, t, kind, seg, codes, scales, zp, x)
+    want = x @ P.values(codes, scales, zp, seg).T
+    assert np.array_equal(got, P.round_to(want, kind))
+
+
+@pytest.mark.parametrize("t", [1, 5, 8])
+@pytest.mark.parametrize("seg", [32, 64, 128])
+def test_few_vectors_with_an_entry_near_the_end_of_the_range(hy, t, seg):
+    """One entry of 2^122 beside zeros: fifteen times it is a 32-bit number, and so is every step on the way."""
+    rng = np.random.default_rng(t)
+    m, n = 384, 48
+    codes, scales, zp = _problem(rng, m, n, seg, "bf16", True)
+    scales[:] = 2.0 ** -100
+    x = np.zeros((t, m))
+    x[:, 77] = 2.0 ** 122
+    got = _run_product(hy, "T", m, n, t, "bf16", seg, codes, scales, zp, x)
+    assert np.array_equal(got, x @ P.values(codes, scales, zp, seg).T)
+
+
+@pytest.mark.parametrize("op", ["T", "N"])
+@pytest.mark.parametrize("t", [1, 4, 20, 140])
+@pytest.mark.parametrize("kind", ["f16", "bf16", "f32"])
+def test_an_infinite_entry_gives_infinities_of_the_weights_signs(hy, op, t, kind):
+    """For every number of vectors the same: infinity times the sign of the weight, NaN where the weight is zero."""
+    rng = np.random.default_rng(t)
+    m, n, seg = 200, 150, 32
+    for zeros in (False, True):
+        codes, scales, zp = _problem(rng, m, n, seg, kind, zeros)
+        x = P.round_to(rng.standard_normal((t, m if op == "T" else n)), kind)
+        x[0, 17] = -np.inf
+        got = _run_product(hy, op, m, n, t, kind, seg, codes, scales, zp, x)
+        w = P.values(codes, scales, zp, seg)
+        w = w[:, 17] if op == "T" else w[17]
+        assert np.array_equal(got[0], np.where(w == 0, np.nan, -np.inf * np.sign(w)), equal_nan=True)
+        assert np.isfinite(got[1:]).all()
