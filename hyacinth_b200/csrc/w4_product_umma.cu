@@ -92,6 +92,9 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&v)[32]
         "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
       : "memory");
 }
+__device__ __forceinline__ void tmem_st4(uint32_t addr, const uint32_t (&v)[4]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+}
 // Bounded waits for the pipelines of this kernel, executed by whole warps: a poll by a single lane is not suspended by the
 // hardware, and many warps that poll slow the multiplying warp down (a satisfied wait took it 800 cycles with 20 single-lane
 // pollers).  So few warps poll at a time, the ones that run ahead with pauses in between.
@@ -198,17 +201,12 @@ template <> struct Scale<__nv_bfloat16> {
 // Parts of the correction's operands, the same K range after another: with mid part i (i < mid) V, or what of it is left beyond
 // bfloat16 with part i - mid.
 template <class T> struct Parts { static constexpr bool split = std::is_same<T, __half>::value; static constexpr int mid = split ? 3 : 2, all = split ? 5 : 2; };
-// Eight halves as bfloat16: the nearest, or what it leaves (3 bits, exact).
-__device__ __forceinline__ uint4 factor_part(const uint4& v, bool rest) {
-  uint32_t o[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&o[i]));
-    __nv_bfloat162 b = __floats2bfloat162_rn(f.x, f.y);
-    if (rest) b = __floats2bfloat162_rn(fabsf(f.x) <= 65504.f ? f.x - __low2float(b) : 0.f, fabsf(f.y) <= 65504.f ? f.y - __high2float(b) : 0.f);
-    o[i] = *reinterpret_cast<const uint32_t*>(&b);
-  }
-  return make_uint4(o[0], o[1], o[2], o[3]);
+// Two halves as bfloat16: the nearest, or what it leaves (3 bits, exact; of an infinity a NaN).
+__device__ __forceinline__ uint32_t factor_part(uint32_t v, bool rest) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&v));
+  __nv_bfloat162 b = __floats2bfloat162_rn(f.x, f.y);
+  if (rest) b = __floats2bfloat162_rn(f.x - __low2float(b), f.y - __high2float(b));
+  return *reinterpret_cast<const uint32_t*>(&b);
 }
 
 template <class T, bool TRANS, int STEP>
@@ -471,14 +469,10 @@ product_umma_kernel(const __grid_constant__ CUtensorMap code_map, const __grid_c
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               const int e = (id & 127) + 128 * i, chunk = e & 15;
-              int a = c + (e >> 4), part = 0;
-              if (Parts<T>::split) { part = a / p.rank16; a -= part * p.rank16; }
-              else {
-                if (a >= 2 * p.rank16) a -= 2 * p.rank16;
-                if (a >= p.rank16) a -= p.rank16;
-              }
-              v[i] = load8(reinterpret_cast<const T*>(from + int64_t(a) * p.ld2) + chunk * 8, a < p.rank && part < Parts<T>::all ? valid - chunk * 8 : 0, p.second_aligned != 0);
-              if (Parts<T>::split) v[i] = factor_part(v[i], part >= Parts<T>::mid);
+              int a = c + (e >> 4);
+              if (a >= 2 * p.rank16) a -= 2 * p.rank16;
+              if (a >= p.rank16) a -= p.rank16;
+              v[i] = load8(reinterpret_cast<const T*>(from + int64_t(a) * p.ld2) + chunk * 8, a < p.rank ? valid - chunk * 8 : 0, p.second_aligned != 0);
             }
             group_sync();
 #pragma unroll
@@ -492,20 +486,35 @@ product_umma_kernel(const __grid_constant__ CUtensorMap code_map, const __grid_c
               to[e] = uint32_t(lo) | uint32_t(hi) << 16;
             }
           };
-          if (!Parts<T>::split && p.rank16 <= 64 && 64 % p.rank16 == 0) {      // the pattern repeats every 64 columns
+          // of half the parts are made here; they begin at multiples of 16 columns
+          auto store = [&](int pair) {
+            if constexpr (Parts<T>::split) {
+#pragma unroll
+              for (int e = 0; e < 32; e += 4) {
+                const int column = c0 + 64 * pair + 2 * e;
+                uint32_t part[4] = {};
+                if (column < Parts<T>::all * p.rank16) {
+#pragma unroll
+                  for (int i = 0; i < 4; ++i) part[i] = factor_part(o[e + i], column >= Parts<T>::mid * p.rank16);
+                }
+                tmem_st4(tdst + pair * 32 + e, part);
+              }
+            } else tmem_st32(tdst + pair * 32, o);
+          };
+          if (p.rank16 <= 64 && 64 % p.rank16 == 0) {                // the pattern repeats every 64 columns
             gather(0, o);
             if (p.rank16 == 64) gather(32, o + 16);
             else {
 #pragma unroll
               for (int e = 0; e < 16; ++e) o[16 + e] = o[e];
             }
-            tmem_st32(tdst, o); tmem_st32(tdst + 32, o);
+            store(0); store(1);
           } else {
 #pragma unroll 1
             for (int pair = 0; pair < 2; ++pair) {
-              const int c = Parts<T>::split ? c0 + pair * 64 : (c0 + pair * 64) % (2 * p.rank16);
-              gather(c, o); gather(Parts<T>::split ? c + 32 : (c + 32) % (2 * p.rank16), o + 16);
-              tmem_st32(tdst + pair * 32, o);
+              const int c = (c0 + pair * 64) % (2 * p.rank16);
+              gather(c, o); gather((c + 32) % (2 * p.rank16), o + 16);
+              store(pair);
             }
           }
         } else {
@@ -515,7 +524,7 @@ product_umma_kernel(const __grid_constant__ CUtensorMap code_map, const __grid_c
 #pragma unroll 4
           for (int j = 0; j < (kFull ? 16 : 8); ++j) {
             uint4 v = load8(reinterpret_cast<const T*>(from) + 8 * j, valid - 8 * j, p.second_aligned != 0);
-            if (Parts<T>::split) v = factor_part(v, c >= Parts<T>::mid * p.rank16);
+            if (Parts<T>::split) { const bool rest = c >= Parts<T>::mid * p.rank16; v = make_uint4(factor_part(v.x, rest), factor_part(v.y, rest), factor_part(v.z, rest), factor_part(v.w, rest)); }
             sts128(dst + (half + (j >> 3)) * (G::operand_bytes / 2) + (((j & 7) << 4) ^ swz), v.x, v.y, v.z, v.w);
           }
         }
