@@ -163,6 +163,13 @@ __device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask, uint32_t b
   return r;
 }
 
+// The first `left` of a word's eight rows, the zero point in the others.
+__device__ __forceinline__ uint32_t rows_only(uint32_t w, int left, uint32_t zero) {
+  left = min(max(left, 0), 8);
+  const uint32_t mask = ((1u << 4 * ((left + 1) >> 1)) - 1u) | ((1u << 4 * (left >> 1)) - 1u) << 16;
+  return (w & mask) | (zero * 0x11111111u & ~mask);
+}
+
 // Scale and zero point of one (column, segment), as the pairs that the dequantisation multiplies and subtracts.
 template <class T> struct Scale;
 // half: 0x6400 | q is 1024 + q and 0x6400 | 16 q is 1024 + 16 q, both exact
@@ -396,6 +403,7 @@ product_umma_kernel(const __grid_constant__ CUtensorMap code_map, const __grid_c
     // column of W within the step; for 'T' that is the output, which has to be this thread's lane of tensor memory
     const int row = TRANS ? 32 * (warp & 3) + lane : kFull ? id & 127 : id & 63, half = kFull ? 0 : (id >> 6) & 1;
     const uint32_t swz = (row & 7) << 4;
+    const int ragged = p.m % kStep ? p.code_steps - 1 : -1;        // 'T': the step that ends behind the last row
     // An operand buffer is free when the step before on it, k - bufs, was multiplied: the barrier that also frees that step's ring
     // stage.  A group waits for its own steps only and a barrier cannot overtake it: step k + ring is not loaded, and step
     // k - bufs + ring >= k not multiplied, before step k was, which needs this group (bufs <= ring).  It cannot be early either:
@@ -426,6 +434,17 @@ product_umma_kernel(const __grid_constant__ CUtensorMap code_map, const __grid_c
         uint32_t s[2], z; uint4 q[kQuarters];
         asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(s[0]), "=r"(s[1]) : "r"(at + row * 8));
         asm volatile("ld.shared.u32 %0, [%1];" : "=r"(z) : "r"(at + G::cols * 8 + row * 4));
+        if (TRANS && k == ragged) {
+          // rows behind the last one: their X is zero, but what is stored there times the scale may be infinite.  Done in place, so that the
+          // other steps keep their loads together.
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            const uint32_t there = codes + ((c ^ chunk) << 4);
+            const uint4 w = lds128(there);
+            const int left = p.m - k * kStep - 8 * c;
+            sts128(there, rows_only(w.x, left, z & 15), rows_only(w.y, left - 32, (z >> 8) & 15), rows_only(w.z, left - 64, (z >> 16) & 15), rows_only(w.w, left - 96, (z >> 24) & 15));
+          }
+        }
 #pragma unroll
         for (int c = 0; c < kQuarters; ++c) q[c] = lds128(codes + (((2 * half + c) ^ chunk) << 4));
 #pragma unroll

@@ -137,3 +137,27 @@ def test_an_infinite_entry_gives_infinities_of_the_weights_signs(hy, op, t, kind
         w = w[:, 17] if op == "T" else w[17]
         assert np.array_equal(got[0], np.where(w == 0, np.nan, -np.inf * np.sign(w)), equal_nan=True)
         assert np.isfinite(got[1:]).all()
+
+
+# ---- rows behind the last one ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("t", [1, 8, 9, 20, 200])
+@pytest.mark.parametrize("m", [1, 7, 33, 135, 200, 253])
+@pytest.mark.parametrize("seg", [32, 128])
+def test_rows_behind_the_last_one_do_not_count_whatever_their_scale(hy, t, m, seg):
+    """A segment whose weights reach 60000: the stored 0 of a row that does not exist stands for -8 s, beyond the largest half."""
+    torch = _torch()
+    from hyacinth_b200 import api
+    rng = np.random.default_rng(m)
+    n = 40
+    w = P.round_to(rng.standard_normal((n, m)), "f16")
+    w[:, -1] = 60000
+    segs, ldq = -(-m // seg), -(-m // 128) * 64
+    W = _dev(w, "f16")
+    Q = torch.zeros((n, ldq), dtype=torch.uint8, device="cuda")
+    S = torch.zeros((n, segs), dtype=torch.float16, device="cuda")
+    assert hy.quantize_w4(api.F16, m, n, W, m, seg, api.F16, Q, ldq, S, None, segs, None, 0) == 0
+    x = P.round_to(rng.standard_normal((t, m)) * 0.1, "f16")
+    X, Y = _dev(x, "f16"), torch.zeros((t, n), dtype=torch.float16, device="cuda")
+    assert hy.product_w4("T", m, n, t, api.F16, Q, ldq, seg, S, None, segs, X, m, 0, None, 0, None, 0, Y, n) == 0
+    torch.cuda.synchronize()
+    _check_product(_back(Y, n), "T", m, n, "f16", seg, P.unpack(Q.cpu().numpy(), m), _back(S, segs), None, x)
