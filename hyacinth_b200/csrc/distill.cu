@@ -532,11 +532,10 @@ int32_t launch_distill(const char* fn, const hyacinHandle_t* handle, hyacinPreci
       auto* kernel = distill_plain_kernel<decltype(tag)>;
       static std::atomic<uint64_t> ready{0};
       e = raise_limit(handle, kernel, ready);
-      if (e == cudaSuccess) kernel<<<unsigned(std::min(a.t, 1 << 20)), 512, smem, handle->cudaStream>>>(a);
+      if (e == cudaSuccess) e = w4_start(kernel, dim3(unsigned(std::min(a.t, 1 << 20))), 512, smem, handle->cudaStream, a);
     });
   }
-  if (e != cudaSuccess) { report_cuda_error(e, fn, __FILE__, __LINE__); return -3; }
-  return w4_launched(fn);
+  return w4_result(e, fn);
 }
 
 int32_t check_distill(const char* fn, const hyacinHandle_t* handle, hyacinPrecision_t type, const DistillArgs& a) {

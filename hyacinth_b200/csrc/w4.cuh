@@ -4,6 +4,7 @@
 #include <hyacin_b200.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+#include <utility>
 
 namespace hyb {
 
@@ -51,10 +52,17 @@ inline bool w4_device_ok(const hyacinHandle_t* handle) {
   int device = -1;
   return cudaGetDevice(&device) == cudaSuccess && device == handle->DeviceID;
 }
-inline int32_t w4_launched(const char* what) {
-  const cudaError_t e = cudaGetLastError();
+// A launch that returns its own error: the thread's last one may be of an earlier, unrelated call.
+template <class... P, class... A> cudaError_t w4_start(void (*kernel)(P...), dim3 grid, unsigned threads, size_t smem, cudaStream_t stream, A&&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid; cfg.blockDim = dim3(threads); cfg.dynamicSmemBytes = smem; cfg.stream = stream;
+  return cudaLaunchKernelEx(&cfg, kernel, std::forward<A>(args)...);
+}
+// The return value of an entry point.  An error that is reported here is not left for the next call that asks for the thread's last one.
+inline int32_t w4_result(cudaError_t e, const char* what) {
   if (e == cudaSuccess) return 0;
   report_cuda_error(e, what, __FILE__, __LINE__);
+  cudaGetLastError();
   return -3;
 }
 

@@ -46,8 +46,7 @@ extern "C" int32_t hyacinB200ProductW4(const hyacinHandle_t* handle, char opW, i
   if (in == 0) {
     const int64_t size = int64_t(w4_type_bytes(Xtype));
     count_launch();
-    zero_kernel<<<dim3(unsigned(std::min<int64_t>((out * size + 255) / 256, 1024)), unsigned(std::min(T, 4096))), 256, 0, handle->cudaStream>>>(static_cast<uint8_t*>(Y), ldy * size, out * size, T);
-    return w4_launched(fn);
+    return w4_result(w4_start(zero_kernel, dim3(unsigned(std::min<int64_t>((out * size + 255) / 256, 1024)), unsigned(std::min(T, 4096))), 256, 0, handle->cudaStream, static_cast<uint8_t*>(Y), ldy * size, out * size, T), fn);
   }
   const int per = trans ? product_stream_vectors(Xtype, a) : 0;
   if (Xtype == HYACIN_F32) {

@@ -295,7 +295,7 @@ template <Mode MODE, int TOK> cudaError_t start(const hyacinHandle_t* handle, Si
   if (a.parts > 1) {
     if (e == cudaSuccess) {
       count_launch();
-      join_kernel<<<unsigned((int64_t(a.out) * a.t + 255) / 256), 256, 0, handle->cudaStream>>>(a.scratch, a.parts, a.out, a.t, a.y, a.ldy);
+      e = w4_start(join_kernel, dim3(unsigned((int64_t(a.out) * a.t + 255) / 256)), 256, 0, handle->cudaStream, a.scratch, a.parts, a.out, a.t, a.y, a.ldy);
     }
     HYB_CUDA(cudaFreeAsync(a.scratch, handle->cudaStream));
   }
@@ -329,7 +329,7 @@ int32_t launch_product_single(const hyacinHandle_t* handle, const char* fn, bool
   cudaError_t e = cudaSuccess;
   if (p.rank) {
     e = cudaMallocFromPoolAsync(reinterpret_cast<void**>(&mid), size_t(p.rank) * p.t * sizeof(float), handle->mempool, stream);
-    if (e != cudaSuccess) { report_cuda_error(e, "cudaMallocFromPoolAsync", __FILE__, __LINE__); return -3; }
+    if (e != cudaSuccess) return w4_result(e, "cudaMallocFromPoolAsync");
     SingleArgs b = a;                              // mid(k, t) = sum_r first(r, k) x(r, t)
     b.second = static_cast<const float*>(p.first); b.ld2 = p.ld1; b.out = p.rank; b.y = mid; b.ldy = p.rank;
     e = start_for<kDense>(handle, b);
@@ -337,8 +337,7 @@ int32_t launch_product_single(const hyacinHandle_t* handle, const char* fn, bool
   }
   if (e == cudaSuccess) e = trans ? start_for<kCodesT>(handle, a) : p.t <= kFew && p.m >= 8 * kOut ? start_few(handle, a) : start_for<kCodesN>(handle, a);
   if (mid) HYB_CUDA(cudaFreeAsync(mid, stream));
-  if (e != cudaSuccess) { report_cuda_error(e, fn, __FILE__, __LINE__); return -3; }
-  return w4_launched(fn);
+  return w4_result(e, fn);
 }
 
 }  // namespace hyb

@@ -496,7 +496,7 @@ int32_t launch_product_stream(const hyacinHandle_t* handle, const char* fn, hyac
     using X = decltype(tag);
     if (a.rank) {
       const cudaError_t e = cudaMallocFromPoolAsync(reinterpret_cast<void**>(&mid), size_t(a.rank) * a.t * sizeof(float), handle->mempool, stream);
-      if (e != cudaSuccess) { report_cuda_error(e, "cudaMallocFromPoolAsync", __FILE__, __LINE__); mid = nullptr; rc = -3; return; }
+      if (e != cudaSuccess) { rc = w4_result(e, "cudaMallocFromPoolAsync"); mid = nullptr; return; }
     }
     for (int64_t t0 = 0; t0 < a.t && rc == 0; t0 += per) {
       StreamParams p{};
@@ -521,19 +521,19 @@ int32_t launch_product_stream(const hyacinHandle_t* handle, const char* fn, hyac
         const bool both = wide && reinterpret_cast<uintptr_t>(a.first) % 16 == 0 && a.ld1 * sizeof(X) % 16 == 0;
         if (sizeof(X) == 2 && (p.t > 2 || !both)) {                  // a cluster per 16 x 16 entries
           const cudaError_t e = launch_mid_float(handle, type, a.first, a.ld1, a.m, a.rank, p.x, a.ldx, p.t, mid + t0 * a.rank, both);
-          if (e != cudaSuccess) { report_cuda_error(e, fn, __FILE__, __LINE__); rc = -3; return; }
+          if (e != cudaSuccess) { rc = w4_result(e, fn); return; }
         } else {
           // the product's blocks move in beside this kernel's only if the SM is already split between cache and shared memory their way
           static std::atomic<uint64_t> carved{0};
           const uint64_t mine = uint64_t(1) << (handle->DeviceID & 63);
           if (!(carved.load() & mine)) { HYB_CUDA(cudaFuncSetAttribute(mid_kernel<X>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared)); carved.fetch_or(mine); }
           count_launch();
-          mid_kernel<X><<<dim3(a.rank, (p.t + 7) / 8), p.t == 1 ? 64 : 256, 0, stream>>>(static_cast<const X*>(a.first), a.ld1, a.m, a.rank, static_cast<const X*>(p.x), a.ldx, p.t, mid + t0 * a.rank, both);
+          const cudaError_t e = w4_start(mid_kernel<X>, dim3(a.rank, (p.t + 7) / 8), p.t == 1 ? 64 : 256, 0, stream, static_cast<const X*>(a.first), a.ld1, a.m, a.rank, static_cast<const X*>(p.x), a.ldx, p.t, mid + t0 * a.rank, int(both));
+          if (e != cudaSuccess) { rc = w4_result(e, fn); return; }
         }
       }
       const cudaError_t e = p.seg_sub % 4 == 0 ? dispatch<X, 4>(handle, map, p, smem) : p.seg_sub % 2 == 0 ? dispatch<X, 2>(handle, map, p, smem) : dispatch<X, 1>(handle, map, p, smem);
-      if (e != cudaSuccess) { report_cuda_error(e, fn, __FILE__, __LINE__); rc = -3; }
-      else rc = w4_launched(fn);
+      rc = w4_result(e, fn);
     }
   });
   if (mid) HYB_CUDA(cudaFreeAsync(mid, stream));

@@ -741,7 +741,7 @@ template <class T, bool TRANS, int STEP> int32_t launch(const hyacinHandle_t* ha
   auto cleanup = [&] { if (x_copy) HYB_CUDA(cudaFreeAsync(x_copy, stream)); if (mid) HYB_CUDA(cudaFreeAsync(mid, stream)); };
   auto allocate = [&](void** p, size_t bytes) {
     const cudaError_t e = cudaMallocFromPoolAsync(p, bytes, handle->mempool, stream);
-    if (e != cudaSuccess) { report_cuda_error(e, "cudaMallocFromPoolAsync", __FILE__, __LINE__); *p = nullptr; }
+    if (w4_result(e, "cudaMallocFromPoolAsync")) *p = nullptr;
     return e == cudaSuccess;
   };
   const void* x = a.x; int64_t ldx = a.ldx;
@@ -751,8 +751,9 @@ template <class T, bool TRANS, int STEP> int32_t launch(const hyacinHandle_t* ha
     if (!allocate(&x_copy, size_t(ldo) * a.t * 2)) return -3;
     for (int64_t t = 0; t < a.t; t += 65535) {
       count_launch();
-      align_rows_kernel<<<dim3((in + 255) / 256, unsigned(std::min<int64_t>(65535, a.t - t))), 256, 0, stream>>>(
-          static_cast<const uint16_t*>(a.x) + t * a.ldx, a.ldx, in, static_cast<uint16_t*>(x_copy) + t * ldo, ldo);
+      const cudaError_t e = w4_start(align_rows_kernel, dim3((in + 255) / 256, unsigned(std::min<int64_t>(65535, a.t - t))), 256, 0, stream,
+                                     static_cast<const uint16_t*>(a.x) + t * a.ldx, a.ldx, in, static_cast<uint16_t*>(x_copy) + t * ldo, ldo);
+      if (e != cudaSuccess) { cleanup(); return w4_result(e, fn); }
     }
     x = x_copy; ldx = ldo;
   }
@@ -803,7 +804,7 @@ template <class T, bool TRANS, int STEP> int32_t launch(const hyacinHandle_t* ha
     fine = encode_2d(&mid_map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, mid, uint64_t(ldm), a.t, uint64_t(ldm) * 2, 64, p.nt, CU_TENSOR_MAP_SWIZZLE_128B);
     const int aligned = reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx % 8 == 0 && reinterpret_cast<uintptr_t>(a.first) % 16 == 0 && a.ld1 % 8 == 0;
     const cudaError_t e = start_mid<T>(handle, static_cast<const T*>(a.first), a.ld1, in, a.rank, static_cast<const T*>(x), ldx, a.t, static_cast<__nv_bfloat16*>(mid), ldm, aligned, nullptr);
-    if (e != cudaSuccess) { report_cuda_error(e, fn, __FILE__, __LINE__); fine = false; }
+    if (w4_result(e, fn)) fine = false;
   }
   if (!fine) { cleanup(); return -3; }
   auto* kernel = product_umma_kernel<T, TRANS, STEP>;
@@ -811,7 +812,7 @@ template <class T, bool TRANS, int STEP> int32_t launch(const hyacinHandle_t* ha
   const uint64_t bit = uint64_t(1) << (handle->DeviceID & 63);
   if (!(ready.load() & bit)) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit);
-    if (e != cudaSuccess) { report_cuda_error(e, "cudaFuncSetAttribute", __FILE__, __LINE__); cleanup(); return -3; }
+    if (e != cudaSuccess) { cleanup(); return w4_result(e, "cudaFuncSetAttribute"); }
     ready.fetch_or(bit);
   }
   cudaLaunchConfig_t cfg{};
@@ -822,9 +823,8 @@ template <class T, bool TRANS, int STEP> int32_t launch(const hyacinHandle_t* ha
   cfg.attrs = attr; cfg.numAttrs = attrs;
   count_launch();
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, code_map, x_map, mid_map, p);
-  if (e != cudaSuccess) report_cuda_error(e, fn, __FILE__, __LINE__);
   cleanup();
-  return e == cudaSuccess ? w4_launched(fn) : -3;
+  return w4_result(e, fn);
 }
 
 }  // namespace

@@ -277,6 +277,7 @@ extern "C" int32_t hyacinB200QuantizeW4(const hyacinHandle_t* handle, hyacinPrec
   if (blocks > 0x7fffffff) return w4_refuse(fn, "too many segments");
   timer_mark(handle, Segment::Replicated);
   count_launch();
+  cudaError_t e = cudaSuccess;
   if (segM == 32 || segM == 64 || segM == 128 || segM == 256) {
     const int64_t groups = (int64_t(M) + 255) / 256;
     const int w_aligned = reinterpret_cast<uintptr_t>(W) % 16 == 0 && int64_t(ldw) * int64_t(w4_type_bytes(Wtype)) % 16 == 0;
@@ -285,12 +286,12 @@ extern "C" int32_t hyacinB200QuantizeW4(const hyacinHandle_t* handle, hyacinPrec
     const int64_t chunks = std::max<int64_t>(1, std::min<int64_t>({(int64_t(N) + 7) / 8, 8 * int64_t(handle->DeviceSMs) / groups, 65535}));
     with_w4_type(Wtype, [&](auto t) { with_w4_type(Stype, [&](auto s) {
       auto* kernel = zeros ? quantize_w4_warp_kernel<decltype(t), decltype(s), false> : quantize_w4_warp_kernel<decltype(t), decltype(s), true>;
-      kernel<<<dim3(unsigned(groups), unsigned(chunks)), 256, 0, handle->cudaStream>>>(a, w_aligned, r_aligned);
+      e = w4_start(kernel, dim3(unsigned(groups), unsigned(chunks)), 256, 0, handle->cudaStream, a, w_aligned, r_aligned);
     }); });
-    return w4_launched("quantize_w4_warp_kernel");
+    return w4_result(e, "quantize_w4_warp_kernel");
   }
   with_w4_type(Wtype, [&](auto t) { with_w4_type(Stype, [&](auto s) {
-    quantize_w4_kernel<decltype(t), decltype(s)><<<unsigned(blocks), 256, 0, handle->cudaStream>>>(a);
+    e = w4_start(quantize_w4_kernel<decltype(t), decltype(s)>, dim3(unsigned(blocks)), 256, 0, handle->cudaStream, a);
   }); });
-  return w4_launched("quantize_w4_kernel");
+  return w4_result(e, "quantize_w4_kernel");
 }

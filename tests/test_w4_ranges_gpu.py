@@ -161,3 +161,32 @@ def test_rows_behind_the_last_one_do_not_count_whatever_their_scale(hy, t, m, se
     assert hy.product_w4("T", m, n, t, api.F16, Q, ldq, seg, S, None, segs, X, m, 0, None, 0, None, 0, Y, n) == 0
     torch.cuda.synchronize()
     _check_product(_back(Y, n), "T", m, n, "f16", seg, P.unpack(Q.cpu().numpy(), m), _back(S, segs), None, x)
+
+
+# ---- errors of other calls --------------------------------------------------------------------------------------------------
+def test_an_earlier_error_is_not_reported_again(hy, capfd):
+    """A product whose scratch nobody can allocate (2^20 x 2^29 numbers) returns -3 before anything is launched; the next calls succeed."""
+    torch = _torch()
+    from hyacinth_b200 import api
+    n, m = 4, 128
+    W = torch.ones((n, m), device="cuda")
+    Q, S = torch.zeros((n, 64), dtype=torch.uint8, device="cuda"), torch.zeros((n, 1), device="cuda")
+    Y, loss = torch.zeros((1, n), device="cuda"), torch.zeros(1, device="cuda")
+    ids, teacher, stats = torch.zeros((1, 1), dtype=torch.int32, device="cuda"), torch.zeros((1, 1), device="cuda"), torch.zeros((1, 2), device="cuda")
+
+    def fail():
+        assert hy.product_w4("N", m, n, 1 << 29, api.F32, Q, 64, 128, S, None, 1, W, m, 1 << 20, W, m, W, n, Y, m) == -3
+    calls = [lambda: hy.quantize_w4(api.F32, m, n, W, m, 128, api.F32, Q, 64, S, None, 1, None, 0),
+             lambda: hy.quantize_w4(api.F32, m, n, W, m, 96, api.F32, Q, 64, torch.zeros((n, 2), device="cuda"), None, 2, None, 0),
+             lambda: hy.product_w4("T", m, n, 1, api.F32, Q, 64, 128, S, None, 1, W, m, 0, None, 0, None, 0, Y, n),
+             lambda: hy.product_w4("T", 0, n, 1, api.F32, Q, 64, 128, S, None, 1, W, m, 0, None, 0, None, 0, Y, n),
+             lambda: hy.distill_loss(api.F32, n, 1, Y, n, 1, ids, teacher, 1, 1.0, None, None, loss, stats, None, 0),
+             lambda: hy.distill_grad(api.F32, n, 1, Y, n, 1, ids, teacher, 1, 1.0, None, None, stats, Y, n)]
+    A, V, sv = torch.randn((8, 64), dtype=torch.float64, device="cuda"), torch.zeros((8, 8), dtype=torch.float64, device="cuda"), torch.zeros(8, dtype=torch.float64, device="cuda")
+    fit = (lambda: hy.tsvd_fit(1e-6, "N", 64, 8, 8, A, 64, sv, V, 8, 64, api.F64) - 8)
+    for call in calls + [fit]:
+        fail()
+        capfd.readouterr()
+        assert call() == 0
+        torch.cuda.synchronize()
+        assert capfd.readouterr().err == ""
