@@ -62,6 +62,11 @@ ProfileScope::~ProfileScope() {
 void timer_mark(const hyacinHandle_t* handle, Segment seg) {
   auto* t = static_cast<SegmentTimer*>(handle->timer);
   if (!t || t->current == seg) return;
+  // An event recorded into a graph has no time of its own, and the class of work would be taken for marked: work being captured is not
+  // timed.  (The legacy stream beside another stream's capture gives an error here; recording on it would end that capture.)
+  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(handle->cudaStream, &capture) != cudaSuccess) { cudaGetLastError(); return; }
+  if (capture != cudaStreamCaptureStatusNone) return;
   cudaEvent_t e; if (cudaEventCreate(&e) != cudaSuccess) return;
   HYB_CUDA(cudaEventRecord(e, handle->cudaStream));
   t->events.emplace_back(t->current, e); t->current = seg;

@@ -190,3 +190,33 @@ def test_an_earlier_error_is_not_reported_again(hy, capfd):
         assert call() == 0
         torch.cuda.synchronize()
         assert capfd.readouterr().err == ""
+
+
+def test_segment_timer_beside_a_captured_call(monkeypatch):
+    """A handle with a timer: what is captured into a graph is not timed (its events would have no time), eager calls still are."""
+    torch = _torch()
+    from hyacinth_b200 import api
+    monkeypatch.setenv("HYACIN_CREATE_TIMER", "1")
+    n, m = 512, 4096
+    W = torch.randn((n, m), device="cuda")
+    Q, S = torch.zeros((n, m // 2), dtype=torch.uint8, device="cuda"), torch.zeros((n, m // 128), device="cuda")
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with api.Hyacin(stream=stream.cuda_stream) as h, torch.cuda.stream(stream):
+        def call():
+            assert h.quantize_w4(api.F32, m, n, W, m, 128, api.F32, Q, m // 2, S, None, m // 128, None, 0) == 0
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=stream):
+            call()
+        g.replay()
+        for _ in range(3):
+            call()
+        assert h.sync_timer("R")["R"] > 0
+        call()
+        other = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(other, stream=stream):
+            call()
+        other.replay()
+        call()
+        assert h.sync_timer("R")["R"] > 0
+        del g, other
