@@ -550,7 +550,7 @@ int32_t check_distill(const char* fn, const hyacinHandle_t* handle, hyacinPrecis
   if (a.dz == a.z && a.lddz != a.ldz) return w4_refuse(fn, "dZ in place of Z needs the same leading dimension");
   if (!w4_on_boundary(w4_type_bytes(type), a.z, a.dz) || !w4_on_boundary(4, a.ids, a.teacher, a.teacher_lse, a.weight, a.loss, a.stats_out, a.stats_in))
     return w4_refuse(fn, "a pointer that is not on a boundary of its type");
-  if (!w4_device_ok(handle)) return w4_refuse(fn, "the handle belongs to another device than the current one");
+  if (w4_refuse_handle(fn, handle)) return -1;
   return 0;
 }
 

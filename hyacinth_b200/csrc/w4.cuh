@@ -47,10 +47,13 @@ inline int32_t w4_refuse(const char* fn, const char* why) {
 // Pointers lie on a boundary of their type's size: the kernels' loads would fault otherwise.
 inline bool w4_on_boundary(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 template <class... P> bool w4_on_boundary(size_t bytes, P... p) { return (w4_on_boundary(static_cast<const void*>(p), bytes) && ...); }
-// The handle's device must be the current one: launches would otherwise go to the wrong GPU.
-inline bool w4_device_ok(const hyacinHandle_t* handle) {
+// The handle's device must be the current one: launches would otherwise go to the wrong GPU.  A zero-initialised handle names device 0,
+// but has neither its number of SMs, by which grids are divided, nor a pool.
+inline int32_t w4_refuse_handle(const char* fn, const hyacinHandle_t* handle) {
   int device = -1;
-  return cudaGetDevice(&device) == cudaSuccess && device == handle->DeviceID;
+  if (cudaGetDevice(&device) != cudaSuccess || device != handle->DeviceID) return w4_refuse(fn, "the handle belongs to another device than the current one");
+  if (handle->DeviceSMs < 1 || !handle->mempool) return w4_refuse(fn, "the handle has not been through hyacinCreate");
+  return 0;
 }
 // A launch that returns its own error: the thread's last one may be of an earlier, unrelated call.
 template <class... P, class... A> cudaError_t w4_start(void (*kernel)(P...), dim3 grid, unsigned threads, size_t smem, cudaStream_t stream, A&&... args) {

@@ -40,7 +40,7 @@ extern "C" int32_t hyacinB200ProductW4(const hyacinHandle_t* handle, char opW, i
   }
   if (!w4_on_boundary(w4_type_bytes(Xtype), Y) || (in > 0 && !w4_on_boundary(w4_type_bytes(Xtype), X, scales)) || (in > 0 && rank > 0 && !w4_on_boundary(w4_type_bytes(Xtype), U, V)))
     return w4_refuse(fn, "a pointer that is not on a boundary of its type");
-  if (!w4_device_ok(handle)) return w4_refuse(fn, "the handle belongs to another device than the current one");
+  if (w4_refuse_handle(fn, handle)) return -1;
   const ProductArgs a{codes, ldq, M, N, T, segM, scales, zeros, lds, X, ldx, rank, trans ? U : V, trans ? ldu : ldv, trans ? V : U, trans ? ldv : ldu, Y, ldy};
   timer_mark(handle, Segment::Replicated);
   if (in == 0) {

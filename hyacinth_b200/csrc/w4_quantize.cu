@@ -271,7 +271,7 @@ extern "C" int32_t hyacinB200QuantizeW4(const hyacinHandle_t* handle, hyacinPrec
   if (ldw < M || lds < segs || (R && ldr < M)) return w4_refuse(fn, "leading dimension too small");
   if (ldq % 16 || ldq < (int64_t(M) + 127) / 128 * 64 || reinterpret_cast<uintptr_t>(codes) % 16) return w4_refuse(fn, "codes: 16-byte aligned, ldq a multiple of 16 and at least 64 ceil(M / 128)");
   if (!w4_on_boundary(w4_type_bytes(Wtype), W) || !w4_on_boundary(w4_type_bytes(Stype), scales) || !w4_on_boundary(4, R)) return w4_refuse(fn, "a pointer that is not on a boundary of its type");
-  if (!w4_device_ok(handle)) return w4_refuse(fn, "the handle belongs to another device than the current one");
+  if (w4_refuse_handle(fn, handle)) return -1;
   QuantizeArgs a{W, ldw, M, N, segM, segs, codes, ldq, scales, zeros, lds, R, ldr};
   const int64_t blocks = (int64_t(N) * segs + 7) / 8;
   if (blocks > 0x7fffffff) return w4_refuse(fn, "too many segments");

@@ -158,7 +158,7 @@ int32_t hyacinB200PivotedCholesky(const hyacinHandle_t* handle, double eps, int3
  *
  * All calls are asynchronous on handle->cudaStream, may be captured into a CUDA graph, and return 0, -1 for arguments
  * they do not take (message on stderr, nothing launched), or -3 when CUDA refused a launch or an allocation.  The handle
- * has to belong to the current device.  Scratch comes from handle->mempool in stream order.  Outputs do not overlap inputs
+ * has to come from hyacinCreate on the device that is current.  Scratch comes from handle->mempool in stream order.  Outputs do not overlap inputs
  * unless stated.  M, N and T of the products are at most 2^31 - 256, and pointers lie on a boundary of their type.  Results do not depend on timing: there are no atomic sums. */
 #define HYACIN_B200_BF16 ((hyacinPrecision_t)32)
 

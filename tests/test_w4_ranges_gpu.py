@@ -220,3 +220,23 @@ def test_segment_timer_beside_a_captured_call(monkeypatch):
         call()
         assert h.sync_timer("R")["R"] > 0
         del g, other
+
+
+def test_a_handle_that_was_never_created_is_refused(hy, capfd):
+    """Zero-initialised, it names device 0, the current one, but has neither its number of SMs nor a pool."""
+    import ctypes
+    torch = _torch()
+    from hyacinth_b200 import api
+    lib, raw = api.load(), api.HyacinHandle()
+    h = ctypes.byref(raw)
+    W = torch.ones((4, 128), device="cuda")
+    Q, S = torch.zeros((4, 64), dtype=torch.uint8, device="cuda"), torch.zeros((4, 1), device="cuda")
+    Y, stats = torch.zeros((40, 4), device="cuda"), torch.zeros((40, 2), device="cuda")
+    w, q, s, y, st = (t.data_ptr() for t in (W, Q, S, Y, stats))
+    assert lib.hyacinB200QuantizeW4(h, api.F32, 128, 4, w, 128, 128, api.F32, q, 64, s, None, 1, None, 0) == -1
+    for kind in (api.F32, api.F16):
+        for t in (1, 4):
+            assert lib.hyacinB200ProductW4(h, b"T", 128, 4, t, kind, q, 64, 128, s, None, 1, w, 128, 0, None, 0, None, 0, y, 4) == -1
+    assert lib.hyacinB200DistillLoss(h, api.F32, 4, 1, y, 4, 0, None, None, 0, 1.0, None, None, st, None, None, 0) == -1
+    assert lib.hyacinB200DistillGrad(h, api.F32, 4, 1, y, 4, 0, None, None, 0, 1.0, None, None, st, y, 4) == -1
+    assert capfd.readouterr().err.count("hyacinCreate") == 7
