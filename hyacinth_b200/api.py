@@ -20,7 +20,7 @@ DEFAULT_LIB = os.path.join(_PKG, "libhyacin.so")
 # hyacinPrecision_t
 F64, F64_COMPLEX, F32, F32_COMPLEX, F16, F16_COMPLEX, DD, DD_COMPLEX, TF, TF_COMPLEX, QF, QF_COMPLEX = range(12)
 ELEM_BYTES = [8, 16, 4, 8, 2, 4, 16, 32, 12, 24, 16, 32]
-BF16 = 32            # HYACIN_B200_BF16: taken by the 4-bit weight and distillation entry points only
+BF16 = 14            # HYACIN_B200_BF16: taken by the 4-bit weight and distillation entry points only
 
 PUBLIC_SYMBOLS = [
     "hyacinCreate", "hyacinDestroy", "hyacinInterpolateFit", "hyacinTsvdFit", "hyacinTsvdFitSegmentN",

@@ -160,7 +160,7 @@ int32_t hyacinB200PivotedCholesky(const hyacinHandle_t* handle, double eps, int3
  * they do not take (message on stderr, nothing launched), or -3 when CUDA refused a launch or an allocation.  The handle
  * has to come from hyacinCreate on the device that is current.  Scratch comes from handle->mempool in stream order.  Outputs do not overlap inputs
  * unless stated.  M, N and T of the products are at most 2^31 - 256, and pointers lie on a boundary of their type.  Results do not depend on timing: there are no atomic sums. */
-#define HYACIN_B200_BF16 ((hyacinPrecision_t)32)
+#define HYACIN_B200_BF16 ((hyacinPrecision_t)14)      /* within the values that the enumeration's type can hold, 0 .. 15 */
 
 /* 4-bit form of W (type Wtype, leading dimension ldw).  scales has type Stype.  zeros == NULL: symmetric,
  * s = Stype(max|w| / 7), q = clamp(rint(w / s), -7, 7) + 8.  Otherwise lo = min(0, min w), hi = max(0, max w),
