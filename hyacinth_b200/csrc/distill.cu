@@ -81,6 +81,9 @@ __host__ __device__ constexpr size_t list_bytes(int k) { return 32 * 12 + size_t
 // What is known of the teacher, and of the student's listed classes, before the rest of the row has been seen.
 struct Listed { double rest, mass, top, sum; };      // p_r, sum p + p_r; log-sum-exp of the student's listed classes as top + log(sum), top = -inf without any
 
+// exp(z / tau - top), top the maximum over the listed classes.  Maxima leave NaNs out, so a list of NaNs has no top, but its sum is one.
+__device__ __forceinline__ double relative_exp(float z, double inv_tau, double top) { return top == -INFINITY ? (z == -INFINITY ? 0. : double(z)) : exp(double(z) * inv_tau - top); }
+
 // Reads the list.  Ends with a barrier.
 template <class T> __device__ Listed load_list(const DistillArgs& a, int64_t token, const T* z, List& s) {
   double top = -INFINITY, student = -INFINITY;
@@ -117,7 +120,7 @@ template <class T> __device__ Listed load_list(const DistillArgs& a, int64_t tok
     int first = s.id[i] >= 0; double ps = 0.;
     for (int j = 0; j < a.k; ++j) if (s.id[j] == s.id[i]) { ps += s.p[j]; if (j < i) first = 0; }
     s.first[i] = first; s.psum[i] = ps;
-    s.e[i] = s.id[i] >= 0 && r.top > -INFINITY ? exp(double(s.z[i]) * a.inv_tau - r.top) : 0.;
+    s.e[i] = s.id[i] >= 0 ? relative_exp(s.z[i], a.inv_tau, r.top) : 0.;
     if (first) e += s.e[i];
   }
   r.sum = block_reduce(e, Add{}, s.buf);
@@ -150,9 +153,9 @@ __device__ __forceinline__ double listed_loss(const DistillArgs& a, const List& 
 __device__ __forceinline__ double outside_loss(const DistillArgs& a, const Listed& l, const Student& st, double log_total, float top, float outside) {
   return l.rest > 0. ? l.rest * (log(l.rest) - (st.no_outside ? -INFINITY : log(double(outside)) + double(top) * a.inv_tau - st.ref - log_total)) : 0.;
 }
-// dKL/dz = factor * 2^(z scale - top scale) outside the list
+// dKL/dz = factor * 2^(z scale - top scale) outside the list; without anything there 0, or what a list of NaNs makes of it
 __device__ __forceinline__ double outside_factor(const DistillArgs& a, const Listed& l, const Student& st, float outside, float weight) {
-  return st.no_outside ? 0. : double(weight) * a.inv_tau * (l.mass * st.outside_share / st.total - l.rest / double(outside));
+  return st.no_outside ? 0. * st.total : double(weight) * a.inv_tau * (l.mass * st.outside_share / st.total - l.rest / double(outside));
 }
 __device__ __forceinline__ float listed_gradient(const DistillArgs& a, const List& s, const Listed& l, const Student& st, float weight, int i) {
   return float(double(weight) * a.inv_tau * ((st.total == 0. ? 0. : l.mass * s.e[i] * st.list_share / st.total) - s.psum[i]));
@@ -308,7 +311,7 @@ template <class T> __device__ Listed list_by_warp(const DistillArgs& a, int64_t 
     const bool ok = s.id[i] >= 0;
     const double l = s.logp[i] - norm, p = ok ? exp(l) : 0.;
     s.logp[i] = l; s.p[i] = p; s.first[i] = ok;
-    s.e[i] = ok && student32 != -INFINITY ? exp(double(s.z[i]) * a.inv_tau - r.top) : 0.;
+    s.e[i] = ok ? relative_exp(s.z[i], a.inv_tau, r.top) : 0.;
     sum += p;
   }
   sum = warp_reduce(sum, Add{});
@@ -440,7 +443,8 @@ template <class T> __global__ void __launch_bounds__(kClusterThreads, 3) distill
       top = warp_reduce(pm, Max{});
       if (top == -INFINITY) top = 0.f;
       const double scale = double(float(1.4426950408889634 * a.inv_tau));
-      const double share = pm == -INFINITY ? 0. : pm == top ? double(ps) : double(ps) * exp2((double(pm) - double(top)) * scale);
+      // a part without a maximum holds nothing, or nothing but NaNs: its sum says which
+      const double share = pm == -INFINITY || pm == top ? double(ps) : double(ps) * exp2((double(pm) - double(top)) * scale);
       outside = float(warp_reduce(share, Add{}));
     }
     const Student st(a, l, top, outside);
