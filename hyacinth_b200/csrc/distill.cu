@@ -17,7 +17,8 @@
 // Bound: DRAM, less what the phases of a token (copy, maximum, sum, exchange, gradient) leave idle with three CTAs per SM.  512 tokens of
 // 128000 bfloat16 logits, a fifth masked, loss and gradient: 69 us with the launch, 3.4 TB/s; the plain kernel took 590.
 // exp is taken as 2^(z scale - c), scale = log2(e) / tau and c = float(top scale), one fused multiply-add and one ex2 per entry;
-// what rounding c loses, kappa = top scale - c, is known in 64 bits and put back into the sum, so the loss does not see it.
+// what rounding c loses, kappa = top scale - c, is known in 64 bits and put back into the sum, so the loss does not see it.  Beyond
+// |c| = 2^27 kappa itself would leave the range of 2^x; there the difference z - top is formed first, one instruction more per entry.
 #include "w4.cuh"
 #include "ptx_sm100.cuh"
 #include <atomic>
@@ -46,10 +47,21 @@ struct Exponent {
   __device__ __forceinline__ Exponent(double tau, float t) : scale(float(1.4426950408889634 / tau)), c(t * scale), top(t) {}
   __device__ double fix() const {
     const double x = (double(c) - double(top) * double(scale)) * 0.69314718055994530942;
-    return !(fabsf(c) <= 3.402823466e38f) ? 1. : fabs(x) < 1e-4 ? 1. + x * (1. + x * (0.5 + x * (1. / 6.))) : exp(x);
+    return fabs(x) < 1e-4 ? 1. + x * (1. + x * (0.5 + x * (1. / 6.))) : exp(x);
   }
   __device__ __forceinline__ float operator()(float z) const { return ex2(fmaf(z, scale, -c)); }
+  __device__ __forceinline__ bool far() const { return !(fabsf(c) < 134217728.f); }
 };
+struct FarExponent {
+  float scale, top;
+  __device__ double fix() const { return 1.; }
+  __device__ __forceinline__ float operator()(float z) const { return ex2((z - top) * scale); }
+};
+// f with the form that serves; the same for every thread of a token.
+template <class F> __device__ __forceinline__ void with_exponent(double tau, float top, F&& f) {
+  const Exponent e(tau, top);
+  if (e.far()) f(FarExponent{e.scale, top}); else f(e);
+}
 
 // Sum / maximum over the block, the same in every thread.  buf: 32 entries.
 template <class V, class F> __device__ V block_reduce(V v, F f, V* buf) {
@@ -190,10 +202,11 @@ template <class T> __global__ void __launch_bounds__(512) distill_plain_kernel(D
       for (int j = threadIdx.x; j < a.n; j += blockDim.x) if (!(listed[j >> 5] >> (j & 31) & 1)) top = fmaxf(top, to_f32(z[j]));
       top = block_reduce(top, Max{}, s.fbuf);
       if (top == -INFINITY) top = 0.f;
-      const Exponent e(a.tau, top);
-      double sum = 0.;
-      for (int j = threadIdx.x; j < a.n; j += blockDim.x) if (!(listed[j >> 5] >> (j & 31) & 1)) sum += e(to_f32(z[j]));
-      outside = float(block_reduce(sum, Add{}, s.buf) * e.fix());
+      with_exponent(a.tau, top, [&](auto e) {
+        double sum = 0.;
+        for (int j = threadIdx.x; j < a.n; j += blockDim.x) if (!(listed[j >> 5] >> (j & 31) & 1)) sum += e(to_f32(z[j]));
+        outside = float(block_reduce(sum, Add{}, s.buf) * e.fix());
+      });
     }
     const Student st(a, l, top, outside);
     if (a.loss || a.stats_out) {
@@ -205,10 +218,11 @@ template <class T> __global__ void __launch_bounds__(512) distill_plain_kernel(D
       }
     }
     if (dz) {
-      const Exponent e(a.tau, top);
-      const float factor = float(outside_factor(a, l, st, outside, weight) * e.fix());
-      for (int j = threadIdx.x; j < a.n; j += blockDim.x)
-        if (!(listed[j >> 5] >> (j & 31) & 1)) dz[j] = from_f32<T>(factor * e(to_f32(z[j])));
+      with_exponent(a.tau, top, [&](auto e) {
+        const float factor = float(outside_factor(a, l, st, outside, weight) * e.fix());
+        for (int j = threadIdx.x; j < a.n; j += blockDim.x)
+          if (!(listed[j >> 5] >> (j & 31) & 1)) dz[j] = from_f32<T>(factor * e(to_f32(z[j])));
+      });
       for (int i = threadIdx.x; i < a.k; i += blockDim.x) if (s.first[i]) dz[s.id[i]] = from_f32<T>(listed_gradient(a, s, l, st, weight, i));
     }
   }
@@ -408,28 +422,29 @@ template <class T> __global__ void __launch_bounds__(kClusterThreads, 3) distill
     main_sync();
 #pragma unroll
     for (int w = 0; w < 8; ++w) m = fmaxf(m, warp_max[w]);
-    const Exponent e(a.tau, m == -INFINITY ? 0.f : m);
-    float sum = threadIdx.x < 2 * V ? e(edge[threadIdx.x]) : 0.f;
+    with_exponent(a.tau, m == -INFINITY ? 0.f : m, [&](auto e) {
+      float sum = threadIdx.x < 2 * V ? e(edge[threadIdx.x]) : 0.f;
 #pragma unroll 2
-    for (int v = threadIdx.x; v < v1 - v0; v += kMainThreads) {
-      float f[V]; unpack<T>(slice[v], f);
+      for (int v = threadIdx.x; v < v1 - v0; v += kMainThreads) {
+        float f[V]; unpack<T>(slice[v], f);
 #pragma unroll
-      for (int i = 0; i < V; ++i) f[i] = e(f[i]);
+        for (int i = 0; i < V; ++i) f[i] = e(f[i]);
 #pragma unroll
-      for (int d = V / 2; d; d /= 2)
+        for (int d = V / 2; d; d /= 2)
 #pragma unroll
-        for (int i = 0; i < d; ++i) f[i] += f[i + d];
-      sum += f[0];
-    }
-    const double mine = warp_reduce(double(sum), Add{});
-    if (lane == 0) warp_sum[warp] = mine;
-    main_sync();
-    if (threadIdx.x == 0) {
-      double total = 0.;
+          for (int i = 0; i < d; ++i) f[i] += f[i + d];
+        sum += f[0];
+      }
+      const double mine = warp_reduce(double(sum), Add{});
+      if (lane == 0) warp_sum[warp] = mine;
+      main_sync();
+      if (threadIdx.x == 0) {
+        double total = 0.;
 #pragma unroll
-      for (int w = 0; w < 8; ++w) total += warp_sum[w];
-      part[0] = m; part[1] = float(total * e.fix());
-    }
+        for (int w = 0; w < 8; ++w) total += warp_sum[w];
+        part[0] = m; part[1] = float(total * e.fix());
+      }
+    });
   }
   if (a.splits > 1) { __syncwarp(); cluster_arrive(); cluster_wait(); }      // also: every CTA has read the listed logits, the gradient may go in their place
   else __syncthreads();
@@ -448,8 +463,7 @@ template <class T> __global__ void __launch_bounds__(kClusterThreads, 3) distill
       outside = float(warp_reduce(share, Add{}));
     }
     const Student st(a, l, top, outside);
-    const Exponent e(a.tau, top);
-    if (lane == 0) { shared_top = top; shared_factor = float(outside_factor(a, l, st, outside, weight) * e.fix()); }
+    if (lane == 0) with_exponent(a.tau, top, [&](auto e) { shared_top = top; shared_factor = float(outside_factor(a, l, st, outside, weight) * e.fix()); });
     __syncthreads();
     if (a.splits > 1) cluster_arrive();              // peers may leave once everybody has read
     if (first && (a.loss || a.stats_out)) {
@@ -474,23 +488,24 @@ template <class T> __global__ void __launch_bounds__(kClusterThreads, 3) distill
     __syncthreads();
     if (a.splits > 1) cluster_arrive();
     if (dz) {
-      const Exponent e(a.tau, shared_top);
       const float factor = shared_factor;
+      with_exponent(a.tau, shared_top, [&](auto e) {
 #pragma unroll 2
-      for (int v = threadIdx.x; v < v1 - v0; v += kMainThreads) {
-        float f[V]; unpack<T>(slice[v], f);
+        for (int v = threadIdx.x; v < v1 - v0; v += kMainThreads) {
+          float f[V]; unpack<T>(slice[v], f);
 #pragma unroll
-        for (int i = 0; i < V; ++i) f[i] = factor * e(f[i]);
-        T* to = dz + head + (v0 + v) * V;
-        if (same) __stcs(reinterpret_cast<uint4*>(to), pack<T>(f));
-        else
+          for (int i = 0; i < V; ++i) f[i] = factor * e(f[i]);
+          T* to = dz + head + (v0 + v) * V;
+          if (same) __stcs(reinterpret_cast<uint4*>(to), pack<T>(f));
+          else
 #pragma unroll
-          for (int i = 0; i < V; ++i) to[i] = from_f32<T>(f[i]);
-      }
-      if (threadIdx.x < 2 * V) {
-        const int j = int(threadIdx.x) < V ? int(threadIdx.x) : tail0 + int(threadIdx.x) - V;
-        if (int(threadIdx.x) < V ? first && j < head : last && j < a.n) dz[j] = from_f32<T>(factor * e(edge[threadIdx.x]));
-      }
+            for (int i = 0; i < V; ++i) to[i] = from_f32<T>(f[i]);
+        }
+        if (threadIdx.x < 2 * V) {
+          const int j = int(threadIdx.x) < V ? int(threadIdx.x) : tail0 + int(threadIdx.x) - V;
+          if (int(threadIdx.x) < V ? first && j < head : last && j < a.n) dz[j] = from_f32<T>(factor * e(edge[threadIdx.x]));
+        }
+      });
       __syncthreads();
     }
   }

@@ -192,8 +192,8 @@ int32_t hyacinB200ProductW4(const hyacinHandle_t* handle, char opW, int32_t M, i
  * weight[t] * dKL_t / dz; weight == NULL means 1; a token with weight 0 is not read and gets loss 0 and a zero gradient.
  * loss, dZ and stats may each be NULL; stats (2 floats per token) is what hyacinB200DistillGrad needs to give the same
  * gradient later, with the weights known by then (NaN for a token that had weight 0).  1e-30 <= tau <= 1e30, 0 <= K <= 1024,
- * 1 <= N <= 2^20; finite
- * logits stay below 2^127 tau in magnitude.  A student probability of zero under a positive teacher probability gives an infinite loss and a
+ * 1 <= N <= 2^20;
+ * finite logits may have any size.  A NaN among a token's logits makes its loss and gradient NaN.  A student probability of zero under a positive teacher probability gives an infinite loss and a
  * finite gradient. */
 int32_t hyacinB200DistillLoss(const hyacinHandle_t* handle, hyacinPrecision_t Ztype, int32_t N, int32_t T, const void* Z, int32_t ldz,
                               int32_t K, const int32_t* ids, const float* teacher, int32_t ldk, double tau, const float* teacherLse,

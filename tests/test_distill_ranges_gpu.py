@@ -49,3 +49,69 @@ def test_nan_in_a_row_spoils_its_loss_and_gradient(hy, n, kind, tail):
     r.dZ.fill_(9.0)
     d = r.grad()
     assert bool(torch.isnan(d[1:8, :n]).all()) and torch.equal(d[0], clean[0])
+
+
+def _by_logarithms(z, ids, teacher, tau, lse):
+    """Loss, gradient and a scale for its errors in 64 bits, by log-sum-exp throughout, for distinct ids.  Probabilities are formed
+    relative to the largest logit: at 1e30 the logarithm of their number would be lost beside it."""
+    u = z.astype(np.float64) / tau
+
+    def lsumexp(a):
+        top = a.max(1, keepdims=True)
+        return top[:, 0] + np.log(np.exp(a - top).sum(1))
+
+    def softmax(a):
+        e = np.exp(a - a.max(1, keepdims=True))
+        return e / e.sum(1, keepdims=True)
+    rows = np.arange(len(z))[:, None]
+    score = teacher.astype(np.float64) / tau
+    logp = score - (lsumexp(score) if lse is None else lse.astype(np.float64))[:, None]
+    p = np.exp(logp)
+    rest = np.zeros(len(z)) if lse is None else np.maximum(0, 1 - p.sum(1))
+    total = lsumexp(u)
+    inside = np.zeros(z.shape, dtype=bool)
+    inside[rows, ids] = True
+    outside = lsumexp(np.where(inside, -np.inf, u))
+    loss = (p * (logp - (u[rows, ids] - total[:, None]))).sum(1)
+    loss += np.where(rest > 0, rest * (np.log(np.where(rest > 0, rest, 1)) - (outside - total)), 0)
+    q = softmax(u)
+    target = np.zeros(z.shape)
+    target[rows, ids] = p
+    share = rest[:, None] * softmax(np.where(inside, -np.inf, u))
+    mass = (p.sum(1) + rest)[:, None]
+    return loss, (q * mass - target - share) / tau, (q * mass + target + share) / tau
+
+
+@pytest.mark.parametrize("n,kind", [(300, "f32"), (5001, "bf16"), (60000, "f16"), (128000, "bf16"), (1 << 20, "f32")])
+@pytest.mark.parametrize("tau,tail", [(1.0, False), (1.0, True), (0.7, True), (3.0, False)])
+def test_logits_of_any_finite_size(hy, n, kind, tau, tail):
+    """Everything outside the list at one mask value, down to the type's lowest; one class far above all others; classes a few
+    places apart far from zero."""
+    torch = _torch()
+    rng = np.random.default_rng(n)
+    t, k = 8, 6
+    top = float(torch.finfo(P.kinds()[kind][0]).max)
+    size = (lambda v: min(v, top))
+    z, ids, teacher, lse = _problem(rng, n, t, k, kind, tau, False)
+    if tail:                                         # the rest weighs a third of the listed classes
+        lse = (np.log(np.exp(teacher.astype(np.float64) / tau).sum(1)) + np.log(4 / 3)).astype(np.float32)
+    inside = np.zeros(z.shape, dtype=bool)
+    inside[np.arange(t)[:, None], ids] = True
+    for row, value in ((1, 1e9), (2, 1e10), (3, 1e30), (4, top)):
+        z[row] = np.where(inside[row], z[row], -size(value))
+    z[5, np.flatnonzero(~inside[5])[n // 3]] = size(1e10)
+    z[6, np.flatnonzero(~inside[6])[n // 2]] = size(1e30)
+    z[7] = np.where(rng.random(n) < 0.5, 3e9, 3e9 + 256) if kind == "f32" else z[7]
+    z = P.round_to(z, kind)
+    r = Run(hy, z, ids, teacher, tau, lse, None, kind)
+    d = r.step()
+    want_loss, want, scale = _by_logarithms(z, ids, teacher, tau, lse)
+    loss, g = r.loss.double().cpu().numpy(), d[:, :n].double().cpu().numpy()
+    fits = np.abs(want_loss) < np.finfo(np.float32).max
+    assert np.isfinite(loss[fits]).all() and np.isposinf(loss[~fits]).all()
+    assert (np.abs(loss - want_loss)[fits] <= (P.HALF_STEP["f32"] * np.abs(want_loss) + 4 * TERM)[fits]).all()
+    tol = P.HALF_STEP[kind] * np.abs(want) + 4 * TERM * scale + P.TINY[kind]
+    assert np.isfinite(g).all() and (np.abs(g - want) <= tol).all(), (np.abs(g - want) / tol).max(axis=1)
+    once = r.dZ.clone()
+    r.dZ.fill_(9.0)
+    assert torch.equal(r.grad(), once)
