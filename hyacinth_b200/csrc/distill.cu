@@ -1,7 +1,7 @@
 // Distillation loss against a teacher's top logits, and its gradient.
 //
 // Per token, with u = z / tau and the list i = 1 .. K of classes c_i with teacher logits t_i:
-//     p_i = exp(t_i / tau - teacherLse), p_r = max(0, 1 - sum p)   or, without teacherLse, p_i = softmax over the list, p_r = 0
+//     p_i = exp(t_i / tau - teacherLse), p_r = max(0, 1 - sum p), 0 when every class is listed   or, without teacherLse, p_i = softmax over the list, p_r = 0
 //     lse = log sum_j exp u_j,  lse_r = log sum over the classes outside the list
 //     KL  = sum_i p_i (log p_i - (u_{c_i} - lse)) + p_r (log p_r - (lse_r - lse))
 //     dKL/dz_j = (q_j mass - P_j) / tau                        listed: P_j = sum of its p_i, mass = sum p + p_r
@@ -124,18 +124,20 @@ template <class T> __device__ Listed load_list(const DistillArgs& a, int64_t tok
   }
   sum = block_reduce(sum, Add{}, s.buf);
   Listed r;
-  r.rest = a.teacher_lse ? fmax(0., 1. - sum) : 0.;
-  r.mass = sum + r.rest;
   r.top = block_reduce(student, Max{}, s.buf);
-  double e = 0.;
+  double e = 0.; int classes = 0;
   for (int i = threadIdx.x; i < a.k; i += blockDim.x) {
     int first = s.id[i] >= 0; double ps = 0.;
     for (int j = 0; j < a.k; ++j) if (s.id[j] == s.id[i]) { ps += s.p[j]; if (j < i) first = 0; }
     s.first[i] = first; s.psum[i] = ps;
     s.e[i] = s.id[i] >= 0 ? relative_exp(s.z[i], a.inv_tau, r.top) : 0.;
     if (first) e += s.e[i];
+    classes += first;
   }
   r.sum = block_reduce(e, Add{}, s.buf);
+  r.rest = a.teacher_lse ? fmax(0., 1. - sum) : 0.;
+  if (a.k >= a.n && int(block_reduce(double(classes), Add{}, s.buf)) == a.n) r.rest = 0.;      // what sum p leaves of 1 is rounding
+  r.mass = sum + r.rest;
   __syncthreads();
   return r;
 }
@@ -338,10 +340,14 @@ template <class T> __device__ Listed list_by_warp(const DistillArgs& a, int64_t 
       for (int j = 0; j < a.k; ++j) if (s.id[j] == s.id[i]) { ps += s.p[j]; if (j < i) first = 0; }
       s.first[i] = first; s.psum[i] = ps;
     }
-  double e = 0.;
-  for (int i = lane; i < a.k; i += 32) if (s.first[i]) e += s.e[i];
+  double e = 0.; int classes = 0;
+  for (int i = lane; i < a.k; i += 32) if (s.first[i]) { e += s.e[i]; ++classes; }
   r.sum = warp_reduce(e, Add{});
-  if (a.teacher_lse) { r.rest = fmax(0., 1. - sum); r.mass = sum + r.rest; }
+  if (a.teacher_lse) {
+    r.rest = fmax(0., 1. - sum);
+    if (a.k >= a.n && warp_reduce(classes, Add{}) == a.n) r.rest = 0.;      // what sum p leaves of 1 is rounding
+    r.mass = sum + r.rest;
+  }
   else { r.rest = 0.; r.mass = sum > 0. ? 1. : sum == 0. ? 0. : sum; }
   return r;
 }

@@ -187,7 +187,8 @@ int32_t hyacinB200ProductW4(const hyacinHandle_t* handle, char opW, int32_t M, i
  * probabilities.  With u = z / tau, q = softmax(u) and p = softmax(teacher / tau) over the listed entries,
  *     KL_t = sum_i p_i (log p_i - log q_i).
  * teacherLse != NULL (T floats: log-sum-exp of ALL the teacher's logits over tau) makes p the teacher's true probabilities and
- * everything that is not listed one more outcome: KL_t += p_r log(p_r / q_r), p_r = max(0, 1 - sum p_i), q_r = sum of q outside.
+ * everything that is not listed one more outcome: KL_t += p_r log(p_r / q_r), p_r = max(0, 1 - sum p_i), q_r = sum of q outside; p_r = 0
+ * when every class is listed.
  * loss[t] = weight[t] * KL_t and dZ (N x T, type Ztype, leading dimension lddz; may be Z itself with lddz == ldz) =
  * weight[t] * dKL_t / dz; weight == NULL means 1; a token with weight 0 is not read and gets loss 0 and a zero gradient.
  * loss, dZ and stats may each be NULL; stats (2 floats per token) is what hyacinB200DistillGrad needs to give the same

@@ -115,3 +115,36 @@ def test_logits_of_any_finite_size(hy, n, kind, tau, tail):
     once = r.dZ.clone()
     r.dZ.fill_(9.0)
     assert torch.equal(r.grad(), once)
+
+
+@pytest.mark.parametrize("n,repeat", [(1, False), (5, False), (64, False), (1000, False), (40, True)])
+def test_a_list_of_every_class_leaves_no_rest(hy, n, repeat):
+    """With every class listed nothing is left to be one more outcome, however sum p rounds: the loss is that of the listed classes."""
+    torch = _torch()
+    rng = np.random.default_rng(n)
+    t = 12
+    z, ids, teacher, lse = _problem(rng, n, t, n, "f32", 1.0, True)
+    if repeat:                                       # a class twice, none left out; another list leaves one out
+        ids = np.concatenate([ids, ids[:, :1]], axis=1)
+        teacher = np.concatenate([teacher, teacher[:, :1] - 30], axis=1).astype(np.float32)
+        ids[1, 3] = ids[1, 2]
+    lse = lse + np.float32(1e-6) * rng.integers(-1, 2, t).astype(np.float32)
+    r = Run(hy, z, ids, teacher, 1.0, lse, None, "f32")
+    d = r.step()
+    loss, g = r.loss.double().cpu().numpy(), d.double().cpu().numpy()
+    for row in range(t):
+        if repeat and row == 1:
+            want, grad, _ = P.distill(z[1:2], ids[1:2], teacher[1:2], 1.0, lse[1:2], None)
+            assert abs(loss[1] - want[0]) <= 4 * TERM + 2.0 ** -24 * want[0]
+            continue
+        u = z[row] - z[row].max()
+        logq = u - np.log(np.exp(u).sum())
+        p = np.zeros(n)
+        listed = np.exp(teacher[row].astype(np.float64) - float(lse[row]))
+        np.add.at(p, ids[row], listed)
+        want = (listed * (teacher[row].astype(np.float64) - float(lse[row]) - logq[ids[row]])).sum()
+        assert abs(loss[row] - want) <= 4 * TERM + 2.0 ** -24 * abs(want), (row, loss[row], want)
+        assert (np.abs(g[row] - (np.exp(logq) * p.sum() - p)) <= 4 * TERM * (np.exp(logq) + p) + 2.0 ** -24).all()
+    once = d.clone()
+    r.dZ.fill_(9.0)
+    assert torch.equal(r.grad(), once)
