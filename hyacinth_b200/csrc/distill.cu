@@ -12,10 +12,11 @@
 //
 // Two kernels.  distill_cluster_kernel keeps a token's logits in the shared memory of a cluster of one to eight CTAs: they are read
 // from DRAM once, with bulk copies, and the gradient is written from there; one exchange of (maximum, sum) per CTA is all the
-// communication.  Slices of at most 72 KiB leave three CTAs per SM, whose loads, arithmetic and stores overlap.
+// communication.  Several CTAs per SM (see kSliceBytes) overlap their loads, arithmetic and stores.
 // distill_plain_kernel (one block per token, passes over global memory) takes rows that do not fit a cluster.
-// Bound: DRAM, less what the phases of a token (copy, maximum, sum, exchange, gradient) leave idle with three CTAs per SM.  512 tokens of
-// 128000 bfloat16 logits, a fifth masked, loss and gradient: 69 us with the launch, 3.4 TB/s; the plain kernel took 590.
+// Bound: the phases of a token (copy, maximum, sum, exchange, gradient), which three CTAs per SM do not hide: 34 % of DRAM, 48 % of the issue
+// slots and of the exponentials' pipe.  512 tokens of 128000 bfloat16 logits, a fifth masked, loss and gradient: 70 us with the launch,
+// 3.4 TB/s; the plain kernel took 590.
 // exp is taken as 2^(z scale - c), scale = log2(e) / tau and c = float(top scale), one fused multiply-add and one ex2 per entry;
 // what rounding c loses, kappa = top scale - c, is known in 64 bits and put back into the sum, so the loss does not see it.  Beyond
 // |c| = 2^27 kappa itself would leave the range of 2^x; there the difference z - top is formed first, one instruction more per entry.
@@ -518,7 +519,9 @@ template <class T> __global__ void __launch_bounds__(kClusterThreads, 3) distill
   if (a.splits > 1) cluster_wait();
 }
 
-// Slices of at most 72 KiB where eight CTAs allow it (three CTAs per SM), otherwise what one CTA per SM takes.
+// Slices of at most 72 KiB where eight CTAs allow it, otherwise what one CTA per SM takes.  With the list and 8 KiB of tables three CTAs fit
+// an SM up to slices of some 64 KiB and two beyond, which still beat three or four of half the slice, whose phases are as long: 512
+// x 131072 bfloat16 (64 KiB) 96 us, in twice the CTAs 113; 1024 x 32768 (64 KiB) 49 against 56; 1024 x 36000 (70 KiB) 51 against 58.
 constexpr int kSliceBytes = 72 * 1024, kSmemMost = 216 * 1024;
 
 template <class T> cudaError_t raise_limit(const hyacinHandle_t* handle, T* kernel, std::atomic<uint64_t>& ready) {

@@ -50,8 +50,9 @@ extern "C" int32_t hyacinB200ProductW4(const hyacinHandle_t* handle, char opW, i
   }
   const int per = trans ? product_stream_vectors(Xtype, a) : 0;
   if (Xtype == HYACIN_F32) {
-    // A pass of the streaming kernel over 4096 x 4096 takes 10 us (four vectors), the tiled kernel 37 us for up to 16 vectors, 49 for up to 32; with
-    // few columns the streaming kernel leaves SMs idle and the tiled one splits the rows (16384 x 200 times 4: 49 against 16 us).
+    // Five passes of the streaming kernel are where it meets the tiled one: 4096 x 4096 times 16, four passes, 39.6 against 42.5 us, times 20,
+    // five, 49.3 against 49.0, six would be 59 against 49.7; 8192 x 4096 times 10, five of two vectors, 62 against 81; 4096 x 16384 times 20 99
+    // against 182.  With few columns the streaming kernel leaves SMs idle and the tiled one splits the rows (16384 x 200 times 4: 49 against 16).
     const bool filled = N >= (T <= per ? 2 : 8) * handle->DeviceSMs;
     if (per > 0 && T <= 5 * per && filled) return launch_product_stream(handle, fn, Xtype, a);
     return launch_product_single(handle, fn, trans, a);

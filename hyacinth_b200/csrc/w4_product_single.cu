@@ -1,15 +1,17 @@
 // Products with a 4-bit weight matrix in single precision where the streaming kernel does not serve: opW 'N', many vectors, very long x.
 //
-// Y (out x T) = A X, A = Wq^T or Wq, in 32 bits throughout.  A block of 128 threads computes 128 outputs x TOK vectors: steps of 32 along the sum
+// Y (out x T) = A X, A = Wq^T or Wq, in 32 bits throughout: scale times code (or, for few vectors, scale times x) is rounded to 32 bits, then the
+// sums.  A block of 128 threads computes 128 outputs x TOK vectors: steps of 32 along the sum
 // bring the dequantised weights and x to shared memory as floats, a thread holds 8 x TOK / 8 sums.  A step's sums start from
 // zero and are then added to the total, so no term passes through more than 32 + K / 32 additions.  The next step's words are on their way
 // in registers meanwhile.  The correction V (U^T X) is more steps of the same sum with mid = U^T X as x, and mid itself the same
 // kernel over a plain matrix.  Few tiles: a cluster of up to 8 blocks splits the steps, sums joined in a fixed order.
 // Bound: the floating-point pipe, 128 multiply-adds per clock and SM (72 TFLOP/s at 1.9 GHz), and shared memory beside it: four 16-byte loads, sixteen
 // wavefronts, per 64 multiply-adds of a warp.  8 x 8 sums per thread need half the loads of 8 x 4 (276 -> 236 us below); two blocks per SM
-// leave eight warps to cover what remains.  Measured, 4096 x 4096 with segments of 64 rows: opW 'N', 16 vectors 37 us, 32 43 us, 64 64 us,
-// 256 236 us (36 TFLOP/s); opW 'T', 256 vectors 252 us; 200 x 32768 times 32, opW 'N' (two tiles, 1024 steps) 42 us, 263 without the second split.
-// The kernel for few vectors takes 42 us for eight, two passes of it, where this one takes 37.
+// leave eight warps to cover what remains: 32 % of the multiply pipe and 43 % of the issue slots for 256 vectors.  Measured, 4096 x 4096 with
+// segments of 64 rows: opW 'N', 16 vectors 37 us, 32 44 us, 64 63 us, 256 234 us (37 TFLOP/s); opW 'T', 16 vectors 42 us, 256 255 us;
+// 200 x 32768 times 32, opW 'N' (two tiles, 1024 steps) 45 us, 263 without the second split.  The kernel for few vectors would take two
+// passes of 21 us for eight, where this one takes 36.
 #include "w4_product.h"
 #include <algorithm>
 
@@ -205,7 +207,8 @@ template <Mode MODE, int TOK> __global__ void __launch_bounds__(kThreads, 2) pro
 // Few vectors, opW 'N': a block of 256 threads takes 128 rows, thread (word, lane) the eight rows of a word in every 16th column, for up to
 // four vectors; x times the scale is formed once per word.  A cluster of up to eight such blocks splits the columns; sums meet
 // in shared memory, in a fixed order.
-// Bound: the floating-point pipe, 8 conversions and 32 multiply-adds per word and four vectors; 4096 x 4096, four vectors: 24 us.
+// Bound: the latency of plain loads, one scale and up to four x for each word, four columns of a thread in flight; 35 % of the issue slots
+// and 19 % of the multiply pipe are used.  4096 x 4096, one vector 21 us, four 22.
 constexpr int kFew = 4, kFewLanes = 16, kFewThreads = 16 * kFewLanes;
 __device__ __forceinline__ float ld_cluster(const float* at, uint32_t rank) {
   uint32_t remote; float v;

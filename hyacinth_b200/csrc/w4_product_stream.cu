@@ -16,12 +16,10 @@
 // lane's four code pairs of a word meet the lane's 16 bytes of x for those eight rows, read from shared memory in their natural
 // order.  Six more warps fetch scales and zero points, coalesced along a table row, into the
 // same ring, and one adds the partial sums of the multiplying warps.
-// Bound.  DRAM, at 23 bytes per clock and SM: 710 cycles for a stage of 16 KiB, for which the extraction takes 450 cycles of the
-// integer pipe (7 instructions per eight codes at half rate) and the matrix pipe 256 per eight vectors.  Measured, matrices cycled
-// through more than the L2: bfloat16 4096 x 16384, one vector 14.7 us (2.4 TB/s), eight 17.1 us; half 8192 x 16384 with zero points for
-// every 64 rows 25.6 us (2.9 TB/s; 54 % of the issue slots used; two instructions less per word, with the nibbles of the second and
-// fourth pair left in place, made it 26.5); 4096 x 4096 6.4 us, of which a start
-// from nothing (launch, x and its sums, the first copies) takes four.
+// Bound.  Latency: barrier, shared load, extraction, matrix instruction and scaling follow one another in each of the 16 warps.  Half 8192 x
+// 16384 with zero points for every 64 rows uses 57 % of the issue slots, 15 % of the matrix pipe and 32 % of DRAM.  Measured, matrices
+// cycled through more than the L2: that case 26.3 us (2.8 TB/s; 22.9 with segments of 128 rows); bfloat16 4096 x 16384, one vector 15.4 us
+// (2.2 TB/s), eight 16.6 us; 4096 x 4096 7.0 us.  The subtraction of the offsets costs 0 to 5 % of these.
 #include "w4_product.h"
 #include "ptx_sm100.cuh"
 #include <algorithm>
@@ -56,7 +54,8 @@ struct StreamParams {
 
 struct StreamBars { uint64_t full[kMaxRing], empty[kMaxRing], joint_full[kJoints], joint_empty[kJoints]; uint32_t abort_flag; };
 
-// Two codes each: offset + q as extracted.
+// Two codes each: offset + q as extracted, by joining the code's bits to the exponent of a number whose last places are whole (the classic
+// conversion of integers, e.g. Warren, Hacker's Delight, 2003; for 4-bit weights in half Kim et al., arXiv:2211.10017, 2022).
 template <bool HALF> struct Codes;
 template <> struct Codes<true> {       // 0x6400 | q = 1024 + q
   static constexpr uint32_t kBits = 0x64006400u; static constexpr int kOffset = 1024;

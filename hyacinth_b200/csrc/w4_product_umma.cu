@@ -19,12 +19,13 @@
 // Few tiles: a cluster of up to 8 CTAs splits the K steps of one tile and adds the partial sums through distributed shared memory
 // in a fixed order.
 // Rounding: s (q - zero) has up to 15 significant bits (8 of s, 5 of q for bfloat16) and is rounded to the operand type, which
-// is what the matrix instruction takes; one half step, independent per weight, of the size of the rounding of Y itself.
-// Bound: the hand-overs between the roles.  A step takes 750 cycles with 32 tokens, of which the dequantising warps fill 250 and the tensor
-// pipe 260, and 1140 with 256, of which the pipe fills 1030; the first step's operand is there after 5700 cycles (copies, scales,
-// dequantising, each behind the other).  Measured, matrices cycled through more than the L2: 4096 x 16384 bfloat16 times 32 tokens 21.3 us
-// (1.7 TB/s), 128 tokens 24.3 us (707 TFLOP/s), 256 tokens 32.7 us (1050 TFLOP/s, 0.66 of measured); half with segments of 64 rows
-// and zero points, opW 'N', 64 tokens 27.0 us.  Without the code stream the first of these takes 1.6 us less, without dequantising 2 us.
+// is what the matrix instruction takes; one half step, independent per weight, of the size of the rounding of Y itself (error against
+// 64 bits 0.0021 instead of the 0.0017 of that rounding alone for bfloat16, 0.00027 instead of 0.00021 for half).  A weight beyond 65504 is an
+// infinity for half.
+// Bound: the hand-overs between the roles: 4096 x 16384 bfloat16 times 32 tokens keeps the tensor pipe busy for 9 % of the time, the issue
+// slots for 41 % and DRAM for 16 %, times 256 tokens for 47, 33 and 10 %.  Measured, matrices cycled through more than the L2: 32 tokens 22.0
+// us (1.6 TB/s), 128 tokens 25.0 us (690 TFLOP/s), 256 tokens 33.0 us (1040 TFLOP/s, 0.65 of measured); half with segments of 64 rows and
+// zero points, opW 'N', 64 tokens 27.4 us.  The correction, rank 64, adds 5.0 us to the first of these and 7.5 to the third (half: 8 and 10).
 #include "w4_product.h"
 #include "ptx_sm100.cuh"
 #include <algorithm>
@@ -172,7 +173,7 @@ __device__ __forceinline__ uint32_t rows_only(uint32_t w, int left, uint32_t zer
 
 // Scale and zero point of one (column, segment), as the pairs that the dequantisation multiplies and subtracts.
 template <class T> struct Scale;
-// half: 0x6400 | q is 1024 + q and 0x6400 | 16 q is 1024 + 16 q, both exact
+// half: 0x6400 | q is 1024 + q and 0x6400 | 16 q is 1024 + 16 q, both exact (published for 4-bit weights by Kim et al., arXiv:2211.10017, 2022)
 template <> struct Scale<__half> {
   uint16_t bits = 0; int zero = 0;
   struct Ready { __half2 s, low, high; };

@@ -1,8 +1,9 @@
 // 4-bit form of a weight matrix: per (column, segment) scale s = max|w| / 7 (or (hi - lo) / 15 with a zero point), codes
 // q = rint(w / s) + zero, and the residual w - s (q - zero) that a low-rank fit takes.
 //
-// The quotient decides a whole number, so it is taken in 64 bits: w and s carry at most 24 bits, a quotient that is not
-// exactly a half differs from it by at least 2^-28 relative, and rint of the 64-bit quotient is that of the exact one.
+// The quotient decides a whole number, so it is rounded as if it were exact.  In 64 bits that needs no care: w and s carry at most 24
+// bits, a quotient that is not exactly a half differs from it by at least 2^-28 relative, and rint of the 64-bit quotient is that of the exact
+// one.  Scales and quotients of ordinary size are done in 32 bits with one correction step, as said at rounded_quotient and quotient_bits.
 #include "w4.cuh"
 #include <algorithm>
 
@@ -40,7 +41,7 @@ __device__ __noinline__ float quotient_in_64_bits(float v, float s) { return flo
 __device__ __forceinline__ float reciprocal(float s) { float r; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s)); return r; }
 
 // x / by for 7 and 15.  A product with the rounded reciprocal is within a last place, and one step corrects it (Markstein, IBM J. Res. Dev.
-// 34, 1990; all 2^23 fractions compared with the division on the CPU); the range keeps the remainder's last place above the smallest number.
+// 34, 1990; a test compares all 2^23 fractions with the division); the range keeps the remainder's last place above the smallest number.
 __device__ __forceinline__ float divided(float x, float by) {
   if (!(x > 1e-28f && x < 1e30f)) return __fdiv_rn(x, by);
   const float inverse = by == 7.f ? 1.f / 7.f : 1.f / 15.f, q = __fmul_rn(x, inverse);
@@ -87,9 +88,10 @@ __device__ __forceinline__ float largest_of(float a, float b, float c) { float d
 // segment's lanes are neighbours and find its extremes with shuffles, so W is read once and everything stays in registers.
 // Rows that are not 16-byte aligned pass through shared memory, so that DRAM sees whole lines all the same.
 // A warp walks down the columns of its row group with the next columns' loads in flight.
-// Bound: DRAM (read W, write half a byte per weight, and 4 bytes of residual where asked for); instruction issue for matrices of a few
-// columns per warp.  Measured: 16384 x 4096 bfloat16 with residual 77 us, 5.6 TB/s; 4096 x 4096 bfloat16 14.7 us, 2.9 TB/s; 8190 x 2049
-// float, rows off their alignment, zero points and residual 31 us, 4.6 TB/s (23.7 us aligned).
+// Bound: with residual (4 more bytes written per weight) DRAM and issue, 60 and 64 % of either; without it instruction issue, 78 % of the slots
+// beside 32 % of DRAM (4096 x 16384 bfloat16), and for small matrices the start and end of a walk over few columns.  Measured: 16384 x
+// 4096 bfloat16 with residual 77 us, 5.6 TB/s; 4096 x 4096 bfloat16 15.4 us, 2.7 TB/s; 8190 x 2049 float, rows off their alignment, zero
+// points and residual 31 us, 4.6 TB/s (23.7 us aligned).
 template <class T, class S, bool SYMMETRIC, bool WIDE> __device__ __forceinline__ void quantize_columns(const QuantizeArgs& a, int r_aligned, float* turn) {
   constexpr int kWords = int(sizeof(T)) * 8 / 16, kDepth = WIDE && sizeof(T) == 2 ? 2 : 1;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;

@@ -158,24 +158,30 @@ int32_t hyacinB200PivotedCholesky(const hyacinHandle_t* handle, double eps, int3
  *
  * All calls are asynchronous on handle->cudaStream, may be captured into a CUDA graph, and return 0, -1 for arguments
  * they do not take (message on stderr, nothing launched), or -3 when CUDA refused a launch or an allocation.  The handle
- * has to come from hyacinCreate on the device that is current.  Scratch comes from handle->mempool in stream order.  Outputs do not overlap inputs
- * unless stated.  M, N and T of the products are at most 2^31 - 256, and pointers lie on a boundary of their type.  Results do not depend on timing: there are no atomic sums. */
+ * has to come from hyacinCreate on the device that is current.  Scratch comes from handle->mempool in stream order.  Outputs do not
+ * overlap inputs unless stated.  M, N and T of the products are at most 2^31 - 256, and pointers lie on a boundary of their type.
+ * Results do not depend on timing: there are no atomic sums. */
 #define HYACIN_B200_BF16 ((hyacinPrecision_t)14)      /* within the values that the enumeration's type can hold, 0 .. 15 */
 
 /* 4-bit form of W (type Wtype, leading dimension ldw).  scales has type Stype.  zeros == NULL: symmetric,
  * s = Stype(max|w| / 7), q = clamp(rint(w / s), -7, 7) + 8.  Otherwise lo = min(0, min w), hi = max(0, max w),
  * s = Stype((hi - lo) / 15), zero = clamp(rint(-lo / s), 0, 15), q = clamp(rint(w / s) + zero, 0, 15).  Quotients are rounded as if
- * exact, ties to even.  A scale of zero gives q = zero (8, or 0).  A segment that holds a NaN or an infinity gets a NaN scale and
- * q = zero.  R (float, ldr >= M) receives W - Wq when it is not NULL. */
+ * exact, ties to even.  A scale of zero gives q = zero (8, or 0), one beyond the largest number of Stype is infinite and gives the same.  A
+ * segment that holds a NaN or an infinity gets a NaN scale and q = zero.  R (float, ldr >= M) receives W - Wq when it is not NULL. */
 int32_t hyacinB200QuantizeW4(const hyacinHandle_t* handle, hyacinPrecision_t Wtype, int32_t M, int32_t N, const void* W, int32_t ldw,
                              int32_t segM, hyacinPrecision_t Stype, uint8_t* codes, int64_t ldq, void* scales, uint8_t* zeros,
                              int32_t lds, float* R, int32_t ldr);
 
 /* opW 'T': Y (N x T) = Wq^T X + V (U^T X), X (M x T).   opW 'N': Y (M x T) = Wq X + U (V^T X), X (N x T), the gradient of
  * the former to its input.  U is M x rank, V is N x rank; rank 0 leaves the correction out.  scales, X, Y, U and V have type
- * Xtype.  Any T >= 0.  Sums are held in 32 bits and Y is rounded once.  The 16-bit types round the
- * scaled weights to 16 bits before the product for opW 'N' and, but for some scale tables, for T > 8; single precision rounds
- * nothing but its sums.  rank <= 2^20. */
+ * Xtype.  Any T >= 0.  rank <= 2^20.  Sums are held in 32 bits and Y is rounded once.  Besides:
+ *   - the 16-bit types round the scaled weights s (q - zero) to 16 bits before the product for opW 'N' and, but for some scale tables,
+ *     for T > 8 (half: weights beyond 65504 become infinite there); for opW 'T' and few vectors they are exact, and it is (q - zero) x that
+ *     must stay below 2^128 before the scale comes in;
+ *   - U^T X (V^T X) is held in 32 bits; where the scaled weights are rounded, bfloat16 rounds it to 16 bits, half does not;
+ *   - single precision rounds s (q - zero), or s x, to 32 bits; for opW 'T' and few vectors x below 2^-110 in magnitude loses places.
+ * An infinite entry of X gives infinities of the weights' signs, NaN where a weight is zero.  An infinite entry of the factor applied last
+ * (V for 'T', U for 'N') may give NaN for an infinity. */
 int32_t hyacinB200ProductW4(const hyacinHandle_t* handle, char opW, int32_t M, int32_t N, int32_t T, hyacinPrecision_t Xtype,
                             const uint8_t* codes, int64_t ldq, int32_t segM, const void* scales, const uint8_t* zeros, int32_t lds,
                             const void* X, int32_t ldx, int32_t rank, const void* U, int32_t ldu, const void* V, int32_t ldv,
@@ -193,9 +199,8 @@ int32_t hyacinB200ProductW4(const hyacinHandle_t* handle, char opW, int32_t M, i
  * weight[t] * dKL_t / dz; weight == NULL means 1; a token with weight 0 is not read and gets loss 0 and a zero gradient.
  * loss, dZ and stats may each be NULL; stats (2 floats per token) is what hyacinB200DistillGrad needs to give the same
  * gradient later, with the weights known by then (NaN for a token that had weight 0).  1e-30 <= tau <= 1e30, 0 <= K <= 1024,
- * 1 <= N <= 2^20;
- * finite logits may have any size.  A NaN among a token's logits makes its loss and gradient NaN.  A student probability of zero under a positive teacher probability gives an infinite loss and a
- * finite gradient. */
+ * 1 <= N <= 2^20; finite logits may have any size.  A NaN among a token's logits makes its loss and gradient NaN.  A student
+ * probability of zero under a positive teacher probability gives an infinite loss and a finite gradient. */
 int32_t hyacinB200DistillLoss(const hyacinHandle_t* handle, hyacinPrecision_t Ztype, int32_t N, int32_t T, const void* Z, int32_t ldz,
                               int32_t K, const int32_t* ids, const float* teacher, int32_t ldk, double tau, const float* teacherLse,
                               const float* weight, float* loss, float* stats, void* dZ, int32_t lddz);
