@@ -240,3 +240,64 @@ def test_a_handle_that_was_never_created_is_refused(hy, capfd):
     assert lib.hyacinB200DistillLoss(h, api.F32, 4, 1, y, 4, 0, None, None, 0, 1.0, None, None, st, None, None, 0) == -1
     assert lib.hyacinB200DistillGrad(h, api.F32, 4, 1, y, 4, 0, None, None, 0, 1.0, None, None, st, y, 4) == -1
     assert capfd.readouterr().err.count("hyacinCreate") == 7
+
+
+# ---- the same beside other shapes ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("op,t,rank,m,n", [("T", 20, 7, 501, 203), ("T", 300, 33, 500, 203), ("N", 20, 7, 203, 501), ("N", 300, 65, 203, 500), ("T", 20, 1000, 256, 130),
+                                           ("N", 12, 700, 130, 256), ("T", 40, 64, 512, 5000), ("T", 3, 20, 501, 203)])
+def test_correction_of_odd_shapes(hy, op, t, rank, m, n):
+    """Factors off their alignment, several tiles of tokens, ranks of many steps, more tiles than a cluster shares."""
+    for kind in ("f16", "bf16"):
+        _correction_only(hy, op, kind, rank, t, (3, 1, -12), m, n)
+        _correction_only(hy, op, kind, rank, t, (-24, -8, 9), m, n)
+
+
+@pytest.mark.parametrize("t", [9, 13, 16])
+def test_vectors_beside_a_scattered_table_are_exact(hy, t):
+    """Tables whose rows cannot be fetched a block at a time stream up to sixteen vectors, with the same promise."""
+    rng = np.random.default_rng(t)
+    m, n, seg = 500, 150, 32
+    for kind, bits in (("f16", 10), ("bf16", 7)):
+        codes, scales, zp = _problem(rng, m, n, seg, kind, True)
+        scales[:] = 1
+        x = 1 + rng.integers(0, 1 << bits, (t, m)) * 2.0 ** -bits
+        got = _run_product(hy, "T", m, n, t, kind, seg, codes, scales, zp, x, pads=(1, 0, 0))
+        assert np.array_equal(got, P.round_to(x @ P.values(codes, scales, zp, seg).T, kind))
+
+
+@pytest.mark.parametrize("op,t", [("T", 20), ("N", 20)])
+def test_half_with_a_correction_captured_and_replayed(op, t):
+    """The correction's parts, scratch of the call, in two graphs replayed on two streams at once."""
+    torch = _torch()
+    from hyacinth_b200 import api
+    rng = np.random.default_rng(t)
+    m, n, rank, seg = 640, 384, 24, 128
+    inn, out = (m, n) if op == "T" else (n, m)
+    codes, scales, _ = _problem(rng, m, n, seg, "f16", False)
+    Q, S = torch.from_numpy(P.pack(codes, m // 2)).cuda(), _dev(scales, "f16")
+    u, v = P.round_to(0.1 * rng.standard_normal((rank, m)), "f16"), P.round_to(0.1 * rng.standard_normal((rank, n)), "f16")
+    U, V = _dev(u, "f16"), _dev(v, "f16")
+    xs = [P.round_to(rng.standard_normal((t, inn)), "f16") for _ in range(2)]
+    X, Y = [_dev(x, "f16") for x in xs], [torch.zeros((t, out), dtype=torch.float16, device="cuda") for _ in range(2)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    handles, graphs = [api.Hyacin(stream=s.cuda_stream) for s in streams], []
+    for i in range(2):
+        with torch.cuda.stream(streams[i]):
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=streams[i]):
+                assert handles[i].product_w4(op, m, n, t, api.F16, Q, m // 2, seg, S, None, m // seg, X[i], inn, rank, U, m, V, n, Y[i], out) == 0
+            graphs.append(g)
+    for _ in range(4):
+        for y in Y:
+            y.zero_()
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for i in range(2):
+            _check_product(_back(Y[i], out), op, m, n, "f16", seg, codes, scales, None, xs[i], u, v)
+    del graphs, g
+    for h in handles:
+        h.destroy()
